@@ -297,6 +297,107 @@ pkv_status pkv_paged_attention_auto_fp8(
     int B, int q_rows, int out_rows, int Hq, int Hkv, int head_dim,
     int physical_pages, int page_size, int max_pages, void* stream);
 
+/* ---- e4m3 K/V cache with block scales ----
+ * pkv_paged_attention_auto over pools of e4m3 values ([P][Hkv][page][128])
+ * with one float scale per block of block_tokens tokens and head:
+ * K = k_scales[p][h][t / block_tokens] * value, V likewise; scales are
+ * [P][Hkv][page_size / block_tokens], block_tokens a multiple of 16 that
+ * divides page_size.  A scale is positive and finite, or zero for a block of
+ * zeros.  q and output are fp16 or bf16 (dtype).  Pages and scales of tokens
+ * past a row's length are never used, whatever they hold.  No counterpart in
+ * the reference. */
+pkv_status pkv_paged_attention_auto_fp8_block(
+    const void* q_source, const void* k_pages, const void* v_pages, const float* k_scales,
+    const float* v_scales, const int32_t* block_table, const int32_t* seq_lens,
+    const int32_t* q_indices, const int32_t* out_indices, void* output,
+    void* workspace, size_t workspace_bytes, int32_t* merge_counters,
+    int B, int q_rows, int out_rows, int Hq, int Hkv, int head_dim,
+    int physical_pages, int page_size, int max_pages, int block_tokens,
+    pkv_dtype dtype, void* stream);
+
+/* ---- Prompts ----
+ * A prompt (or a chunk of one) enters the cache in two calls and is attended
+ * to in a third: pkv_prompt_slots gives its tokens places, pkv_kv_write or
+ * pkv_kv_write_fp8_block puts its K/V there, pkv_prompt_attention computes its
+ * rows from the same packed K/V.  Tokens of all rows are packed one row after
+ * another; cu_seqlens[b] is row b's first token.  No counterpart in the
+ * reference, whose pools are pre-filled
+ * (tests/benchmark_serving_trace.py:253-263). */
+
+/* Block tables and slot map of a batch, from its lengths.  Row b holds
+ * cached_lens[b] tokens already (its first ceil(cached / page_size)
+ * block_table entries are mapped) and gets new_lens[b] more.  The rows, in
+ * order, take the pages they open from the top of the free stack
+ * (free_pages[*free_count - 1], [*free_count - 2], ...), as pkv_kv_append
+ * does, and record them in block_table.  Written:
+ *   slots[cu_seqlens[b] + i] = page * page_size + offset of the row's i-th new
+ *     token, for i < new_lens[b]; -1 for the tokens of a row that is not
+ *     served and behind the last row's tokens, up to num_slots;
+ *   cu_seqlens [B + 1]; seq_lens[b] = cached + new (cached if not served);
+ *   *free_left = *free_count less the pages taken (may be the same word).
+ * A row is not served if its lengths are negative or exceed
+ * max_pages * page_size (PKV_DEVERR_LOGICAL_PAGE), or if it needs pages and
+ * the rows up to it need more than the stack holds (PKV_DEVERR_NO_PAGE).
+ * free_pages NULL: every page is in block_table already (free_count,
+ * free_left and counters are not used).  A page id that is negative or too
+ * large for 32-bit slots gives slot -1 (PKV_DEVERR_PAGE_ID); more new tokens
+ * than num_slots set PKV_DEVERR_SLOT, those beyond get no slot.  counters: one
+ * zeroed int32, left zero.  No buffer written may overlap cached_lens or
+ * new_lens.  Two calls that overlap on the GPU must not share a stack or
+ * counters. */
+pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
+                            int32_t* block_table, int32_t* slots, int32_t* cu_seqlens,
+                            int32_t* seq_lens, const int32_t* free_pages,
+                            const int32_t* free_count, int32_t* free_left, int32_t* counters,
+                            int B, int max_pages, int page_size, int num_slots,
+                            int free_capacity, void* stream);
+
+/* Writes T packed tokens, k / v [T][Hkv][128] with the given token and head
+ * strides (elements, multiples of 8), into 16-bit pools: token t of head h
+ * goes to slot slots[t] = page * page_size + offset.  A negative slot skips
+ * its token; one beyond the pool skips it and sets PKV_DEVERR_SLOT.  Of two
+ * tokens with one slot either may stay. */
+pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pages,
+                        const int32_t* slots, int T, int Hkv, int head_dim, long long k_stride,
+                        long long k_head_stride, long long v_stride, long long v_head_stride,
+                        int physical_pages, int page_size, pkv_dtype dtype, void* stream);
+
+/* The same into e4m3 pools with block scales (layout of
+ * pkv_paged_attention_auto_fp8_block); dtype is that of k / v.  The tokens of
+ * a call that fall into one block must be consecutive and in slot order, as
+ * pkv_prompt_slots places them.  A block's scale becomes the least power of two,
+ * at least 2^-24, that brings the tokens' largest magnitude to 448 or below,
+ * and at least the old scale if the first of them is not the block's first
+ * token: the earlier tokens stay, moved to the new scale if it grew.  Values
+ * are rounded to nearest, ties to even.  Infinities and NaN do not set a
+ * scale: the first are stored as +-448, the second as NaN. */
+pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, void* v_pages,
+                                  float* k_scales, float* v_scales, const int32_t* slots, int T,
+                                  int Hkv, int head_dim, long long k_stride,
+                                  long long k_head_stride, long long v_stride,
+                                  long long v_head_stride, int physical_pages, int page_size,
+                                  int block_tokens, pkv_dtype dtype, void* stream);
+
+/* Causal attention of packed sequences.  Sequence b has the query rows
+ * [cu_seqlens_q[b], cu_seqlens_q[b + 1]) and the keys
+ * [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (NULL: the query rows); its last row
+ * sees its last key, so row i of lq sees the keys j <= i + lk - lq of lk, and a
+ * row that sees none gives zeros.  q [q_tokens][Hq][128], k / v
+ * [k_tokens][Hkv][128] with the given strides (elements, multiples of 8),
+ * output [q_tokens][Hq][128] contiguous; softmax scale 1 / sqrt(128).  lse
+ * (or NULL): [q_tokens][Hq] natural log of each row's sum of exponentials,
+ * -inf for a row that sees no key.  Rows of no sequence are left as they
+ * were, and a row's result depends on no key that it does not see, whatever
+ * those hold.  A sequence whose ranges lie outside the tokens is skipped and
+ * sets PKV_DEVERR_INDEX. */
+pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                void* output, float* lse, int B, int q_tokens, int k_tokens,
+                                int Hq, int Hkv, int head_dim, long long q_stride,
+                                long long q_head_stride, long long k_stride,
+                                long long k_head_stride, long long v_stride,
+                                long long v_head_stride, pkv_dtype dtype, void* stream);
+
 /* ---- KV append (the write side of a decode step) ----
  * Writes one new token per row into the paged pools: row b's k_new[b] /
  * v_new[b] ([B][Hkv][128], same 16-bit dtype as the pools) land at token

@@ -11,7 +11,8 @@ is no fallback path (build it with ``python -m persistentkv_attention_b200.build
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
+from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_longlong, c_size_t,
+                    c_uint32, c_void_p)
 import os
 from pathlib import Path
 
@@ -145,6 +146,22 @@ SIGNATURES = {
         [_P, _P, _P, c_float, c_float, _P, _P, _P, _P, _P, _P, c_size_t, _P, c_int, c_int,
          c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P],
     ),
+    "pkv_paged_attention_auto_fp8_block": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P, c_int, c_int, c_int, c_int,
+         c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P],
+    ),
+    "pkv_prompt_slots": (
+        c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
+    "pkv_kv_write": (
+        c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong,
+                c_longlong, c_int, c_int, c_int, _P]),
+    "pkv_kv_write_fp8_block": (
+        c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_longlong, c_longlong,
+                c_longlong, c_longlong, c_int, c_int, c_int, c_int, _P]),
+    "pkv_prompt_attention": (
+        c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
+                c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, _P]),
     "pkv_kv_append": (
         c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                 c_int, _P]),

@@ -15,6 +15,7 @@
 
 #include "../../include/pkv_b200.h"
 #include "pkv_aux_kernels.cuh"
+#include "pkv_internal.h"
 #include "pkv_launch.cuh"
 
 using namespace pkv;
@@ -147,6 +148,21 @@ pkv_status current_device(DeviceState** out) {
     *out = &ds;
     return PKV_OK;
 }
+
+}  // namespace
+
+namespace pkv_internal {
+pkv_status device_state(int* sm_count, unsigned** error_word) {
+    DeviceState* ds = nullptr;
+    const pkv_status st = current_device(&ds);
+    if (st != PKV_OK) return st;
+    *sm_count = ds->sm_count;
+    *error_word = ds->error_word;
+    return PKV_OK;
+}
+}  // namespace pkv_internal
+
+namespace {
 
 // ------------------------------------------------------------ tensor maps
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -350,6 +366,8 @@ pkv_status launch(LaunchSpec& ls, void* stream_ptr) {
     ls.dp.error = ds->error_word;
     ls.dp.stamps = ds->stamps;
     ls.sm_count = ds->sm_count;
+    if (ls.scale_block > 0)
+        return pkv_internal::launch_block8(ls, static_cast<cudaStream_t>(stream_ptr));
     ls.load = ls.kv8 ? kLoadCpAsync : g_gather_mode.load(std::memory_order_relaxed);
     ls.fma = g_math_mode.load(std::memory_order_relaxed) == PKV_MATH_FMA;
     CUtensorMap tk, tv;
@@ -762,13 +780,20 @@ void xg_fill(DecodeParams& dp, const pkv_exchange& x) {
     dp.xg_counters = reinterpret_cast<unsigned*>(x.base + x.counters_off);
 }
 
+// Scales of an e4m3 pool with one scale per `block` tokens and head.
+struct BlockScales {
+    const float* k;
+    const float* v;
+    int block;
+};
+
 pkv_status auto_common(const Common& c, const int32_t* seq_lens, const int32_t* q_indices,
                        const int32_t* out_indices, void* output, float* state_out,
                        void* workspace, size_t workspace_bytes, int32_t* merge_counters,
                        int q_rows, int out_rows, void* stream,
                        const pkv_exchange* xg = nullptr, bool pdl = false,
                        const float* kv8_scales = nullptr, const void* plan = nullptr,
-                       int groups = 0);
+                       int groups = 0, const BlockScales* block_scales = nullptr);
 
 }  // namespace
 
@@ -832,7 +857,8 @@ pkv_status auto_common(const Common& c, const int32_t* seq_lens, const int32_t* 
                        const int32_t* out_indices, void* output, float* state_out,
                        void* workspace, size_t workspace_bytes, int32_t* merge_counters,
                        int q_rows, int out_rows, void* stream, const pkv_exchange* xg,
-                       bool pdl, const float* kv8_scales, const void* plan, int groups) {
+                       bool pdl, const float* kv8_scales, const void* plan, int groups,
+                       const BlockScales* block_scales) {
     const int B = c.B, Hq = c.Hq, Hkv = c.Hkv;
     const int max_pages = c.max_pages, page_size = c.page_size;
     pkv_status st = check_common(c);
@@ -894,6 +920,11 @@ pkv_status auto_common(const Common& c, const int32_t* seq_lens, const int32_t* 
         ls.kv8 = true;
         ls.dp.scale_log2 *= kv8_scales[0];
         ls.dp.v_scale = kv8_scales[1];
+    }
+    if (block_scales != nullptr) {
+        ls.k_scales = block_scales->k;
+        ls.v_scales = block_scales->v;
+        ls.scale_block = block_scales->block;
     }
     return launch(ls, stream);
 }
@@ -1060,6 +1091,30 @@ pkv_status pkv_paged_attention_auto_fp8(
     return auto_common(c, seq_lens, q_indices, out_indices, output, nullptr, workspace,
                        workspace_bytes, merge_counters, q_rows, out_rows, stream, nullptr, false,
                        scales);
+}
+
+pkv_status pkv_paged_attention_auto_fp8_block(
+    const void* q_source, const void* k_pages, const void* v_pages, const float* k_scales,
+    const float* v_scales, const int32_t* block_table, const int32_t* seq_lens,
+    const int32_t* q_indices, const int32_t* out_indices, void* output, void* workspace,
+    size_t workspace_bytes, int32_t* merge_counters, int B, int q_rows, int out_rows, int Hq,
+    int Hkv, int head_dim, int physical_pages, int page_size, int max_pages, int block_tokens,
+    pkv_dtype dtype, void* stream) {
+    if (output == nullptr) return fail(PKV_ERR_INVALID_ARGUMENT, "output must be a CUDA tensor");
+    if (k_scales == nullptr || v_scales == nullptr)
+        return fail(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must be CUDA tensors");
+    if (page_size <= 0) return fail(PKV_ERR_INVALID_ARGUMENT, "page_size must be positive");
+    if (block_tokens <= 0 || block_tokens % 16 != 0 || page_size % block_tokens != 0)
+        return fail(PKV_ERR_UNSUPPORTED,
+                    "a scale block must be a multiple of 16 tokens that divides the page; got %d "
+                    "tokens in pages of %d",
+                    block_tokens, page_size);
+    Common c{q_source, k_pages, v_pages, block_table, B, Hq, Hkv, head_dim,
+             physical_pages, page_size, max_pages, dtype};
+    const BlockScales scales{k_scales, v_scales, block_tokens};
+    return auto_common(c, seq_lens, q_indices, out_indices, output, nullptr, workspace,
+                       workspace_bytes, merge_counters, q_rows, out_rows, stream, nullptr, false,
+                       nullptr, nullptr, 0, &scales);
 }
 
 // ------------------------------------------------------------ KV append

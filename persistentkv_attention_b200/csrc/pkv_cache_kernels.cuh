@@ -1,0 +1,394 @@
+// pkv_cache_kernels.cuh -- the prompt side of the paged cache: block tables
+// and slot maps from request lengths, and the writes of packed K/V tokens
+// into 16-bit pools and into e4m3 pools with one scale per block of tokens
+// and head.  Included by pkv_prompt.cu only.
+#pragma once
+
+#include "pkv_device.cuh"
+
+namespace pkv {
+
+// ------------------------------------------------------------ prompt slots
+struct SlotsParams {
+    const int32_t* cached_lens;  // [B]
+    const int32_t* new_lens;     // [B]
+    int32_t* block_table;        // [B][max_pages]
+    int32_t* slots;              // [num_slots]
+    int32_t* cu_seqlens;         // [B + 1]
+    int32_t* seq_lens;           // [B]
+    const int32_t* free_pages;   // stack, or null (every page is already mapped)
+    const int32_t* free_count;
+    int32_t* free_left;          // may be free_count
+    int32_t* counters;           // [1] zeroed; finished CTAs
+    unsigned* error;
+    int B, max_pages, page_size, num_slots, free_capacity;
+};
+
+constexpr int kSlotThreads = 256;
+constexpr int kSlotTokensPerCta = 1024;
+
+// Sum over the CTA of one 64-bit value per thread, exclusive prefix returned,
+// total in `total`.  Both 32-bit halves are sums of non-negative values below
+// 2^31, so they do not carry into one another.
+__device__ __forceinline__ unsigned long long slot_scan(unsigned long long v,
+                                                        unsigned long long* s_warp,
+                                                        unsigned long long& total) {
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    unsigned long long x = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    unsigned long long before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kSlotThreads / 32; ++w) {
+        const unsigned long long t = s_warp[w];
+        before += w < warp ? t : 0ull;
+        total += t;
+    }
+    __syncthreads();
+    return before + x - v;
+}
+
+// Everything a token's slot depends on is a prefix sum over the rows before
+// its own: its first token, and the number of pages those rows take from the
+// stack.  So each CTA scans all rows (256 at a time) and fills the slots of
+// its own kSlotTokensPerCta tokens, and no CTA waits for another; the token's
+// row comes from a binary search in the scanned prefixes.  New pages are read
+// from the stack, never from block_table, where another CTA may still be
+// writing them.  Bound: launch and scan latency for a few rows (the work is a
+// few KB), the 4 B per token written for many.
+__global__ void __launch_bounds__(kSlotThreads)
+    pkv_prompt_slots_kernel(const __grid_constant__ SlotsParams p) {
+    __shared__ unsigned long long s_warp[kSlotThreads / 32];
+    __shared__ int s_start[kSlotThreads], s_cached[kSlotThreads], s_need[kSlotThreads];
+    const int t = threadIdx.x;
+    const long long limit = (long long)p.max_pages * p.page_size;
+    int avail = 0;
+    if (p.free_pages != nullptr) {
+        avail = *p.free_count;
+        if (avail < 0) avail = 0;
+        if (avail > p.free_capacity) {
+            if (blockIdx.x == 0 && t == 0) raise_error(p.error, kErrIndex);
+            avail = p.free_capacity;
+        }
+    }
+    const long long t0 = (long long)blockIdx.x * kSlotTokensPerCta;
+    const long long t1 = min(t0 + kSlotTokensPerCta, (long long)p.num_slots);
+    long long tokens = 0, pages = 0;  // of the rows before the current chunk
+    int taken = 0;
+    bool bad_len = false, no_page = false, bad_page = false;
+    for (int base = 0; base < p.B; base += kSlotThreads) {
+        const int b = base + t;
+        int c = 0, n = 0, need = 0;
+        bool valid = true;
+        if (b < p.B) {
+            c = __ldg(p.cached_lens + b);
+            n = __ldg(p.new_lens + b);
+            valid = c >= 0 && n >= 0 && (long long)c + n <= limit;
+            if (n < 0) n = 0;
+            if (!valid) bad_len = true;
+            if (valid && p.free_pages != nullptr)
+                need = (c + n + p.page_size - 1) / p.page_size -
+                       (c + p.page_size - 1) / p.page_size;
+        }
+        unsigned long long total;
+        const unsigned long long pre =
+            slot_scan(((unsigned long long)(unsigned)n << 32) | (unsigned)need, s_warp, total);
+        const long long start = tokens + (long long)(pre >> 32);
+        const long long before = pages + (long long)(pre & 0xffffffffull);
+        const bool short_of = need > 0 && before + need > avail;
+        const bool served = valid && !short_of;
+        if (short_of) no_page = true;
+        if (served && need > 0) taken = max(taken, (int)(before + need));
+        if (b < p.B && blockIdx.x == 0) {
+            p.cu_seqlens[b] = (int)min(start, (long long)INT_MAX);
+            p.seq_lens[b] = served ? c + n : max(c, 0);
+        }
+        // rows of this chunk for the token search; -1 marks a row not served
+        s_start[t] = (int)min(start, (long long)INT_MAX);
+        s_cached[t] = served ? c : -1;
+        s_need[t] = (int)min(before, (long long)INT_MAX);
+        __syncthreads();
+        const long long end = tokens + (long long)(total >> 32);
+        const int rows = min(kSlotThreads, p.B - base);
+        const long long lo = max(t0, tokens), hi = min(t1, end);
+        for (long long tok = lo + t; tok < hi; tok += kSlotThreads) {
+            // the last row that starts at or before tok (rows of no tokens that
+            // start there come before it)
+            int a = 0, z = rows;
+            while (z - a > 1) {
+                const int m = (a + z) >> 1;
+                if ((long long)s_start[m] <= tok) a = m; else z = m;
+            }
+            const int cached = s_cached[a];
+            int slot = -1;
+            if (cached >= 0) {
+                const int pos = cached + (int)(tok - s_start[a]);
+                const int j = pos / p.page_size;
+                const int off = pos - j * p.page_size;
+                int32_t* entry = p.block_table + (size_t)(base + a) * p.max_pages + j;
+                const int first = (cached + p.page_size - 1) / p.page_size;
+                int page;
+                if (p.free_pages != nullptr && j >= first) {
+                    page = __ldg(p.free_pages + (avail - 1 - s_need[a] - (j - first)));
+                    if (off == 0) *entry = page;
+                } else {
+                    page = *entry;
+                }
+                if (page < 0 || page > (INT_MAX - p.page_size) / p.page_size) {
+                    bad_page = true;
+                } else {
+                    slot = page * p.page_size + off;
+                }
+            }
+            p.slots[tok] = slot;
+        }
+        tokens = end;
+        pages += (long long)(total & 0xffffffffull);
+        __syncthreads();
+    }
+    for (long long tok = max(t0, tokens) + t; tok < t1; tok += kSlotThreads) p.slots[tok] = -1;
+    if (bad_page) raise_error(p.error, kErrPageId);
+    if (blockIdx.x == 0) {
+        if (bad_len) raise_error(p.error, kErrLogicalPage);
+        if (no_page) raise_error(p.error, kErrNoPage);
+        if (t == 0) {
+            if (tokens > p.num_slots) raise_error(p.error, kErrSlot);
+            p.cu_seqlens[p.B] = (int)min(tokens, (long long)INT_MAX);
+        }
+    }
+    if (p.free_pages != nullptr) {
+        // every thread has read *free_count; the last CTA to get here writes
+        // what is left (free_left may be the same word)
+        taken = __reduce_max_sync(0xffffffffu, taken);
+        if ((t & 31) == 0) s_start[t >> 5] = taken;
+        __syncthreads();
+        if (t == 0) {
+#pragma unroll
+            for (int w = 1; w < kSlotThreads / 32; ++w) taken = max(taken, s_start[w]);
+            __threadfence();
+            if (atomicAdd(p.counters, 1) == (int)gridDim.x - 1) {
+                *p.counters = 0;
+                *p.free_left = avail - taken;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ 16-bit write
+struct WriteParams {
+    const uint8_t* k;  // [T][Hkv][128] 16-bit elements, token / head strides in bytes
+    const uint8_t* v;
+    uint8_t* k_pages;  // [P][Hkv][page][128], 16-bit or e4m3
+    uint8_t* v_pages;
+    float* k_scales;   // [P][Hkv][page / block] (e4m3 pools)
+    float* v_scales;
+    const int32_t* slots;  // [T]
+    unsigned* error;
+    long long k_tok, k_head, v_tok, v_head;
+    long long num_slots;  // P * page
+    int T, Hkv, page_size, block;
+};
+
+constexpr int kWriteThreads = 256;
+
+// One thread moves one 16-byte piece of a token's K and the same piece of its
+// V.  A copy: HBM-bound for long prompts.
+__global__ void __launch_bounds__(kWriteThreads)
+    pkv_kv_write_kernel(const __grid_constant__ WriteParams p) {
+    constexpr int kPieces = kRowBytes / 16;
+    const int per_token = p.Hkv * kPieces;
+    const long long i = (long long)blockIdx.x * kWriteThreads + threadIdx.x;
+    const long long t = i / per_token;
+    if (t >= p.T) return;
+    const int r = (int)(i - t * per_token);
+    const int h = r / kPieces, piece = r % kPieces;
+    const int slot = __ldg(p.slots + t);
+    if (slot < 0) return;  // padding
+    if (slot >= p.num_slots) {
+        if (r == 0) raise_error(p.error, kErrSlot);
+        return;
+    }
+    const uint4 kv = __ldg(reinterpret_cast<const uint4*>(p.k + t * p.k_tok + h * p.k_head) + piece);
+    const uint4 vv = __ldg(reinterpret_cast<const uint4*>(p.v + t * p.v_tok + h * p.v_head) + piece);
+    const int page = slot / p.page_size;
+    const size_t row = ((size_t)page * p.Hkv + h) * p.page_size + (slot - page * p.page_size);
+    reinterpret_cast<uint4*>(p.k_pages + row * kRowBytes)[piece] = kv;
+    reinterpret_cast<uint4*>(p.v_pages + row * kRowBytes)[piece] = vv;
+}
+
+// ------------------------------------------------------------ e4m3 block write
+// The tokens of a call that fall into one block of the cache (`block` slots of
+// one page) are a run of consecutive tokens.  One warp takes one run of one
+// head's K or V: the block's scale is the least power of two, at least 2^-24,
+// that brings the run's largest magnitude to e4m3's 448 or below, and, when
+// the run starts inside the block, at least the block's old scale, whose
+// earlier tokens stay.  A power of two makes x / scale and the move of old
+// codes to a larger scale exact up to e4m3's own rounding, and costs no
+// precision: e4m3 is a floating format, so a scale within a factor of two of
+// the tightest one keeps the same 3 mantissa bits.
+constexpr int kScaleExpMin = -24;
+
+__device__ __forceinline__ float block_scale(float amax) {
+    const unsigned bits = __float_as_uint(amax);
+    // amax = 1.f * 2^(E - 127); 448 = 1.75 * 2^8
+    int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    if (e < kScaleExpMin) e = kScaleExpMin;
+    return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t x);
+template <>
+__device__ __forceinline__ float2 to_float2<__half>(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+template <>
+__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t x) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+}
+
+// |x| where it is finite, else 0: infinities and NaN do not set a scale.
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Two e4m3 codes times a power of two, rounded back to e4m3.
+__device__ __forceinline__ uint32_t rescale_e4m3x2(uint32_t codes, float ratio) {
+    const __half2_raw h =
+        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return e4m3x2(f.x * ratio, f.y * ratio);
+}
+
+constexpr int kRunRows = 16;  // tokens held in registers at a time
+
+// Warp w of the grid: window of 16 tokens w / (2 Hkv), head (w / 2) % Hkv, K or
+// V by w % 2; it takes the runs that start in its window.  Lane l holds 16
+// bytes (8 elements) of tokens l / 16 + 2 i: 8 loads in flight, 4 KB a warp.
+template <typename T>
+__global__ void __launch_bounds__(kWriteThreads)
+    pkv_kv_write_block_kernel(const __grid_constant__ WriteParams p) {
+    const int lane = threadIdx.x & 31;
+    const long long w = ((long long)blockIdx.x * kWriteThreads + threadIdx.x) >> 5;
+    const long long window = w / (2 * p.Hkv);
+    const long long t0 = window * kRunRows;
+    if (t0 >= p.T) return;
+    const int r = (int)(w - window * (2 * p.Hkv));
+    const int h = r >> 1;
+    const bool is_v = (r & 1) != 0;
+    const uint8_t* src = is_v ? p.v + h * p.v_head : p.k + h * p.k_head;
+    const long long tok_stride = is_v ? p.v_tok : p.k_tok;
+    uint8_t* pool = is_v ? p.v_pages : p.k_pages;
+    float* scales = is_v ? p.v_scales : p.k_scales;
+    const int nblk = p.page_size / p.block;
+    // blocks of the window's tokens and of the token before it; -1 is padding
+    auto block_of = [&](long long t) -> int {
+        if (t < 0 || t >= p.T) return -1;
+        const int s = __ldg(p.slots + t);
+        if (s < 0) return -1;
+        if (s >= p.num_slots) {
+            if (r == 0) raise_error(p.error, kErrSlot);
+            return -1;
+        }
+        return s / p.block;
+    };
+    const int blk = block_of(t0 + lane - 1);  // lane 0: the token before the window
+    const int prev = __shfl_up_sync(0xffffffffu, blk, 1);
+    unsigned starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= kRunRows && blk >= 0 &&
+                                                     blk != prev);
+    const int half = lane >> 4, piece = lane & 15;
+    while (starts != 0u) {
+        const int sl = __ffs(starts) - 1;
+        starts &= starts - 1;
+        const int run_blk = __shfl_sync(0xffffffffu, blk, sl);
+        const long long first = t0 + sl - 1;
+        // length of the run
+        int n = 0;
+        while (true) {
+            const unsigned same =
+                __ballot_sync(0xffffffffu, block_of(first + n + lane) == run_blk);
+            const int more = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+            n += more;
+            if (more < 32) break;
+        }
+        const int page = run_blk / nblk, g = run_blk % nblk;
+        float* scale_at = scales + ((size_t)page * p.Hkv + h) * nblk + g;
+        uint8_t* block_base =
+            pool + (((size_t)page * p.Hkv + h) * p.page_size + (size_t)g * p.block) * kHeadDim;
+        const int kept = __ldg(p.slots + first) - run_blk * p.block;
+        uint4 x[kRunRows / 2];
+        float amax = 0.f;
+        auto load = [&](int base) {
+#pragma unroll
+            for (int i = 0; i < kRunRows / 2; ++i) {
+                const int row = base + half + 2 * i;
+                x[i] = row < n ? __ldg(reinterpret_cast<const uint4*>(src + (first + row) * tok_stride) +
+                                       piece)
+                               : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        for (int base = 0; base < n; base += kRunRows) {
+            load(base);
+#pragma unroll
+            for (int i = 0; i < kRunRows / 2; ++i) {
+                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = to_float2<T>(u[j]);
+                    amax = fmaxf(amax, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+                }
+            }
+        }
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+        float scale = block_scale(amax);
+        if (kept > 0) {
+            const float old = *scale_at;
+            if (old > scale) {
+                scale = old;
+            } else if (old < scale) {
+                // the earlier tokens move to the larger scale
+                const float ratio = old / scale;
+                for (int o = half; o < kept; o += 2) {
+                    uint2* at = reinterpret_cast<uint2*>(block_base + (size_t)o * kHeadDim) + piece;
+                    uint2 c = *at;
+                    c.x = rescale_e4m3x2(c.x, ratio) | (rescale_e4m3x2(c.x >> 16, ratio) << 16);
+                    c.y = rescale_e4m3x2(c.y, ratio) | (rescale_e4m3x2(c.y >> 16, ratio) << 16);
+                    *at = c;
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) *scale_at = scale;
+        // 1 / scale: exact for a power of two (an old scale may be any value)
+        const float inv = 1.0f / scale;
+        for (int base = 0; base < n; base += kRunRows) {
+            if (n > kRunRows) load(base);
+#pragma unroll
+            for (int i = 0; i < kRunRows / 2; ++i) {
+                const int row = base + half + 2 * i;
+                if (row >= n) continue;
+                const int off = __ldg(p.slots + first + row) - run_blk * p.block;
+                const float2 a = to_float2<T>(x[i].x), b = to_float2<T>(x[i].y);
+                const float2 c = to_float2<T>(x[i].z), d = to_float2<T>(x[i].w);
+                uint2 out;
+                out.x = e4m3x2(a.x * inv, a.y * inv) | (e4m3x2(b.x * inv, b.y * inv) << 16);
+                out.y = e4m3x2(c.x * inv, c.y * inv) | (e4m3x2(d.x * inv, d.y * inv) << 16);
+                reinterpret_cast<uint2*>(block_base + (size_t)off * kHeadDim)[piece] = out;
+            }
+        }
+    }
+}
+
+}  // namespace pkv

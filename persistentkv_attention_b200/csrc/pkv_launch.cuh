@@ -8,6 +8,7 @@
 #include <atomic>
 
 #include "../../include/pkv_b200.h"
+#include "pkv_internal.h"
 #include "pkv_kernels.cuh"
 
 #ifndef PKV_RING_SLOTS
@@ -20,15 +21,15 @@ constexpr int kSlots = PKV_RING_SLOTS;               // ring depth (8 KB per slo
 constexpr int kCtasPerSm = PKV_MIN_CTAS_PER_SM;      // resident decode CTAs per SM
 constexpr int kMaxDevices = 64;
 
-// printf-style error reporting into the thread-local message of pkv_api.cu.
-pkv_status fail_fmt(pkv_status st, const char* fmt, ...);
-pkv_status ok();
-
 struct LaunchSpec {
     pkv::DecodeParams dp;
     bool merge;        // run the separate merge kernel after decode (pkv_api.cu)
     bool pdl = false;  // decode may launch early behind the previous kernel (it waits on it)
     bool kv8 = false;  // e4m3 K/V pools (cp.async producer)
+    // e4m3 pools with one scale per scale_block tokens and head (launch_block8)
+    const float* k_scales = nullptr;
+    const float* v_scales = nullptr;
+    int scale_block = 0;
     bool lean = false; // the planned step route (pkv_decode_kernel's LEAN form)
     bool fma = false;  // CUDA-core consumer math where the route allows it (PKV_MATH_FMA)
     int load = pkv::kLoadCpAsync;  // gather: pkv::kLoadTma or pkv::kLoadCpAsync
@@ -121,6 +122,9 @@ pkv_status launch_typed(const LaunchSpec& ls, const CUtensorMap& tk, const CUten
 template <typename T, int BR, int LOAD, bool KV8>
 pkv_status launch_g(const LaunchSpec& ls, const CUtensorMap& tk, const CUtensorMap& tv,
                     cudaStream_t s);
+
+// Decode over e4m3 pools with block scales (pkv_block8.cu).
+pkv_status launch_block8(const LaunchSpec& ls, cudaStream_t stream);
 
 #define PKV_DEFINE_LAUNCH_G(T, BR, LOAD, KV8)                                                    \
     template <>                                                                                   \

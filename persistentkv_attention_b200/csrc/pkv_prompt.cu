@@ -1,0 +1,261 @@
+// pkv_prompt.cu -- C ABI of the prompt side (declared in include/pkv_b200.h):
+// block tables and slot maps, K/V writes by slot, attention of packed prompts.
+// No counterpart in the reference, which decodes over pre-filled pools.
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "../../include/pkv_b200.h"
+#include "pkv_cache_kernels.cuh"
+#include "pkv_internal.h"
+#include "pkv_prompt_kernels.cuh"
+
+using namespace pkv;
+using pkv_internal::device_state;
+using pkv_internal::fail_fmt;
+using pkv_internal::ok;
+
+namespace {
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+pkv_status launched(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return fail_fmt(PKV_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+    return ok();
+}
+
+// Strides (in elements) of a [T][H][128] operand: 16-byte rows, forward.  The
+// stride of a dimension of one entry means nothing and becomes a dense one.
+pkv_status check_strides(const char* name, int T, int H, long long* tok, long long* head) {
+    if (H <= 1) *head = kHeadDim;
+    if (T <= 1) *tok = *head * H;
+    if (*tok <= 0 || *head <= 0 || *tok % 8 != 0 || *head % 8 != 0)
+        return fail_fmt(PKV_ERR_MISALIGNED, "%s strides must be positive multiples of 8 elements",
+                        name);
+    return PKV_OK;
+}
+
+// Shared checks of the two writes; fills everything but the scales.
+pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_pages,
+                        void* v_pages, const int32_t* slots, int T, int Hkv, int head_dim,
+                        long long k_stride, long long k_head_stride, long long v_stride,
+                        long long v_head_stride, int physical_pages, int page_size,
+                        pkv_dtype dtype) {
+    if (k == nullptr || v == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k and v must be CUDA tensors");
+    if (k_pages == nullptr || v_pages == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_pages and v_pages must be CUDA tensors");
+    if (slots == nullptr) return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "slots must be a CUDA tensor");
+    if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "k has wrong dtype");
+    if (head_dim != kHeadDim)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "PersistentKV extension currently requires d=128");
+    if (T < 0 || Hkv <= 0 || physical_pages <= 0 || page_size <= 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid write shape");
+    if ((long long)physical_pages * page_size >= (1ll << 31))
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "the pool holds %lld slots, beyond 32-bit slots",
+                        (long long)physical_pages * page_size);
+    pkv_status st = check_strides("k", T, Hkv, &k_stride, &k_head_stride);
+    if (st == PKV_OK) st = check_strides("v", T, Hkv, &v_stride, &v_head_stride);
+    if (st != PKV_OK) return st;
+    if (misaligned(k) || misaligned(v) || misaligned(k_pages) || misaligned(v_pages))
+        return fail_fmt(PKV_ERR_MISALIGNED, "k, v and the pools must be 16-byte aligned");
+    wp.k = static_cast<const uint8_t*>(k);
+    wp.v = static_cast<const uint8_t*>(v);
+    wp.k_pages = static_cast<uint8_t*>(k_pages);
+    wp.v_pages = static_cast<uint8_t*>(v_pages);
+    wp.k_scales = wp.v_scales = nullptr;
+    wp.slots = slots;
+    wp.error = nullptr;
+    wp.k_tok = 2 * k_stride;
+    wp.k_head = 2 * k_head_stride;
+    wp.v_tok = 2 * v_stride;
+    wp.v_head = 2 * v_head_stride;
+    wp.num_slots = (long long)physical_pages * page_size;
+    wp.T = T;
+    wp.Hkv = Hkv;
+    wp.page_size = page_size;
+    wp.block = page_size;
+    return PKV_OK;
+}
+
+pkv_status grid_of(long long threads, int per_cta, unsigned* grid) {
+    const long long n = (threads + per_cta - 1) / per_cta;
+    if (n > INT_MAX) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many tokens for one launch");
+    *grid = (unsigned)n;
+    return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
+                            int32_t* block_table, int32_t* slots, int32_t* cu_seqlens,
+                            int32_t* seq_lens, const int32_t* free_pages,
+                            const int32_t* free_count, int32_t* free_left, int32_t* counters,
+                            int B, int max_pages, int page_size, int num_slots,
+                            int free_capacity, void* stream) {
+    if (B > 0 && (cached_lens == nullptr || new_lens == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "cached_lens and new_lens must be CUDA tensors");
+    if (cu_seqlens == nullptr || (B > 0 && (block_table == nullptr || seq_lens == nullptr)))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                        "block_table, cu_seqlens and seq_lens must be CUDA tensors");
+    if (slots == nullptr && num_slots > 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "slots must be a CUDA tensor");
+    if (free_pages != nullptr &&
+        (free_count == nullptr || free_left == nullptr || counters == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                        "a free-page list needs free_count, free_left and zeroed counters");
+    if (B > 0 && (seq_lens == cached_lens || seq_lens == new_lens || cu_seqlens == cached_lens ||
+                  cu_seqlens == new_lens))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                        "seq_lens and cu_seqlens must not be the tensors they are made from");
+    if (B < 0 || max_pages <= 0 || page_size <= 0 || num_slots < 0 || free_capacity < 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid slot map shape");
+    if ((long long)max_pages * page_size >= (1ll << 31))
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "max_pages * page_size exceeds 32-bit positions");
+    int sms = 0;
+    unsigned* error = nullptr;
+    pkv_status st = device_state(&sms, &error);
+    if (st != PKV_OK) return st;
+    const SlotsParams sp{cached_lens, new_lens,  block_table, slots,     cu_seqlens,
+                         seq_lens,    free_pages, free_count, free_left, counters,
+                         error,       B,          max_pages,  page_size, num_slots,
+                         free_capacity};
+    const int grid = num_slots > 0 ? (int)(((long long)num_slots + kSlotTokensPerCta - 1) /
+                                           kSlotTokensPerCta)
+                                   : 1;
+    pkv_prompt_slots_kernel<<<grid, kSlotThreads, 0, static_cast<cudaStream_t>(stream)>>>(sp);
+    return launched("slot map");
+}
+
+pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pages,
+                        const int32_t* slots, int T, int Hkv, int head_dim, long long k_stride,
+                        long long k_head_stride, long long v_stride, long long v_head_stride,
+                        int physical_pages, int page_size, pkv_dtype dtype, void* stream) {
+    WriteParams wp;
+    pkv_status st = write_params(wp, k, v, k_pages, v_pages, slots, T, Hkv, head_dim, k_stride,
+                                 k_head_stride, v_stride, v_head_stride, physical_pages,
+                                 page_size, dtype);
+    if (st != PKV_OK) return st;
+    if (T == 0) return ok();
+    int sms = 0;
+    st = device_state(&sms, &wp.error);
+    if (st != PKV_OK) return st;
+    unsigned grid = 0;
+    st = grid_of((long long)T * Hkv * (kRowBytes / 16), kWriteThreads, &grid);
+    if (st != PKV_OK) return st;
+    pkv_kv_write_kernel<<<grid, kWriteThreads, 0, static_cast<cudaStream_t>(stream)>>>(wp);
+    return launched("K/V write");
+}
+
+pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, void* v_pages,
+                                  float* k_scales, float* v_scales, const int32_t* slots, int T,
+                                  int Hkv, int head_dim, long long k_stride,
+                                  long long k_head_stride, long long v_stride,
+                                  long long v_head_stride, int physical_pages, int page_size,
+                                  int block_tokens, pkv_dtype dtype, void* stream) {
+    WriteParams wp;
+    pkv_status st = write_params(wp, k, v, k_pages, v_pages, slots, T, Hkv, head_dim, k_stride,
+                                 k_head_stride, v_stride, v_head_stride, physical_pages,
+                                 page_size, dtype);
+    if (st != PKV_OK) return st;
+    if (k_scales == nullptr || v_scales == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must be CUDA tensors");
+    if (block_tokens <= 0 || block_tokens % 16 != 0 || page_size % block_tokens != 0)
+        return fail_fmt(PKV_ERR_UNSUPPORTED,
+                        "a scale block must be a multiple of 16 tokens that divides the page; "
+                        "got %d tokens in pages of %d",
+                        block_tokens, page_size);
+    wp.k_scales = k_scales;
+    wp.v_scales = v_scales;
+    wp.block = block_tokens;
+    if (T == 0) return ok();
+    int sms = 0;
+    st = device_state(&sms, &wp.error);
+    if (st != PKV_OK) return st;
+    unsigned grid = 0;
+    const long long windows = ((long long)T + kRunRows - 1) / kRunRows;
+    st = grid_of(windows * 2 * Hkv * 32, kWriteThreads, &grid);
+    if (st != PKV_OK) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == PKV_DTYPE_F16)
+        pkv_kv_write_block_kernel<__half><<<grid, kWriteThreads, 0, s>>>(wp);
+    else
+        pkv_kv_write_block_kernel<__nv_bfloat16><<<grid, kWriteThreads, 0, s>>>(wp);
+    return launched("e4m3 K/V write");
+}
+
+pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                void* output, float* lse, int B, int q_tokens, int k_tokens,
+                                int Hq, int Hkv, int head_dim, long long q_stride,
+                                long long q_head_stride, long long k_stride,
+                                long long k_head_stride, long long v_stride,
+                                long long v_head_stride, pkv_dtype dtype, void* stream) {
+    if (q_tokens > 0 && (q == nullptr || output == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "q and output must be CUDA tensors");
+    if (k_tokens > 0 && (k == nullptr || v == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k and v must be CUDA tensors");
+    if (cu_seqlens_q == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "cu_seqlens_q must be a CUDA tensor");
+    if (cu_seqlens_k == nullptr) cu_seqlens_k = cu_seqlens_q;
+    if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "q has wrong dtype");
+    if (head_dim != kHeadDim)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "PersistentKV extension currently requires d=128");
+    if (Hkv <= 0) return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hkv must be positive");
+    if (Hq <= 0 || Hq % Hkv != 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hq must be divisible by Hkv");
+    const int G = Hq / Hkv;
+    if (!(G == 1 || G == 2 || G == 4 || G == 8))
+        return fail_fmt(PKV_ERR_UNSUPPORTED,
+                        "PersistentKV supports G=Hq/Hkv in {1,2,4,8}; got G=%d from Hq=%d Hkv=%d",
+                        G, Hq, Hkv);
+    if (B < 0 || q_tokens < 0 || k_tokens < 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid prompt shape");
+    pkv_status st = check_strides("q", q_tokens, Hq, &q_stride, &q_head_stride);
+    if (st == PKV_OK) st = check_strides("k", k_tokens, Hkv, &k_stride, &k_head_stride);
+    if (st == PKV_OK) st = check_strides("v", k_tokens, Hkv, &v_stride, &v_head_stride);
+    if (st != PKV_OK) return st;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(output))
+        return fail_fmt(PKV_ERR_MISALIGNED, "q, k, v and output must be 16-byte aligned");
+    if (B == 0 || q_tokens == 0) return ok();
+    PromptParams pp;
+    pp.q = static_cast<const uint8_t*>(q);
+    pp.k = static_cast<const uint8_t*>(k);
+    pp.v = static_cast<const uint8_t*>(v);
+    pp.cu_q = cu_seqlens_q;
+    pp.cu_k = cu_seqlens_k;
+    pp.out = output;
+    pp.lse = lse;
+    pp.q_tok = 2 * q_stride;
+    pp.q_head = 2 * q_head_stride;
+    pp.k_tok = 2 * k_stride;
+    pp.k_head = 2 * k_head_stride;
+    pp.v_tok = 2 * v_stride;
+    pp.v_head = 2 * v_head_stride;
+    pp.B = B;
+    pp.Tq = q_tokens;
+    pp.Tk = k_tokens;
+    pp.Hq = Hq;
+    pp.Hkv = Hkv;
+    pp.scale_log2 = (1.0f / sqrtf((float)kHeadDim)) * kLog2e;
+    int sms = 0;
+    st = device_state(&sms, &pp.error);
+    if (st != PKV_OK) return st;
+    unsigned grid = 0;
+    st = grid_of((long long)q_tokens * Hq * 32, 256, &grid);
+    if (st != PKV_OK) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == PKV_DTYPE_F16)
+        pkv_prompt_rows_kernel<__half><<<grid, 256, 0, s>>>(pp);
+    else
+        pkv_prompt_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(pp);
+    return launched("prompt attention");
+}
+
+}  // extern "C"

@@ -554,6 +554,232 @@ def kv_append(k_new, v_new, k_pages, v_pages, block_table, positions, free_pages
         k_pages.size(2), block_table.size(1), _DTYPES[dt], _stream()))
 
 
+def _check_current_device(*tensors) -> None:
+    """Kernels launch on the current device: every operand must live there."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise RuntimeError(f"operands must be on the current device, cuda:{device}")
+
+
+def _check_packed(t, name: str, dtype) -> None:
+    """A packed operand [tokens, heads, 128]: contiguous heads of 128, any
+    token and head strides (a slice of a fused projection's output is fine)."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if (t.dtype not in dtype) if isinstance(dtype, tuple) else t.dtype != dtype:
+        raise RuntimeError(f"{name} has wrong dtype")
+    if t.dim() != 3:
+        raise RuntimeError(f"{name} has wrong rank")
+    if t.size(2) != HEAD_DIM:
+        raise RuntimeError("PersistentKV extension currently requires d=128")
+    if t.stride(2) != 1:
+        raise RuntimeError(f"{name} must be contiguous in its last dimension")
+
+
+def _check_block_scales(k_pages, k_scales, v_scales) -> int:
+    """Scales [P, Hkv, page / block] of e4m3 pools; returns the block's tokens."""
+    _check_tensor(k_scales, "k_scales", torch.float32, 3)
+    _check_tensor(v_scales, "v_scales", torch.float32, 3)
+    pages, hkv, page_size, _ = k_pages.shape
+    blocks = k_scales.size(2)
+    if k_scales.shape != v_scales.shape or k_scales.size(0) != pages or k_scales.size(1) != hkv:
+        raise RuntimeError("k_scales / v_scales shape must be [P, Hkv, page_size / block]")
+    if blocks == 0 or page_size % blocks != 0 or (page_size // blocks) % 16 != 0:
+        raise RuntimeError("a scale block must be a multiple of 16 tokens that divides the page")
+    return page_size // blocks
+
+
+def paged_attention_auto_fp8_block(q_source, k_pages, v_pages, k_scales, v_scales, block_table,
+                                   seq_lens, output, workspace, q_indices=None, out_indices=None,
+                                   merge_counters=None) -> None:
+    """``paged_attention_auto`` over an e4m3 (``torch.float8_e4m3fn``) K/V cache
+    with one float32 scale per block of tokens and head: ``k_scales`` /
+    ``v_scales`` [P, Hkv, page_size / block], block a multiple of 16 tokens.  q
+    and output are fp16 or bf16.  Half the cache's bytes, read at the same
+    rate.  No counterpart in the reference."""
+    _check_tensor(q_source, "q_source", tuple(_DTYPES), 3)
+    _check_tensor(k_pages, "k_pages", torch.float8_e4m3fn, 4)
+    _check_tensor(v_pages, "v_pages", torch.float8_e4m3fn, 4)
+    _check_tensor(block_table, "block_table", torch.int32, 2)
+    _check_tensor(seq_lens, "seq_lens", torch.int32, 1)
+    _check_tensor(output, "output", q_source.dtype, 3)
+    if v_pages.shape != k_pages.shape or k_pages.size(3) != HEAD_DIM:
+        raise RuntimeError("k_pages / v_pages shape mismatch")
+    physical_pages, hkv, page_size, _ = k_pages.shape
+    block = _check_block_scales(k_pages, k_scales, v_scales)
+    b, max_pages = block_table.shape
+    q_rows, hq, d = q_source.shape
+    if d != HEAD_DIM:
+        raise RuntimeError("PersistentKV extension currently requires d=128")
+    if seq_lens.size(0) != b:
+        raise RuntimeError("seq_lens batch mismatch")
+    if output.size(1) != hq or output.size(2) != d:
+        raise RuntimeError("output shape must match q head dimensions")
+    ptrs = []
+    for name, t in (("q_indices", q_indices), ("out_indices", out_indices)):
+        if t is None:
+            ptrs.append(None)
+        else:
+            _check_tensor(t, name, torch.int32, 1)
+            if t.size(0) != b:
+                raise RuntimeError(f"{name} batch mismatch")
+            ptrs.append(t.data_ptr())
+    # without an index tensor row b reads q_source[b] and writes output[b]
+    if (q_indices is None and q_rows < b) or (out_indices is None and output.size(0) < b):
+        raise RuntimeError("q_source and output need a row per block_table row")
+    ctr = None
+    if merge_counters is not None:
+        _check_tensor(merge_counters, "merge_counters", torch.int32, 2)
+        if merge_counters.size(0) != b or merge_counters.size(1) != hkv:
+            raise RuntimeError("merge_counters shape mismatch")
+        ctr = merge_counters.data_ptr()
+    _check_supported_gqa(hq, hkv)
+    ws_ptr, ws_bytes = _workspace(workspace)
+    _check_current_device(q_source, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens,
+                          output, workspace, q_indices, out_indices, merge_counters)
+    _native.check(_native.load().pkv_paged_attention_auto_fp8_block(
+        q_source.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+        v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptrs[0], ptrs[1],
+        output.data_ptr(), ws_ptr, ws_bytes, ctr, b, q_rows, output.size(0), hq, hkv, d,
+        physical_pages, page_size, max_pages, block, _DTYPES[q_source.dtype], _stream()))
+
+
+def prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens, free_pages,
+                 free_count, free_left, counters, page_size: int) -> None:
+    """Block tables and slot map of a batch, on the GPU, from its lengths.
+
+    Row b holds ``cached_lens[b]`` tokens and gets ``new_lens[b]`` more (int32
+    [B]).  The rows, in order, take the pages they open from the top of the
+    ``free_pages`` stack (``free_count`` int32 [1] entries) into ``block_table``.
+    Written: ``slots`` (page * page_size + offset of every new token, packed; -1
+    for rows not served and behind the last token), ``cu_seqlens`` [B + 1],
+    ``seq_lens`` [B] (the lengths after the call) and ``free_left`` [1] (may be
+    ``free_count``).  ``counters``: one zeroed int32, left zero.  With
+    ``free_pages`` None every page is in ``block_table`` already.  See
+    ``pkv_prompt_slots`` for the rows that are not served.  No counterpart in
+    the reference."""
+    _check_tensor(cached_lens, "cached_lens", torch.int32, 1)
+    _check_tensor(new_lens, "new_lens", torch.int32, 1)
+    _check_tensor(block_table, "block_table", torch.int32, 2)
+    _check_tensor(slots, "slots", torch.int32, 1)
+    _check_tensor(cu_seqlens, "cu_seqlens", torch.int32, 1)
+    _check_tensor(seq_lens, "seq_lens", torch.int32, 1)
+    b, max_pages = block_table.shape
+    if cached_lens.size(0) != b or new_lens.size(0) != b or seq_lens.size(0) != b:
+        raise RuntimeError("cached_lens / new_lens / seq_lens batch mismatch")
+    if cu_seqlens.size(0) != b + 1:
+        raise RuntimeError("cu_seqlens must hold B + 1 values")
+    _positive(page_size, "page_size")
+    fp = fc = fl = ctr = None
+    capacity = 0
+    if free_pages is not None:
+        _check_tensor(free_pages, "free_pages", torch.int32, 1)
+        if free_count is None or free_left is None or counters is None:
+            raise RuntimeError("a free-page list needs free_count, free_left and counters")
+        for name, t in (("free_count", free_count), ("free_left", free_left),
+                        ("counters", counters)):
+            _check_tensor(t, name, torch.int32, 1)
+            if t.size(0) < 1:
+                raise RuntimeError(f"{name} must hold one value")
+        fp, fc = free_pages.data_ptr(), free_count.data_ptr()
+        fl, ctr = free_left.data_ptr(), counters.data_ptr()
+        capacity = free_pages.size(0)
+    _check_current_device(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens,
+                          free_pages, free_count, free_left, counters)
+    _native.check(_native.load().pkv_prompt_slots(
+        cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), slots.data_ptr(),
+        cu_seqlens.data_ptr(), seq_lens.data_ptr(), fp, fc, fl, ctr, b, max_pages,
+        int(page_size), slots.size(0), capacity, _stream()))
+
+
+def _check_write(k, v, k_pages, v_pages, slots, pool_dtype):
+    _check_packed(k, "k", tuple(_DTYPES))
+    _check_packed(v, "v", k.dtype)
+    _check_tensor(k_pages, "k_pages", pool_dtype, 4)
+    _check_tensor(v_pages, "v_pages", pool_dtype, 4)
+    _check_tensor(slots, "slots", torch.int32, 1)
+    if v.shape != k.shape or k_pages.size(1) != k.size(1) or k_pages.size(3) != HEAD_DIM:
+        raise RuntimeError("k / v shape must be [T, Hkv, 128] matching the pools")
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError("v_pages shape mismatch")
+    if slots.size(0) != k.size(0):
+        raise RuntimeError("slots must hold one value per token")
+
+
+def kv_write(k, v, k_pages, v_pages, slots) -> None:
+    """Writes packed tokens ``k`` / ``v`` [T, Hkv, 128] into 16-bit pools of their
+    dtype at ``slots`` [T] (page * page_size + offset; negative skips a token).
+    No counterpart in the reference."""
+    _check_write(k, v, k_pages, v_pages, slots, k.dtype)
+    _check_current_device(k, v, k_pages, v_pages, slots)
+    _native.check(_native.load().pkv_kv_write(
+        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(),
+        k.size(0), k.size(1), HEAD_DIM, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        k_pages.size(0), k_pages.size(2), _DTYPES[k.dtype], _stream()))
+
+
+def kv_write_fp8_block(k, v, k_pages, v_pages, k_scales, v_scales, slots) -> None:
+    """``kv_write`` into e4m3 pools with one scale per block of tokens and head
+    (``paged_attention_auto_fp8_block``'s cache): each block that the call
+    touches gets the least power of two that holds its new tokens, and its
+    earlier tokens if the call starts inside it.  The tokens of one block must
+    be consecutive and in slot order.  No counterpart in the reference."""
+    _check_write(k, v, k_pages, v_pages, slots, torch.float8_e4m3fn)
+    block = _check_block_scales(k_pages, k_scales, v_scales)
+    _check_current_device(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    _native.check(_native.load().pkv_kv_write_fp8_block(
+        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+        v_scales.data_ptr(), slots.data_ptr(), k.size(0), k.size(1), HEAD_DIM, k.stride(0),
+        k.stride(1), v.stride(0), v.stride(1), k_pages.size(0), k_pages.size(2), block,
+        _DTYPES[k.dtype], _stream()))
+
+
+def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse=None) -> None:
+    """Causal attention of packed sequences with grouped heads.
+
+    ``q`` [Tq, Hq, 128], ``k`` / ``v`` [Tk, Hkv, 128] (fp16 or bf16, any token
+    and head strides that are multiples of 8); sequence b has the rows
+    ``cu_seqlens_q[b]`` to ``cu_seqlens_q[b + 1]`` of q and the keys
+    ``cu_seqlens_k[b]`` to ``cu_seqlens_k[b + 1]`` (None: the same), and its
+    last row sees its last key.  ``output`` [Tq, Hq, 128] contiguous; ``lse``
+    (optional, float32 [Tq, Hq]) gets each row's log-sum-exp.  A row that sees
+    no key gives zeros and -inf; rows of no sequence are left as they were.  No
+    counterpart in the reference."""
+    _check_packed(q, "q", tuple(_DTYPES))
+    _check_packed(k, "k", q.dtype)
+    _check_packed(v, "v", q.dtype)
+    _check_tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+    _check_tensor(output, "output", q.dtype, 3)
+    tq, hq, d = q.shape
+    tk, hkv, _ = k.shape
+    if v.shape != k.shape:
+        raise RuntimeError("v shape must match k")
+    if output.shape != q.shape:
+        raise RuntimeError("output shape must match q")
+    b = cu_seqlens_q.size(0) - 1
+    if b < 0:
+        raise RuntimeError("cu_seqlens_q must hold B + 1 values")
+    ck = None
+    if cu_seqlens_k is not None:
+        _check_tensor(cu_seqlens_k, "cu_seqlens_k", torch.int32, 1)
+        if cu_seqlens_k.size(0) != b + 1:
+            raise RuntimeError("cu_seqlens_k batch mismatch")
+        ck = cu_seqlens_k.data_ptr()
+    ls = None
+    if lse is not None:
+        _check_tensor(lse, "lse", torch.float32, 2)
+        if lse.size(0) != tq or lse.size(1) != hq:
+            raise RuntimeError("lse must have shape [Tq, Hq]")
+        ls = lse.data_ptr()
+    _check_supported_gqa(hq, hkv)
+    _check_current_device(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse)
+    _native.check(_native.load().pkv_prompt_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(), ck, output.data_ptr(),
+        ls, b, tq, tk, hq, hkv, d, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+        v.stride(0), v.stride(1), _DTYPES[q.dtype], _stream()))
+
+
 def auto_workspace_bytes(batch: int, hq: int, hkv: int, sm_count: int = 0) -> int:
     """Workspace of ``paged_attention_auto`` (sm_count 0: the current device)."""
     return int(_native.load().pkv_auto_workspace_bytes(batch, hq, hkv, sm_count))
