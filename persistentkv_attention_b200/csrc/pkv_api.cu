@@ -165,10 +165,7 @@ pkv_status device_state(int* sm_count, unsigned** error_word) {
 namespace {
 
 // ------------------------------------------------------------ tensor maps
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using pkv_internal::EncodeTiledFn;
 
 EncodeTiledFn encode_fn() {
     static EncodeTiledFn fn = nullptr;
@@ -186,6 +183,14 @@ EncodeTiledFn encode_fn() {
     });
     return fn;
 }
+
+}  // namespace
+
+namespace pkv_internal {
+EncodeTiledFn encode_tiled() { return encode_fn(); }
+}  // namespace pkv_internal
+
+namespace {
 
 struct MapCacheEntry {
     const void* base = nullptr;

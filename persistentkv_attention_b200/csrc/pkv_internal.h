@@ -3,6 +3,8 @@
 // (both defined in pkv_api.cu).
 #pragma once
 
+#include <cuda.h>
+
 #include "../../include/pkv_b200.h"
 
 namespace pkv_internal {
@@ -13,5 +15,12 @@ pkv_status ok();
 
 // SM count and error word of the current device, which must be an sm_100 one.
 pkv_status device_state(int* sm_count, unsigned** error_word);
+
+// cuTensorMapEncodeTiled, reached at run time; null where it is unavailable.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled();
 
 }  // namespace pkv_internal

@@ -1,6 +1,8 @@
 // pkv_prompt.cu -- C ABI of the prompt side (declared in include/pkv_b200.h):
 // block tables and slot maps, K/V writes by slot, attention of packed prompts.
 // No counterpart in the reference, which decodes over pre-filled pools.
+#include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -8,7 +10,7 @@
 #include "../../include/pkv_b200.h"
 #include "pkv_cache_kernels.cuh"
 #include "pkv_internal.h"
-#include "pkv_prompt_kernels.cuh"
+#include "pkv_prompt_mma.cuh"
 
 using namespace pkv;
 using pkv_internal::device_state;
@@ -86,6 +88,65 @@ pkv_status grid_of(long long threads, int per_cta, unsigned* grid) {
     if (n > INT_MAX) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many tokens for one launch");
     *grid = (unsigned)n;
     return PKV_OK;
+}
+
+// The operand [T][H][128] as a 3-D tensor (element, head, token); one box is 64
+// elements (one 128-byte line) of 128 tokens of one head.
+pkv_status token_map(CUtensorMap* map, const void* base, int T, int H, long long tok_bytes,
+                     long long head_bytes, pkv_dtype dtype) {
+    const cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)H, (cuuint64_t)T};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_bytes, (cuuint64_t)tok_bytes};
+    const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)kPmTile};
+    const cuuint32_t elem[3] = {1u, 1u, 1u};
+    const pkv_internal::EncodeTiledFn fn = pkv_internal::encode_tiled();
+    if (fn == nullptr) return fail_fmt(PKV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const CUresult r = fn(map,
+                          dtype == PKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          3, const_cast<void*>(base), dims, strides, box, elem,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail_fmt(PKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return PKV_OK;
+}
+
+template <typename T>
+pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, cudaStream_t stream) {
+    CUtensorMap mq, mk, mv;
+    pkv_status st = token_map(&mq, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
+    // without keys no block is ever loaded: any valid map does
+    if (st == PKV_OK)
+        st = pp.Tk > 0 ? token_map(&mk, pp.k, pp.Tk, pp.Hkv, pp.k_tok, pp.k_head, dtype)
+                       : token_map(&mk, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
+    if (st == PKV_OK)
+        st = pp.Tk > 0 ? token_map(&mv, pp.v, pp.Tk, pp.Hkv, pp.v_tok, pp.v_head, dtype)
+                       : token_map(&mv, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
+    if (st != PKV_OK) return st;
+    auto kern = pkv_prompt_mma_kernel<T>;
+    static std::atomic<unsigned long long> attr_done{0ull};  // devices already set up
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(attr_done.load(std::memory_order_acquire) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPmSmemBytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail_fmt(PKV_ERR_CUDA, "cudaFuncSetAttribute failed: %s",
+                            cudaGetErrorString(e));
+        }
+        attr_done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const int G = pp.Hq / pp.Hkv;
+    const int rows = G == 1 ? 2 * kPmTile : kPmTile;
+    // every sequence has at most one tile that is not full
+    const long long tiles = std::min<long long>((long long)pp.Tq / rows + pp.B, pp.Tq);
+    unsigned grid = 0;
+    st = grid_of(tiles * (G == 1 ? pp.Hq : pp.Hq / 2), 1, &grid);
+    if (st != PKV_OK) return st;
+    kern<<<grid, kPmThreads, kPmSmemBytes, stream>>>(pp, mq, mk, mv);
+    return launched("prompt attention");
 }
 
 }  // namespace
@@ -247,15 +308,9 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
     int sms = 0;
     st = device_state(&sms, &pp.error);
     if (st != PKV_OK) return st;
-    unsigned grid = 0;
-    st = grid_of((long long)q_tokens * Hq * 32, 256, &grid);
-    if (st != PKV_OK) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == PKV_DTYPE_F16)
-        pkv_prompt_rows_kernel<__half><<<grid, 256, 0, s>>>(pp);
-    else
-        pkv_prompt_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(pp);
-    return launched("prompt attention");
+    return dtype == PKV_DTYPE_F16 ? launch_prompt<__half>(pp, dtype, s)
+                                  : launch_prompt<__nv_bfloat16>(pp, dtype, s);
 }
 
 }  // extern "C"

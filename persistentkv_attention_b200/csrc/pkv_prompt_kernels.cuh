@@ -95,38 +95,4 @@ __device__ __forceinline__ void prompt_row(const PromptParams& p, const uint8_t*
     if (lse != nullptr && lane == 0) *lse = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
-// The sequence of packed query row t: the last b with cu_q[b] <= t.
-__device__ __forceinline__ int prompt_sequence(const PromptParams& p, int t) {
-    int a = 0, z = p.B;
-    while (z - a > 1) {
-        const int m = (a + z) >> 1;
-        if (__ldg(p.cu_q + m) <= t) a = m; else z = m;
-    }
-    return a;
-}
-
-// One warp per (query row, head).
-template <typename T>
-__global__ void __launch_bounds__(256)
-    pkv_prompt_rows_kernel(const __grid_constant__ PromptParams p) {
-    const int lane = threadIdx.x & 31;
-    const long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
-    const int t = (int)(w / p.Hq), h = (int)(w % p.Hq);
-    if (t >= p.Tq) return;
-    const int b = prompt_sequence(p, t);
-    const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1);
-    const int k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
-    if (t < q0 || t >= q1) return;  // behind the last sequence
-    if (q0 < 0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {
-        if (lane == 0) raise_error(p.error, kErrIndex);
-        return;
-    }
-    const int n = max(0, min(k1 - k0, t - q0 + 1 + (k1 - k0) - (q1 - q0)));
-    const int kvh = h / (p.Hq / p.Hkv);
-    prompt_row<T>(p, p.q + t * p.q_tok + h * p.q_head, p.k + k0 * p.k_tok + kvh * p.k_head,
-                  p.v + k0 * p.v_tok + kvh * p.v_head, n,
-                  reinterpret_cast<T*>(p.out) + ((size_t)t * p.Hq + h) * kHeadDim,
-                  p.lse != nullptr ? p.lse + (size_t)t * p.Hq + h : nullptr, lane);
-}
-
 }  // namespace pkv
