@@ -371,8 +371,13 @@ pkv_status launch(LaunchSpec& ls, void* stream_ptr) {
     ls.dp.error = ds->error_word;
     ls.dp.stamps = ds->stamps;
     ls.sm_count = ds->sm_count;
-    if (ls.scale_block > 0)
-        return pkv_internal::launch_block8(ls, static_cast<cudaStream_t>(stream_ptr));
+    if (ls.scale_block > 0) {
+        cudaStream_t s = static_cast<cudaStream_t>(stream_ptr);
+        st = pkv_internal::launch_block8(ls, s);
+        if (st != PKV_OK || !ls.merge) return st;
+        return ls.dtype == PKV_DTYPE_F16 ? launch_merge_t<__half>(ls, s)
+                                         : launch_merge_t<__nv_bfloat16>(ls, s);
+    }
     ls.load = ls.kv8 ? kLoadCpAsync : g_gather_mode.load(std::memory_order_relaxed);
     ls.fma = g_math_mode.load(std::memory_order_relaxed) == PKV_MATH_FMA;
     CUtensorMap tk, tv;

@@ -13,62 +13,599 @@ struct Block8Params {
     int block;  // tokens per scale, a multiple of 16 that divides page_size
 };
 
-// One warp per (row, query head), straight from the formula.
-template <typename T>
-__global__ void __launch_bounds__(32)
-    pkv_block8_rows_kernel(const __grid_constant__ Block8Params bp) {
+// A ring slot holds 32 tokens of one KV head: 32 lines of 128 e4m3 values of K,
+// then of V, 16-byte chunk c of line t at position c ^ (t & 7); its two K and
+// two V scales sit beside the ring.
+constexpr int kB8Tokens = 32;
+constexpr int kB8Line = kHeadDim;              // bytes
+constexpr int kB8Half = kB8Tokens * kB8Line;   // K part of a slot
+static_assert(2 * kB8Half == kSlotBytes, "a slot is the 16-bit ring's slot");
+constexpr int kB8Box = 16;                     // tokens of one page lookup and one scale
+
+// The running maximum that weights refer to is raised only when a row's
+// maximum has grown by more than this many powers of two: weights stay below
+// 2^8 (fp16 holds 2^15), the accumulators are rescaled a few times per row
+// instead of every stage, and the division by the sum takes the factor out.
+constexpr float kB8Lazy = 8.0f;
+
+template <int G, int NSLOTS>
+constexpr size_t block8_smem_bytes() {
+    return decode_smem_bytes<G, NSLOTS>() + NSLOTS * 4 * sizeof(float);
+}
+
+// Two e4m3 values (the low or high half of a word) as two fp16 values: exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t word, bool high) {
+    uint32_t out;
+    const uint16_t h = (uint16_t)(high ? word >> 16 : word);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(out) : "h"(h));
+    return out;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr));
+    return v;
+}
+
+__device__ __forceinline__ float fast_log2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, bool valid) {
+    const uint32_t bytes = valid ? 4u : 0u;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(src),
+                 "r"(bytes)
+                 : "memory");
+}
+
+// Same work division as pkv_decode_kernel's device schedule: CTA g * Hkv + kvh
+// streams the row pieces of group g for one KV head, one producer warp and
+// four consumer warps, every 32-token stage to one warp.
+//
+// Mathematics.  With s_t the scaled score, b_t the V scale of token t's block
+// and p_t = exp(s_t + ln b_t - m):  O = sum p_t v_t / sum p_t / b_t, v_t the raw
+// e4m3 values.  So a V scale costs one add in a weight's exponent and one
+// factor in the sum, never touches the accumulators, and the running maximum
+// is that of a token's contribution s_t + ln b_t, so no block's scale can
+// push another's weights out of fp16's range.  A K scale is a factor of its
+// 16 tokens' scores.
+//
+// Both products run as mma.sync m16n8k16 on fp16 (every e4m3 value is exact in
+// it), 16 tokens x 8 heads and 128 dims x 8 heads.  A lane's 16-byte loads are
+// the fragments: the dims of a product's k index may come in any order that K
+// and Q share, and the dims of the output rows in any order at all, so chunk
+// 2 * (lane % 4) + h of a K line serves four k steps and chunk lane / 4 of two V
+// lines, bytes interleaved, eight output tiles.  No second pass over shared
+// memory and no transpose; that pass is what bounds the per-tensor route.
+// Bound: HBM, 256 bytes per token and KV head.
+template <int G, typename T, int NSLOTS>
+__global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
+    pkv_block8_kernel(const __grid_constant__ Block8Params bp) {
     const DecodeParams& p = bp.d;
-    const int lane = threadIdx.x;
-    const int h = blockIdx.x, b = blockIdx.y;
-    const int kvh = h / (p.Hq / p.Hkv);
-    const int qr = p.q_indices != nullptr ? __ldg(p.q_indices + b) : b;
-    const int orow = p.out_indices != nullptr ? __ldg(p.out_indices + b) : b;
-    if (qr < 0 || qr >= p.q_rows || orow < 0 || orow >= p.out_rows) {
-        if (lane == 0) raise_error(p.error, kErrIndex);
+    using Ops = ElemOps<T>;
+    constexpr int kBoxesPerStage = kB8Tokens / kB8Box;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_u32 = smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + (((raw_u32 + 1023u) & ~1023u) - raw_u32);
+    uint8_t* ring = smem;
+    uint8_t* s_q = ring + (size_t)NSLOTS * kSlotBytes;
+    float* s_merge = reinterpret_cast<float*>(s_q + kDescSlots * kQSlotBytes);
+    ItemDesc* s_desc = reinterpret_cast<ItemDesc*>(ring + merge_region_bytes<G, NSLOTS>());
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_desc + kDescSlots);
+    uint64_t* empty_bar = full_bar + NSLOTS;
+    uint64_t* desc_full = empty_bar + NSLOTS;
+    uint64_t* desc_empty = desc_full + kDescSlots;
+    uint64_t* merge_bar = desc_empty + kDescSlots;
+    uint8_t* s_flag_bytes = reinterpret_cast<uint8_t*>(merge_bar + 2);
+    volatile int* s_flags = reinterpret_cast<volatile int*>(s_flag_bytes);  // [0] abort
+    float* s_mstat = reinterpret_cast<float*>(s_flag_bytes + 64);
+    float* s_lstat = s_mstat + 2 * kConsumerWarps * 8;
+    float* s_mw = s_lstat + 2 * kConsumerWarps * 8;
+    PendingMerge* s_pend = reinterpret_cast<PendingMerge*>(s_mw + mw_floats<G>());
+    float* s_scale = reinterpret_cast<float*>(s_pend + kMaxPending);  // [NSLOTS][4]
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    decode_params_touch(p);
+    griddep_wait();
+    AutoCursor acur;
+    acur.b = acur.b_end = 0;
+    Item first_item;
+    int first_pid = -1;
+    __shared__ int s_my_items;
+    if (warp == kConsumerWarps) {
+        acur = auto_init(p, lane);
+        const int mine = acur.b >= 0 ? acur.b_end - acur.b : 0;
+        if (mine > 0) first_item = auto_item<kB8Box>(p, acur, lane, lane == 0, first_pid);
+        if (lane == 0) s_my_items = mine;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NSLOTS; ++s) {
+            mbar_init(&full_bar[s], 32);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int s = 0; s < kDescSlots; ++s) {
+            mbar_init(&desc_full[s], 33);  // 32 lanes' Q copies + the descriptor store
+            mbar_init(&desc_empty[s], kConsumerWarps);
+        }
+        mbar_init(merge_bar, 1);
+        s_flags[0] = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const int my_items = s_my_items;
+
+    if (warp == kConsumerWarps) {
+        // ============================ producer warp ============================
+        const uint64_t policy = l2_evict_first_policy();
+        const uint32_t ring_base = smem_u32(ring);
+        const uint32_t q_base = smem_u32(s_q);
+        const uint32_t scale_base = smem_u32(s_scale);
+        const int nblk = p.page_size / bp.block;
+        const int t_lane = lane >> 3, c_lane = lane & 7;  // lane's line (of 4) and chunk
+        uint32_t gstage = 0;
+        bool aborted = false;
+        int pid0 = first_pid;
+        Item cur = first_item;
+        auto give_up = [&]() {
+            if (lane == 0) {
+                s_flags[0] = 1;
+                raise_error(p.error, kErrTimeout);
+            }
+            aborted = true;
+        };
+        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+            bool ok = true;
+            if (lane == 0) ok = mbar_wait_bounded(bar, parity, s_flags);
+            return __shfl_sync(0xffffffffu, ok, 0) && s_flags[0] == 0;
+        };
+        for (int s = 0; s < my_items && !aborted; ++s) {
+            if (s == my_items - 1) griddep_launch_dependents();
+            const int e = s % kDescSlots;
+            if (s >= kDescSlots && !wait(&desc_empty[e], ((s / kDescSlots) - 1) & 1)) {
+                give_up();
+                break;
+            }
+            {
+                const bool qok = cur.q_row >= 0;
+                const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(p.q) +
+                                      ((size_t)(qok ? cur.q_row : 0) * p.Hq + (size_t)cur.kvh * G) *
+                                          kRowBytes;
+#pragma unroll
+                for (int c = lane; c < G * 16; c += 32)
+                    cp_async_16(q_base + e * kQSlotBytes + c * 16, qsrc + c * 16, qok ? 16u : 0u,
+                                policy);
+                cp_async_mbar_arrive_noinc(&desc_full[e]);
+                if (lane == 0) {
+                    ItemDesc& d = s_desc[e];
+                    d.row = cur.row;
+                    d.kvh = cur.kvh;
+                    d.split = cur.split;
+                    d.tok_begin = cur.tok_begin;
+                    d.tok_end = cur.tok_end;
+                    d.slot = cur.slot;
+                    d.row_splits = cur.row_splits;
+                    d.out_row = cur.out_row;
+                    mbar_arrive(&desc_full[e]);
+                }
+            }
+            const Item it = cur;
+            const int n_stages = ceil_div_i(it.tok_end - it.tok_begin, kB8Tokens);
+            const int n_boxes = ceil_div_i(it.tok_end - it.tok_begin, kB8Box);
+            const int32_t* bt_row = p.block_table + (size_t)it.row * p.max_pages;
+            const bool has_next = s + 1 < my_items;
+            bool fetched = !has_next;
+            Item nxt = it;
+            int nxt_pid = -1;
+            int pid_next = pid0;
+            // page lookups 32 boxes at a time, one per lane, one round ahead
+            for (int base = 0; base < n_boxes && !aborted; base += 32) {
+                const int box = base + lane;
+                const int tok = it.tok_begin + box * kB8Box;
+                const int pid = pid_next;
+                if (base + 32 < n_boxes)
+                    pid_next = box + 32 < n_boxes ? __ldg(bt_row + (tok + 32 * kB8Box) / p.page_size)
+                                                  : -1;
+                bool ok = box < n_boxes;
+                int y = 0, sc = 0;  // line and scale of the box
+                if (ok) {
+                    if (pid < 0 || pid >= p.num_pages) {
+                        ok = false;
+                        raise_error(p.error, kErrPageId);
+                    } else {
+                        const int head = pid * p.Hkv + it.kvh;
+                        const int off = tok % p.page_size;
+                        y = head * p.page_size + off;
+                        sc = head * nblk + off / bp.block;
+                    }
+                }
+                const int stages_here = min(32 / kBoxesPerStage, n_stages - base / kBoxesPerStage);
+                for (int st = 0; st < stages_here; ++st) {
+                    const uint32_t slot = gstage % NSLOTS;
+                    if (gstage >= (uint32_t)NSLOTS &&
+                        !wait(&empty_bar[slot], ((gstage / NSLOTS) - 1u) & 1u)) {
+                        give_up();
+                        break;
+                    }
+                    const int t0 = it.tok_begin + (base / kBoxesPerStage + st) * kB8Tokens;
+                    const uint32_t dst0 = ring_base + slot * kSlotBytes;
+#pragma unroll
+                    for (int bx = 0; bx < kBoxesPerStage; ++bx) {
+                        const int src = st * kBoxesPerStage + bx;
+                        const int yb = __shfl_sync(0xffffffffu, y, src);
+                        const int sb = __shfl_sync(0xffffffffu, sc, src);
+                        const bool okb = __shfl_sync(0xffffffffu, ok, src);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int t = bx * kB8Box + t_lane + 4 * k;
+                            const bool valid = okb && t0 + t < it.tok_end;
+                            const size_t off =
+                                (valid ? (size_t)(yb + t_lane + 4 * k) : 0) * kB8Line + c_lane * 16;
+                            const uint32_t dst = dst0 + t * kB8Line + ((c_lane ^ (t & 7)) << 4);
+                            const uint32_t bytes = valid ? 16u : 0u;
+                            cp_async_16(dst, p.k_pages + off, bytes, policy);
+                            cp_async_16(dst + kB8Half, p.v_pages + off, bytes, policy);
+                        }
+                        if (lane < 2)
+                            cp_async_4(scale_base + (slot * 4 + 2 * lane + bx) * 4,
+                                       (lane ? bp.v_scales : bp.k_scales) + (okb ? sb : 0), okb);
+                    }
+                    cp_async_mbar_arrive_noinc(&full_bar[slot]);
+                    ++gstage;
+                }
+                if (!fetched) {
+                    fetched = true;
+                    nxt = auto_item<kB8Box>(p, acur, lane, lane == 0, nxt_pid);
+                }
+            }
+            if (!fetched) nxt = auto_item<kB8Box>(p, acur, lane, lane == 0, nxt_pid);
+            cur = nxt;
+            pid0 = nxt_pid;
+        }
+        cp_async_wait_all();  // every copy lands before the CTA exits
         return;
     }
-    const int limit = p.max_pages * p.page_size;
-    int n = __ldg(p.seq_lens + b);
-    if (n > limit) {
-        if (lane == 0) raise_error(p.error, kErrLogicalPage);
-        n = limit;
-    }
-    float q[4];
-    const T* qrow = reinterpret_cast<const T*>(p.q) + ((size_t)qr * p.Hq + h) * kHeadDim;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = (float)qrow[4 * lane + i];
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int nblk = p.page_size / bp.block;
-    for (int t = 0; t < n; ++t) {
-        const int page = __ldg(p.block_table + (size_t)b * p.max_pages + t / p.page_size);
-        if (page < 0 || page >= p.num_pages) {
-            if (lane == 0) raise_error(p.error, kErrPageId);
-            continue;
+
+    // ============================== consumer warps ==============================
+    const int g8 = lane >> 2;         // token row of score tiles / head of B fragments
+    const int t4 = lane & 3;          // head pair of accumulators
+    const uint32_t ring_u32 = smem_u32(ring);
+    uint32_t gbase = 0;
+    int buf = 0;
+    bool aborted = false;
+    int n_pend = 0;
+    int pend_old = 0;
+    uint32_t merge_phase = 0u;
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool ok = mbar_wait_bounded(bar, parity, s_flags);
+        if (__all_sync(0xffffffffu, ok) && s_flags[0] == 0) return true;
+        if (lane == 0) {
+            s_flags[0] = 1;
+            raise_error(p.error, kErrTimeout);
         }
-        const int off = t % p.page_size;
-        const size_t head = (size_t)page * p.Hkv + kvh;
-        const size_t at = (head * p.page_size + off) * kHeadDim + 4 * lane;
-        const float ks = __ldg(bp.k_scales + head * nblk + off / bp.block);
-        const float vs = __ldg(bp.v_scales + head * nblk + off / bp.block);
-        const __nv_fp8_e4m3* k8 = reinterpret_cast<const __nv_fp8_e4m3*>(p.k_pages + at);
-        const __nv_fp8_e4m3* v8 = reinterpret_cast<const __nv_fp8_e4m3*>(p.v_pages + at);
-        float s = 0.f;
+        return false;
+    };
+
+    for (int s = 0; s < my_items; ++s) {
+        if (s == my_items - 1) griddep_launch_dependents();
+        const int e = s % kDescSlots;
+        Item it;
+        it.tok_begin = it.tok_end = 0;
+        it.row = it.kvh = it.split = 0;
+        it.slot = -1;
+        it.row_splits = 2;
+        it.out_row = -1;
+        uint32_t qf[8][2];
+        float qs[2] = {0.f, 0.f};  // score factor of this lane's two heads
+        if (!aborted) aborted = !wait(&desc_full[e], (s / kDescSlots) & 1);
+        if (!aborted) {
+            const ItemDesc& d = s_desc[e];
+            it.row = d.row;
+            it.kvh = d.kvh;
+            it.split = d.split;
+            it.tok_begin = d.tok_begin;
+            it.tok_end = d.tok_end;
+            it.slot = d.slot;
+            it.row_splits = d.row_splits;
+            it.out_row = d.out_row;
+            // Q^T as the B operand: k step 4 h + u holds dims 16 (2 t4 + h) + 4 u + 0 .. 3
+            // of head g8 (zeros beyond the G heads)
+            const uint8_t* qrow = s_q + e * kQSlotBytes + (g8 < G ? g8 : 0) * kRowBytes;
+            uint4 raw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s = fmaf(q[i], (float)k8[i], s);
+            for (int i = 0; i < 4; ++i)
+                raw[i] = g8 < G ? *reinterpret_cast<const uint4*>(qrow + t4 * 64 + i * 16)
+                                : make_uint4(0u, 0u, 0u, 0u);
+            float unit = 1.f;
+            if constexpr (Ops::kSplitP) {
+                // bf16 queries in fp16: the head's row is brought to [2^8, 2^9) by
+                // a power of two, so all 8 bits of every element that matters are
+                // kept (one 2^32 below the largest underflows)
+                float amax = 0.f;
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= ks * p.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float corr = fast_exp2(m - mn), w = fast_exp2(s - mn);
-        m = mn;
-        l = l * corr + w;
+                for (int i = 0; i < 16; ++i) {
+                    const float2 f =
+                        __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+                    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                int ex = (int)(__float_as_uint(amax) >> 23) - 127 - 8;
+                if (!(amax > 0.f) || !(amax < INFINITY)) ex = 0;
+                if (ex < -126) ex = -126;
+                const float down = __uint_as_float((unsigned)(127 - ex) << 23);
+                unit = __uint_as_float((unsigned)(127 + ex) << 23);
+                uint32_t* wm = reinterpret_cast<uint32_t*>(raw);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * corr + w * vs * (float)v8[i];
+                for (int i = 0; i < 16; ++i) {
+                    const float2 f =
+                        __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wm[i]));
+                    wm[i] = ElemOps<__half>::pack(f.x * down, f.y * down);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 a = raw[2 * h], b = raw[2 * h + 1];
+                qf[4 * h][0] = a.x;
+                qf[4 * h][1] = a.y;
+                qf[4 * h + 1][0] = a.z;
+                qf[4 * h + 1][1] = a.w;
+                qf[4 * h + 2][0] = b.x;
+                qf[4 * h + 2][1] = b.y;
+                qf[4 * h + 3][0] = b.z;
+                qf[4 * h + 3][1] = b.w;
+            }
+            // the accumulators' heads are 2 t4 and 2 t4 + 1; head g sits in lanes 4 g
+            qs[0] = p.scale_log2 * __shfl_sync(0xffffffffu, unit, 8 * t4);
+            qs[1] = p.scale_log2 * __shfl_sync(0xffffffffu, unit, 8 * t4 + 4);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&desc_empty[e]);
+        }
+        const int n_stages = aborted ? 0 : ceil_div_i(it.tok_end - it.tok_begin, kB8Tokens);
+
+        float m_run[2] = {-INFINITY, -INFINITY};
+        float l_run[2] = {0.f, 0.f};
+        float acc[8][4];
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
+
+        for (int j = warp; j < n_stages; j += kConsumerWarps) {
+            const uint32_t gs = gbase + (uint32_t)j;
+            const uint32_t slot = gs % NSLOTS;
+            if (!aborted) aborted = !wait(&full_bar[slot], (gs / NSLOTS) & 1u);
+            if (aborted) break;
+            const int valid = min(kB8Tokens, it.tok_end - (it.tok_begin + j * kB8Tokens));
+            const uint32_t kbase = ring_u32 + slot * kSlotBytes;
+            const float4 scales = *reinterpret_cast<const float4*>(s_scale + slot * 4);
+
+            // ---- S^T: 2 x [16 tokens x 8 heads]
+            float sc[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int chunk = 2 * t4 + h;
+                    const uint32_t at = kbase + (16 * i + g8) * kB8Line + ((chunk ^ g8) << 4);
+                    const uint4 lo = lds128(at);                // token 16 i + g8
+                    const uint4 hi = lds128(at + 8 * kB8Line);  // token 16 i + g8 + 8
+                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w};
+                    const uint32_t wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t a[4] = {
+                            e4m3x2_to_f16x2(wl[u], false), e4m3x2_to_f16x2(wh[u], false),
+                            e4m3x2_to_f16x2(wl[u], true), e4m3x2_to_f16x2(wh[u], true)};
+                        ElemOps<__half>::mma(c, a, qf[4 * h + u][0], qf[4 * h + u][1]);
+                    }
+                }
+                const float ks = i == 0 ? scales.x : scales.y;
+                const float vs = i == 0 ? scales.z : scales.w;
+                // a block of zeros (scale 0) still counts in the sum: its scale
+                // becomes 2^-100, far below any weight's contribution
+                const float lg = vs == 0.f ? -100.f : fast_log2(vs);
+                const float f0 = qs[0] * ks, f1 = qs[1] * ks;
+                const bool ok0 = 16 * i + g8 < valid, ok1 = 16 * i + g8 + 8 < valid;
+                sc[i][0] = ok0 ? fmaf(c[0], f0, lg) : -INFINITY;
+                sc[i][1] = ok0 ? fmaf(c[1], f1, lg) : -INFINITY;
+                sc[i][2] = ok1 ? fmaf(c[2], f0, lg) : -INFINITY;
+                sc[i][3] = ok1 ? fmaf(c[3], f1, lg) : -INFINITY;
+            }
+            // ---- running maximum (log2 domain) of heads 2 t4 and 2 t4 + 1
+            float top[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(fmaxf(sc[0][h], sc[0][2 + h]), fmaxf(sc[1][h], sc[1][2 + h]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                top[h] = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            }
+            const bool move0 = top[0] - m_run[0] > kB8Lazy, move1 = top[1] - m_run[1] > kB8Lazy;
+            if (__any_sync(0xffffffffu, move0 || move1)) {
+                const float c0 = move0 ? fast_exp2(m_run[0] - top[0]) : 1.f;
+                const float c1 = move1 ? fast_exp2(m_run[1] - top[1]) : 1.f;
+                if (move0) m_run[0] = top[0];
+                if (move1) m_run[1] = top[1];
+                l_run[0] *= c0;
+                l_run[1] *= c1;
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt) {
+                    acc[mt][0] *= c0;
+                    acc[mt][1] *= c1;
+                    acc[mt][2] *= c0;
+                    acc[mt][3] *= c1;
+                }
+            }
+            // ---- weights, and O^T[128 x 8 heads] += V^T . P^T
+            const float b0 = m_run[0] == -INFINITY ? 0.f : m_run[0];
+            const float b1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float vs = i == 0 ? scales.z : scales.w;
+                // (a masked block's scale may be anything: fmaxf drops a NaN, and a
+                // weight of 0 must not meet an infinity)
+                const float inv = 1.f / fmaxf(vs, 0x1p-100f);
+                float pr[4];
+                pr[0] = fast_exp2(sc[i][0] - b0);
+                pr[1] = fast_exp2(sc[i][1] - b1);
+                pr[2] = fast_exp2(sc[i][2] - b0);
+                pr[3] = fast_exp2(sc[i][3] - b1);
+                l_run[0] = fmaf(pr[0] + pr[2], inv, l_run[0]);
+                l_run[1] = fmaf(pr[1] + pr[3], inv, l_run[1]);
+                const uint32_t pb0 = movmatrix_trans(ElemOps<__half>::pack(pr[0], pr[1]));
+                const uint32_t pb1 = movmatrix_trans(ElemOps<__half>::pack(pr[2], pr[3]));
+                // tokens 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9; chunk g8 holds the dims
+                // 16 g8 + 2 mt + (0, 1) of output tile mt's rows g8 and g8 + 8
+                const int tok = 16 * i + 2 * t4;
+                const uint32_t at = kbase + kB8Half + tok * kB8Line;
+                const uint32_t x0 = (uint32_t)((g8 ^ (2 * t4)) << 4);
+                const uint32_t x1 = (uint32_t)((g8 ^ (2 * t4 + 1)) << 4);
+                const uint4 va = lds128(at + x0);
+                const uint4 vb = lds128(at + kB8Line + x1);
+                const uint4 vc = lds128(at + 8 * kB8Line + x0);
+                const uint4 vd = lds128(at + 9 * kB8Line + x1);
+                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+                const uint32_t wc[4] = {vc.x, vc.y, vc.z, vc.w}, wd[4] = {vd.x, vd.y, vd.z, vd.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        // bytes 2 o, 2 o + 1 of both tokens' words, interleaved
+                        const uint32_t lo = __byte_perm(wa[u], wb[u], o == 0 ? 0x5140 : 0x7362);
+                        const uint32_t hi = __byte_perm(wc[u], wd[u], o == 0 ? 0x5140 : 0x7362);
+                        const uint32_t a[4] = {
+                            e4m3x2_to_f16x2(lo, false), e4m3x2_to_f16x2(lo, true),
+                            e4m3x2_to_f16x2(hi, false), e4m3x2_to_f16x2(hi, true)};
+                        ElemOps<__half>::mma(acc[2 * u + o], a, pb0, pb1);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_bar[slot]);
+        }
+        gbase += (uint32_t)n_stages;
+
+        // ---- combine the four warps' states of this item
+        float* mbuf = s_merge + buf * DecodeSmem<G>::kMergeFloats;
+        float* mstat = s_mstat + buf * kConsumerWarps * 8;
+        float* lstat = s_lstat + buf * kConsumerWarps * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 4);
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 8);
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 16);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int g = 2 * t4 + h;
+                if (g < G)
+                    *reinterpret_cast<float2*>(
+                        mbuf + (warp * G + g) * DecodeSmem<G>::kMergeStride + 16 * g8 + 2 * mt) =
+                        make_float2(acc[mt][h], acc[mt][2 + h]);
+            }
+        }
+        if (lane < 4) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int g = 2 * lane + h;
+                if (g < G) {
+                    mstat[warp * 8 + g] = m_run[h];
+                    lstat[warp * 8 + g] = l_run[h];
+                }
+            }
+        }
+        consumer_bar_sync();
+        const bool direct = it.row_splits == 1;
+#pragma unroll 1
+        for (int idx = threadIdx.x; idx < G * kHeadDim; idx += kConsumerWarps * 32) {
+            const int g = idx / kHeadDim;
+            const int d = idx % kHeadDim;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kConsumerWarps; ++w) mx = fmaxf(mx, mstat[w * 8 + g]);
+            float lsum = 0.f, osum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kConsumerWarps; ++w) {
+                const float mw = mstat[w * 8 + g];
+                const float wt = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
+                lsum = fmaf(wt, lstat[w * 8 + g], lsum);
+                osum = fmaf(wt, mbuf[(w * G + g) * DecodeSmem<G>::kMergeStride + d], osum);
+            }
+            if (direct) {
+                if (it.out_row >= 0 && !aborted) {
+                    T* orow = reinterpret_cast<T*>(p.out) +
+                              ((size_t)it.out_row * p.Hq + (size_t)it.kvh * G + g) * kHeadDim;
+                    orow[d] = Ops::from_float(osum * (lsum == 0.f ? 0.f : 1.f / lsum));
+                }
+            } else if (it.slot >= 0) {
+                const size_t si = ((size_t)it.kvh * p.total_slots + it.slot) * G + g;
+                p.part_acc[si * kHeadDim + d] = osum;
+                if (d == 0) {
+                    p.part_m[si] = mx == -INFINITY ? kNegFltMax : mx * kLn2;
+                    p.part_l[si] = lsum;
+                }
+            }
+        }
+        if (!direct && it.slot >= 0 && p.merge_counters != nullptr) {
+            // fused merge, deferred to the CTA's end (a group holds at most two
+            // split rows: its first and its last)
+            int32_t* ctr = p.merge_counters + (size_t)it.row * p.Hkv + it.kvh;
+            consumer_bar_sync();
+            if (n_pend < kMaxPending) {
+                if (threadIdx.x == 0) {
+                    if (n_pend > 0) s_pend[n_pend - 1].old = pend_old;
+                    PendingMerge& pe = s_pend[n_pend];
+                    pe.row = it.row;
+                    pe.kvh = it.kvh;
+                    pe.s0 = it.slot - it.split;
+                    pe.n = it.row_splits;
+                    pe.out_row = it.out_row;
+                    pend_old = atom_add_acq_rel_gpu(ctr, 1);
+                }
+                ++n_pend;
+            } else if (threadIdx.x == 0) {
+                raise_error(p.error, kErrSlot);
+            }
+        }
+        buf ^= 1;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    T* o = reinterpret_cast<T*>(p.out) + ((size_t)orow * p.Hq + h) * kHeadDim;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[4 * lane + i] = ElemOps<T>::from_float(acc[i] * inv);
+    if (n_pend > 0) {
+        if (threadIdx.x == 0) s_pend[n_pend - 1].old = pend_old;
+        fence_proxy_async_smem();
+        consumer_bar_sync();
+#pragma unroll 1
+        for (int k = 0; k < n_pend; ++k) {
+            const PendingMerge pe = s_pend[k];
+            if (pe.old != pe.n - 1) continue;
+            if (threadIdx.x == 0) p.merge_counters[(size_t)pe.row * p.Hkv + pe.kvh] = 0;
+            if (aborted || s_flags[0] != 0) continue;
+            if (pe.n * G <= kMergeWeights) {
+                merge_bulk<G, T>(p, pe, ring, (uint32_t)merge_region_bytes<G, NSLOTS>(), s_mw,
+                                 merge_bar, merge_phase, s_flags);
+            } else {
+                // more slots than the weight buffer holds: the chunked merge
+                MergeSmem ms{s_mw, s_mw + kMergeChunk * 8, s_merge};
+                const size_t sb = ((size_t)pe.kvh * p.total_slots + pe.s0) * G;
+                T* o = pe.out_row >= 0 ? reinterpret_cast<T*>(p.out) +
+                                             ((size_t)pe.out_row * p.Hq + pe.kvh * G) * kHeadDim
+                                       : nullptr;
+                const XgSink unused{};
+                merge_slots<G, T, kConsumerWarps, true, false>(
+                    p.part_m + sb, p.part_l + sb, p.part_acc + sb * kHeadDim, 0, pe.n, G, 0, ms, o,
+                    nullptr, unused);
+                fence_proxy_async_smem();
+                consumer_bar_sync();
+            }
+        }
+    }
 }
 
 }  // namespace pkv
