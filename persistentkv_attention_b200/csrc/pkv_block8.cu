@@ -5,10 +5,32 @@
 namespace pkv_internal {
 namespace {
 
-template <int G, typename T>
+
+// A pool of e4m3 lines, [lines][128 bytes]; one box is `box` lines.
+pkv_status line_map(CUtensorMap* map, const void* base, long long lines, int box) {
+    const cuuint64_t dims[2] = {(cuuint64_t)pkv::kB8Line, (cuuint64_t)lines};
+    const cuuint64_t strides[1] = {(cuuint64_t)pkv::kB8Line};
+    const cuuint32_t boxes[2] = {(cuuint32_t)pkv::kB8Line, (cuuint32_t)box};
+    const cuuint32_t elem[2] = {1u, 1u};
+    const EncodeTiledFn fn = encode_tiled();
+    if (fn == nullptr) return fail_fmt(PKV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                          strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail_fmt(PKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return PKV_OK;
+}
+
+template <int G, typename T, int BOX>
 pkv_status launch_typed8(const LaunchSpec& ls, cudaStream_t stream) {
     using namespace pkv;
-    auto kern = pkv_block8_kernel<G, T, kSlots>;
+    CUtensorMap tk, tv;
+    pkv_status st = line_map(&tk, ls.k, ls.rows, BOX);
+    if (st == PKV_OK) st = line_map(&tv, ls.v, ls.rows, BOX);
+    if (st != PKV_OK) return st;
+    auto kern = pkv_block8_kernel<G, T, BOX, kSlots>;
     const size_t smem = block8_smem_bytes<G, kSlots>();
     // the device schedule's grid (2 CTAs per SM) must be resident in one wave
     static_assert(2 * (block8_smem_bytes<G, kSlots>() + 1024) <= 228 * 1024,
@@ -42,7 +64,7 @@ pkv_status launch_typed8(const LaunchSpec& ls, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ls.pdl ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, bp);
+    e = cudaLaunchKernelEx(&cfg, kern, bp, tk, tv);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail_fmt(PKV_ERR_CUDA, "decode launch failed: %s", cudaGetErrorString(e));
@@ -50,13 +72,20 @@ pkv_status launch_typed8(const LaunchSpec& ls, cudaStream_t stream) {
     return ok();
 }
 
+// Copies of 32 tokens where pages hold whole ones, else of 16.
+template <int G, typename T>
+pkv_status launch_box8(const LaunchSpec& ls, cudaStream_t stream) {
+    return ls.dp.page_size % 32 == 0 ? launch_typed8<G, T, 32>(ls, stream)
+                                     : launch_typed8<G, T, 16>(ls, stream);
+}
+
 template <typename T>
 pkv_status launch_g8(const LaunchSpec& ls, cudaStream_t stream) {
     switch (ls.G) {
-        case 1: return launch_typed8<1, T>(ls, stream);
-        case 2: return launch_typed8<2, T>(ls, stream);
-        case 4: return launch_typed8<4, T>(ls, stream);
-        case 8: return launch_typed8<8, T>(ls, stream);
+        case 1: return launch_box8<1, T>(ls, stream);
+        case 2: return launch_box8<2, T>(ls, stream);
+        case 4: return launch_box8<4, T>(ls, stream);
+        case 8: return launch_box8<8, T>(ls, stream);
         default: return fail_fmt(PKV_ERR_UNSUPPORTED, "unsupported G=%d", ls.G);
     }
 }

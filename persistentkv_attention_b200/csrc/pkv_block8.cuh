@@ -10,7 +10,7 @@ struct Block8Params {
     DecodeParams d;
     const float* k_scales;  // [P][Hkv][page / block]
     const float* v_scales;
-    int block;  // tokens per scale, a multiple of 16 that divides page_size
+    int block;     // tokens per scale, a multiple of 16 that divides page_size
 };
 
 // A ring slot holds 32 tokens of one KV head: 32 lines of 128 e4m3 values of K,
@@ -20,7 +20,7 @@ constexpr int kB8Tokens = 32;
 constexpr int kB8Line = kHeadDim;              // bytes
 constexpr int kB8Half = kB8Tokens * kB8Line;   // K part of a slot
 static_assert(2 * kB8Half == kSlotBytes, "a slot is the 16-bit ring's slot");
-constexpr int kB8Box = 16;                     // tokens of one page lookup and one scale
+constexpr int kB8Scale = 16;                   // tokens that share a scale at least
 
 // The running maximum that weights refer to is raised only when a row's
 // maximum has grown by more than this many powers of two: weights stay below
@@ -28,9 +28,22 @@ constexpr int kB8Box = 16;                     // tokens of one page lookup and 
 // instead of every stage, and the division by the sum takes the factor out.
 constexpr float kB8Lazy = 8.0f;
 
+// What the producer resolves a round at a time (up to 16 stages of one item,
+// up to 32 page lookups): pool lines of the round's copies, and the scales of
+// its stages, {K, K, V, V} each.  Several rounds' scales are kept, so that
+// short rows do not wait for one another.
+constexpr int kB8Round = 16;  // stages
+constexpr int kB8Rounds = kDescSlots;
+static_assert((kB8Rounds & (kB8Rounds - 1)) == 0, "rounds are counted by masks");
+struct B8Lookups {
+    float scales[kB8Rounds][kB8Round][4];
+    int lines[32];  // -1: no page
+    uint64_t scales_full[kB8Rounds];
+};
+
 template <int G, int NSLOTS>
 constexpr size_t block8_smem_bytes() {
-    return decode_smem_bytes<G, NSLOTS>() + NSLOTS * 4 * sizeof(float);
+    return decode_smem_bytes<G, NSLOTS>() + sizeof(B8Lookups);
 }
 
 // Two e4m3 values (the low or high half of a word) as two fp16 values: exact.
@@ -55,6 +68,7 @@ __device__ __forceinline__ float fast_log2(float x) {
     return y;
 }
 
+// A scale, copied asynchronously.
 __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, bool valid) {
     const uint32_t bytes = valid ? 4u : 0u;
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(src),
@@ -82,12 +96,19 @@ __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, b
 // lines, bytes interleaved, eight output tiles.  No second pass over shared
 // memory and no transpose; that pass is what bounds the per-tensor route.
 // Bound: HBM, 256 bytes per token and KV head.
-template <int G, typename T, int NSLOTS>
+template <int G, typename T, int BOX, int NSLOTS>
 __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
-    pkv_block8_kernel(const __grid_constant__ Block8Params bp) {
+    pkv_block8_kernel(const __grid_constant__ Block8Params bp,
+                      const __grid_constant__ CUtensorMap tmap_k,
+                      const __grid_constant__ CUtensorMap tmap_v) {
+    static_assert(BOX == 16 || BOX == 32, "box rows");
+    // A slot belongs to one consumer warp for good: a barrier's parity cannot
+    // tell a phase from the one two before it, so a warp must not wait for a
+    // slot's next use while another still owes its last one.
+    static_assert(NSLOTS % kConsumerWarps == 0, "every use of a slot is one warp's");
     const DecodeParams& p = bp.d;
     using Ops = ElemOps<T>;
-    constexpr int kBoxesPerStage = kB8Tokens / kB8Box;
+    constexpr int kBoxesPerStage = kB8Tokens / BOX;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -107,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
     float* s_lstat = s_mstat + 2 * kConsumerWarps * 8;
     float* s_mw = s_lstat + 2 * kConsumerWarps * 8;
     PendingMerge* s_pend = reinterpret_cast<PendingMerge*>(s_mw + mw_floats<G>());
-    float* s_scale = reinterpret_cast<float*>(s_pend + kMaxPending);  // [NSLOTS][4]
+    B8Lookups* s_look = reinterpret_cast<B8Lookups*>(s_pend + kMaxPending);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -121,12 +142,12 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
     if (warp == kConsumerWarps) {
         acur = auto_init(p, lane);
         const int mine = acur.b >= 0 ? acur.b_end - acur.b : 0;
-        if (mine > 0) first_item = auto_item<kB8Box>(p, acur, lane, lane == 0, first_pid);
+        if (mine > 0) first_item = auto_item<BOX>(p, acur, lane, lane == 0, first_pid);
         if (lane == 0) s_my_items = mine;
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < NSLOTS; ++s) {
-            mbar_init(&full_bar[s], 32);
+            mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
         for (int s = 0; s < kDescSlots; ++s) {
@@ -134,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
             mbar_init(&desc_empty[s], kConsumerWarps);
         }
         mbar_init(merge_bar, 1);
+        for (int r = 0; r < kB8Rounds; ++r) mbar_init(&s_look->scales_full[r], 32);
         s_flags[0] = 0;
         fence_mbar_init();
     }
@@ -143,12 +165,15 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
     if (warp == kConsumerWarps) {
         // ============================ producer warp ============================
         const uint64_t policy = l2_evict_first_policy();
-        const uint32_t ring_base = smem_u32(ring);
         const uint32_t q_base = smem_u32(s_q);
-        const uint32_t scale_base = smem_u32(s_scale);
         const int nblk = p.page_size / bp.block;
-        const int t_lane = lane >> 3, c_lane = lane & 7;  // lane's line (of 4) and chunk
-        uint32_t gstage = 0;
+        if (lane == 0) {
+            tma_prefetch_map(&tmap_k);
+            tma_prefetch_map(&tmap_v);
+        }
+        uint32_t gstage = 0, ground = 0;
+        uint32_t round_end[kB8Rounds] = {0u, 0u, 0u, 0u};  // of the rounds before, oldest first
+        uint32_t round_len[kB8Rounds] = {0u, 0u, 0u, 0u};
         bool aborted = false;
         int pid0 = first_pid;
         Item cur = first_item;
@@ -196,23 +221,26 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
             }
             const Item it = cur;
             const int n_stages = ceil_div_i(it.tok_end - it.tok_begin, kB8Tokens);
-            const int n_boxes = ceil_div_i(it.tok_end - it.tok_begin, kB8Box);
+            const int n_boxes = ceil_div_i(it.tok_end - it.tok_begin, BOX);
             const int32_t* bt_row = p.block_table + (size_t)it.row * p.max_pages;
             const bool has_next = s + 1 < my_items;
             bool fetched = !has_next;
             Item nxt = it;
             int nxt_pid = -1;
             int pid_next = pid0;
-            // page lookups 32 boxes at a time, one per lane, one round ahead
-            for (int base = 0; base < n_boxes && !aborted; base += 32) {
+            // page lookups a round at a time, one per lane, one round ahead
+            constexpr int kRoundBoxes = kB8Round * kBoxesPerStage;
+            for (int base = 0; base < n_boxes && !aborted; base += kRoundBoxes) {
                 const int box = base + lane;
-                const int tok = it.tok_begin + box * kB8Box;
+                const int tok = it.tok_begin + box * BOX;
                 const int pid = pid_next;
-                if (base + 32 < n_boxes)
-                    pid_next = box + 32 < n_boxes ? __ldg(bt_row + (tok + 32 * kB8Box) / p.page_size)
-                                                  : -1;
-                bool ok = box < n_boxes;
-                int y = 0, sc = 0;  // line and scale of the box
+                if (base + kRoundBoxes < n_boxes)
+                    pid_next = box + kRoundBoxes < n_boxes
+                                   ? __ldg(bt_row + (tok + kRoundBoxes * BOX) / p.page_size)
+                                   : -1;
+                bool ok = lane < kRoundBoxes && box < n_boxes;
+                int y = -1;               // line of the box in the pool
+                int sc = 0, sc_step = 0;  // scales of the box's one or two 16-token parts
                 if (ok) {
                     if (pid < 0 || pid >= p.num_pages) {
                         ok = false;
@@ -222,52 +250,104 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                         const int off = tok % p.page_size;
                         y = head * p.page_size + off;
                         sc = head * nblk + off / bp.block;
+                        sc_step = BOX > kB8Scale && bp.block == kB8Scale ? 1 : 0;
                     }
                 }
-                const int stages_here = min(32 / kBoxesPerStage, n_stages - base / kBoxesPerStage);
-                for (int st = 0; st < stages_here; ++st) {
-                    const uint32_t slot = gstage % NSLOTS;
-                    if (gstage >= (uint32_t)NSLOTS &&
-                        !wait(&empty_bar[slot], ((gstage / NSLOTS) - 1u) & 1u)) {
+                // the scales go where those of the round kB8Rounds before are: every
+                // stage of it must have been consumed (one that the ring has issued
+                // a successor of has been)
+                {
+                    const uint32_t g = round_end[0] - 1u - (uint32_t)lane;
+                    bool free = true;
+                    if ((uint32_t)lane < round_len[0] && gstage <= g + NSLOTS)
+                        free = mbar_wait_bounded(&empty_bar[g % NSLOTS], (g / NSLOTS) & 1u, s_flags);
+                    if (!__all_sync(0xffffffffu, free)) {
                         give_up();
                         break;
                     }
-                    const int t0 = it.tok_begin + (base / kBoxesPerStage + st) * kB8Tokens;
-                    const uint32_t dst0 = ring_base + slot * kSlotBytes;
-#pragma unroll
-                    for (int bx = 0; bx < kBoxesPerStage; ++bx) {
-                        const int src = st * kBoxesPerStage + bx;
-                        const int yb = __shfl_sync(0xffffffffu, y, src);
-                        const int sb = __shfl_sync(0xffffffffu, sc, src);
-                        const bool okb = __shfl_sync(0xffffffffu, ok, src);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int t = bx * kB8Box + t_lane + 4 * k;
-                            const bool valid = okb && t0 + t < it.tok_end;
-                            const size_t off =
-                                (valid ? (size_t)(yb + t_lane + 4 * k) : 0) * kB8Line + c_lane * 16;
-                            const uint32_t dst = dst0 + t * kB8Line + ((c_lane ^ (t & 7)) << 4);
-                            const uint32_t bytes = valid ? 16u : 0u;
-                            cp_async_16(dst, p.k_pages + off, bytes, policy);
-                            cp_async_16(dst + kB8Half, p.v_pages + off, bytes, policy);
-                        }
-                        if (lane < 2)
-                            cp_async_4(scale_base + (slot * 4 + 2 * lane + bx) * 4,
-                                       (lane ? bp.v_scales : bp.k_scales) + (okb ? sb : 0), okb);
-                    }
-                    cp_async_mbar_arrive_noinc(&full_bar[slot]);
-                    ++gstage;
                 }
+                if (lane < kRoundBoxes) {
+                    // a missing box has scale 0
+                    const uint32_t at =
+                        smem_u32(&s_look->scales[ground & (kB8Rounds - 1)][lane / kBoxesPerStage][0]) +
+                                        (lane % kBoxesPerStage) * (BOX / kB8Scale) * 4;
+#pragma unroll
+                    for (int h = 0; h < BOX / kB8Scale; ++h) {
+                        cp_async_4(at + 4 * h, bp.k_scales + sc + h * sc_step, ok);
+                        cp_async_4(at + 8 + 4 * h, bp.v_scales + sc + h * sc_step, ok);
+                    }
+                }
+                cp_async_mbar_arrive_noinc(&s_look->scales_full[ground & (kB8Rounds - 1)]);
+                ++ground;
+                s_look->lines[lane] = y;
+                __syncwarp();
+                const int stages_here = min(kB8Round, n_stages - base / kBoxesPerStage);
+                bool ok_stages = true;
+                if (lane == 0) {
+                    // one thread issues the round's copies
+                    for (int st = 0; st < stages_here; ++st) {
+                        const uint32_t gs = gstage + st;
+                        const uint32_t slot = gs % NSLOTS;
+                        int line[kBoxesPerStage];
+                        uint32_t bytes = 0;
+#pragma unroll
+                        for (int bx = 0; bx < kBoxesPerStage; ++bx) {
+                            line[bx] = s_look->lines[st * kBoxesPerStage + bx];
+                            bytes += line[bx] >= 0 ? 2u * BOX * kB8Line : 0u;
+                        }
+                        if (gs >= (uint32_t)NSLOTS &&
+                            !mbar_wait_bounded(&empty_bar[slot], ((gs / NSLOTS) - 1u) & 1u,
+                                               s_flags)) {
+                            ok_stages = false;
+                            gstage = gs;  // what was issued, for the drain
+                            break;
+                        }
+                        mbar_arrive_expect_tx(&full_bar[slot], bytes);
+                        uint8_t* dst = ring + (size_t)slot * kSlotBytes;
+#pragma unroll
+                        for (int bx = 0; bx < kBoxesPerStage; ++bx) {
+                            if (line[bx] >= 0) {
+                                tma_load_2d(dst + bx * BOX * kB8Line, &tmap_k, 0, line[bx],
+                                            &full_bar[slot], policy);
+                                tma_load_2d(dst + kB8Half + bx * BOX * kB8Line, &tmap_v, 0, line[bx],
+                                            &full_bar[slot], policy);
+                            }
+                        }
+                    }
+                }
+                ok_stages = __shfl_sync(0xffffffffu, ok_stages, 0);
+                if (!ok_stages) {
+                    give_up();
+                    break;
+                }
+                gstage += stages_here;
+#pragma unroll
+                for (int r = 0; r + 1 < kB8Rounds; ++r) {
+                    round_end[r] = round_end[r + 1];
+                    round_len[r] = round_len[r + 1];
+                }
+                round_end[kB8Rounds - 1] = gstage;
+                round_len[kB8Rounds - 1] = stages_here;
                 if (!fetched) {
                     fetched = true;
-                    nxt = auto_item<kB8Box>(p, acur, lane, lane == 0, nxt_pid);
+                    nxt = auto_item<BOX>(p, acur, lane, lane == 0, nxt_pid);
                 }
             }
-            if (!fetched) nxt = auto_item<kB8Box>(p, acur, lane, lane == 0, nxt_pid);
+            if (!fetched) nxt = auto_item<BOX>(p, acur, lane, lane == 0, nxt_pid);
             cur = nxt;
             pid0 = nxt_pid;
         }
-        cp_async_wait_all();  // every copy lands before the CTA exits
+        // Drain: every copy this warp issued lands before the CTA exits.
+        cp_async_wait_all();
+        if (lane == 0) {
+            const uint32_t first = gstage > (uint32_t)NSLOTS ? gstage - NSLOTS : 0u;
+            for (uint32_t g = first; g < gstage; ++g) {
+                if (!mbar_wait_bounded(&full_bar[g % NSLOTS], (g / NSLOTS) & 1u, nullptr)) {
+                    raise_error(p.error, kErrTimeout);
+                    break;
+                }
+            }
+        }
         return;
     }
 
@@ -276,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
     const int t4 = lane & 3;          // head pair of accumulators
     const uint32_t ring_u32 = smem_u32(ring);
     uint32_t gbase = 0;
+    uint32_t ground = 0, seen_round = 0xffffffffu;  // rounds of scales
     int buf = 0;
     bool aborted = false;
     int n_pend = 0;
@@ -375,14 +456,65 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
 
-        for (int j = warp; j < n_stages; j += kConsumerWarps) {
+        // stage gs goes to warp gs % 4, whatever the item it belongs to
+        for (int j = (int)((warp - gbase) & (kConsumerWarps - 1)); j < n_stages;
+             j += kConsumerWarps) {
             const uint32_t gs = gbase + (uint32_t)j;
             const uint32_t slot = gs % NSLOTS;
             if (!aborted) aborted = !wait(&full_bar[slot], (gs / NSLOTS) & 1u);
             if (aborted) break;
             const int valid = min(kB8Tokens, it.tok_end - (it.tok_begin + j * kB8Tokens));
             const uint32_t kbase = ring_u32 + slot * kSlotBytes;
-            const float4 scales = *reinterpret_cast<const float4*>(s_scale + slot * 4);
+            // the stage's round and place in it (rounds count from the item's start)
+            const uint32_t rnd = ground + (uint32_t)(j / kB8Round);
+            if (rnd != seen_round) {
+                aborted = !wait(&s_look->scales_full[rnd & (kB8Rounds - 1)],
+                                (rnd / kB8Rounds) & 1u);
+                if (aborted) break;
+                seen_round = rnd;
+            }
+            const float4 scales =
+                *reinterpret_cast<const float4*>(
+                s_look->scales[rnd & (kB8Rounds - 1)][j % kB8Round]);
+            if (valid < kB8Tokens || scales.z == 0.f || scales.w == 0.f) {
+                // V lines past the row's end or of a scale of 0 (a page that is not
+                // there has that scale too) may hold anything: zero them, so that a
+                // weight of 0 never meets a NaN
+                uint8_t* line0 = ring + (size_t)slot * kSlotBytes + kB8Half;
+                for (int c = lane; c < kB8Tokens * 8; c += 32) {
+                    const int line = c >> 3;
+                    if (line >= valid || (line < kB8Scale ? scales.z : scales.w) == 0.f)
+                        *reinterpret_cast<uint4*>(line0 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+
+            // ---- the stage into registers, and its slot back to the producer
+            uint4 kr[2][2][2], vr[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t at =
+                        kbase + (16 * i + g8) * kB8Line + (((2 * t4 + h) ^ g8) << 4);
+                    kr[i][h][0] = lds128(at);                // token 16 i + g8
+                    kr[i][h][1] = lds128(at + 8 * kB8Line);  // token 16 i + g8 + 8
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // tokens 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+                const uint32_t at = kbase + kB8Half + (16 * i + 2 * t4) * kB8Line;
+                const uint32_t x0 = (uint32_t)((g8 ^ (2 * t4)) << 4);
+                const uint32_t x1 = (uint32_t)((g8 ^ (2 * t4 + 1)) << 4);
+                vr[i][0] = lds128(at + x0);
+                vr[i][1] = lds128(at + kB8Line + x1);
+                vr[i][2] = lds128(at + 8 * kB8Line + x0);
+                vr[i][3] = lds128(at + 9 * kB8Line + x1);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_bar[slot]);
 
             // ---- S^T: 2 x [16 tokens x 8 heads]
             float sc[2][4];
@@ -391,10 +523,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int chunk = 2 * t4 + h;
-                    const uint32_t at = kbase + (16 * i + g8) * kB8Line + ((chunk ^ g8) << 4);
-                    const uint4 lo = lds128(at);                // token 16 i + g8
-                    const uint4 hi = lds128(at + 8 * kB8Line);  // token 16 i + g8 + 8
+                    const uint4 lo = kr[i][h][0], hi = kr[i][h][1];
                     const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w};
                     const uint32_t wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -411,6 +540,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                 // becomes 2^-100, far below any weight's contribution
                 const float lg = vs == 0.f ? -100.f : fast_log2(vs);
                 const float f0 = qs[0] * ks, f1 = qs[1] * ks;
+                if (ks == 0.f) c[0] = c[1] = c[2] = c[3] = 0.f;  // K = 0, whatever the codes
                 const bool ok0 = 16 * i + g8 < valid, ok1 = 16 * i + g8 + 8 < valid;
                 sc[i][0] = ok0 ? fmaf(c[0], f0, lg) : -INFINITY;
                 sc[i][1] = ok0 ? fmaf(c[1], f1, lg) : -INFINITY;
@@ -460,16 +590,9 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                 l_run[1] = fmaf(pr[1] + pr[3], inv, l_run[1]);
                 const uint32_t pb0 = movmatrix_trans(ElemOps<__half>::pack(pr[0], pr[1]));
                 const uint32_t pb1 = movmatrix_trans(ElemOps<__half>::pack(pr[2], pr[3]));
-                // tokens 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9; chunk g8 holds the dims
-                // 16 g8 + 2 mt + (0, 1) of output tile mt's rows g8 and g8 + 8
-                const int tok = 16 * i + 2 * t4;
-                const uint32_t at = kbase + kB8Half + tok * kB8Line;
-                const uint32_t x0 = (uint32_t)((g8 ^ (2 * t4)) << 4);
-                const uint32_t x1 = (uint32_t)((g8 ^ (2 * t4 + 1)) << 4);
-                const uint4 va = lds128(at + x0);
-                const uint4 vb = lds128(at + kB8Line + x1);
-                const uint4 vc = lds128(at + 8 * kB8Line + x0);
-                const uint4 vd = lds128(at + 9 * kB8Line + x1);
+                // chunk g8 holds the dims 16 g8 + 2 mt + (0, 1) of output tile mt's rows
+                // g8 and g8 + 8
+                const uint4 va = vr[i][0], vb = vr[i][1], vc = vr[i][2], vd = vr[i][3];
                 const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
                 const uint32_t wc[4] = {vc.x, vc.y, vc.z, vc.w}, wd[4] = {vd.x, vd.y, vd.z, vd.w};
 #pragma unroll
@@ -486,10 +609,9 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty_bar[slot]);
         }
         gbase += (uint32_t)n_stages;
+        ground += (uint32_t)ceil_div_i(n_stages, kB8Round);
 
         // ---- combine the four warps' states of this item
         float* mbuf = s_merge + buf * DecodeSmem<G>::kMergeFloats;
