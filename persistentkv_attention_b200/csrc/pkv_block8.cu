@@ -56,7 +56,7 @@ pkv_status launch_typed8(const LaunchSpec& ls, cudaStream_t stream) {
     bp.block = ls.scale_block;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ls.dp.auto_groups * ls.dp.Hkv);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kB8Threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -37,9 +37,16 @@ constexpr int kB8Rounds = kDescSlots;
 static_assert((kB8Rounds & (kB8Rounds - 1)) == 0, "rounds are counted by masks");
 struct B8Lookups {
     float scales[kB8Rounds][kB8Round][4];
-    int lines[32];  // -1: no page
-    uint64_t scales_full[kB8Rounds];
+    int lines[kB8Rounds][32];  // -1: no page
+    int stages[kB8Rounds];     // 0: the last round is over
+    uint64_t scales_full[kB8Rounds], lines_full[kB8Rounds];
 };
+
+// Four consumer warps, one producer warp that resolves pages and copies K, one
+// that copies V: the copies of a stage are four instructions of one thread with
+// pages of 16 tokens, and one thread issuing all of them beside the consumers'
+// math falls behind HBM (64 rows up to 32768 tokens: 197 us, two threads 175 us).
+constexpr int kB8Threads = kThreads + 32;
 
 template <int G, int NSLOTS>
 constexpr size_t block8_smem_bytes() {
@@ -97,7 +104,7 @@ __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, b
 // memory and no transpose; that pass is what bounds the per-tensor route.
 // Bound: HBM, 256 bytes per token and KV head.
 template <int G, typename T, int BOX, int NSLOTS>
-__global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
+__global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
     pkv_block8_kernel(const __grid_constant__ Block8Params bp,
                       const __grid_constant__ CUtensorMap tmap_k,
                       const __grid_constant__ CUtensorMap tmap_v) {
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < NSLOTS; ++s) {
-            mbar_init(&full_bar[s], 1);
+            mbar_init(&full_bar[s], 2);  // K and V copies
             mbar_init(&empty_bar[s], 1);
         }
         for (int s = 0; s < kDescSlots; ++s) {
@@ -155,22 +162,78 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
             mbar_init(&desc_empty[s], kConsumerWarps);
         }
         mbar_init(merge_bar, 1);
-        for (int r = 0; r < kB8Rounds; ++r) mbar_init(&s_look->scales_full[r], 32);
+        for (int r = 0; r < kB8Rounds; ++r) {
+            mbar_init(&s_look->scales_full[r], 32);
+            mbar_init(&s_look->lines_full[r], 1);
+        }
         s_flags[0] = 0;
         fence_mbar_init();
     }
     __syncthreads();
     const int my_items = s_my_items;
 
+    // One pool's copies of a round's stages, by one thread: lines of the pool
+    // to part `part` of the ring's slots.  False if a slot did not come free.
+    const uint64_t policy = l2_evict_first_policy();
+    auto copy_round = [&](const CUtensorMap& map, int part, const int* lines, int stages,
+                          uint32_t& gs) -> bool {
+        for (int st = 0; st < stages; ++st, ++gs) {
+            const uint32_t slot = gs % NSLOTS;
+            int line[kBoxesPerStage];
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int bx = 0; bx < kBoxesPerStage; ++bx) {
+                line[bx] = lines[st * kBoxesPerStage + bx];
+                bytes += line[bx] >= 0 ? (uint32_t)(BOX * kB8Line) : 0u;
+            }
+            if (gs >= (uint32_t)NSLOTS &&
+                !mbar_wait_bounded(&empty_bar[slot], ((gs / NSLOTS) - 1u) & 1u, s_flags))
+                return false;
+            mbar_arrive_expect_tx(&full_bar[slot], bytes);
+            uint8_t* dst = ring + (size_t)slot * kSlotBytes + part * kB8Half;
+#pragma unroll
+            for (int bx = 0; bx < kBoxesPerStage; ++bx)
+                if (line[bx] >= 0)
+                    tma_load_2d(dst + bx * BOX * kB8Line, &map, 0, line[bx], &full_bar[slot], policy);
+        }
+        return true;
+    };
+    // Every copy a thread issued lands before the CTA exits.
+    auto drain = [&](uint32_t gs) {
+        for (uint32_t g = gs > (uint32_t)NSLOTS ? gs - NSLOTS : 0u; g < gs; ++g) {
+            if (!mbar_wait_bounded(&full_bar[g % NSLOTS], (g / NSLOTS) & 1u, nullptr)) {
+                raise_error(p.error, kErrTimeout);
+                break;
+            }
+        }
+    };
+
+    if (warp == kConsumerWarps + 1) {
+        // ============================ V copies ============================
+        if (lane == 0) {
+            tma_prefetch_map(&tmap_v);
+            uint32_t gs = 0;
+            for (uint32_t r = 0;; ++r) {
+                const int at = (int)(r & (kB8Rounds - 1));
+                bool ok = mbar_wait_bounded(&s_look->lines_full[at], (r / kB8Rounds) & 1u, s_flags);
+                const int stages = ok ? s_look->stages[at] : 0;
+                if (ok && stages == 0) break;
+                ok = ok && copy_round(tmap_v, 1, s_look->lines[at], stages, gs);
+                if (!ok) {
+                    s_flags[0] = 1;
+                    raise_error(p.error, kErrTimeout);
+                    break;
+                }
+            }
+            drain(gs);
+        }
+        return;
+    }
     if (warp == kConsumerWarps) {
         // ============================ producer warp ============================
-        const uint64_t policy = l2_evict_first_policy();
         const uint32_t q_base = smem_u32(s_q);
         const int nblk = p.page_size / bp.block;
-        if (lane == 0) {
-            tma_prefetch_map(&tmap_k);
-            tma_prefetch_map(&tmap_v);
-        }
+        if (lane == 0) tma_prefetch_map(&tmap_k);
         uint32_t gstage = 0, ground = 0;
         uint32_t round_end[kB8Rounds] = {0u, 0u, 0u, 0u};  // of the rounds before, oldest first
         uint32_t round_len[kB8Rounds] = {0u, 0u, 0u, 0u};
@@ -188,6 +251,16 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
             bool ok = true;
             if (lane == 0) ok = mbar_wait_bounded(bar, parity, s_flags);
             return __shfl_sync(0xffffffffu, ok, 0) && s_flags[0] == 0;
+        };
+        // The next round's place in the lookups: that of the round kB8Rounds
+        // before, all of whose stages must have been consumed (one that the ring
+        // has issued a successor of has been).
+        auto round_free = [&]() -> bool {
+            const uint32_t g = round_end[0] - 1u - (uint32_t)lane;
+            bool free = true;
+            if ((uint32_t)lane < round_len[0] && gstage <= g + NSLOTS)
+                free = mbar_wait_bounded(&empty_bar[g % NSLOTS], (g / NSLOTS) & 1u, s_flags);
+            return __all_sync(0xffffffffu, free);
         };
         for (int s = 0; s < my_items && !aborted; ++s) {
             if (s == my_items - 1) griddep_launch_dependents();
@@ -253,67 +326,34 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
                         sc_step = BOX > kB8Scale && bp.block == kB8Scale ? 1 : 0;
                     }
                 }
-                // the scales go where those of the round kB8Rounds before are: every
-                // stage of it must have been consumed (one that the ring has issued
-                // a successor of has been)
-                {
-                    const uint32_t g = round_end[0] - 1u - (uint32_t)lane;
-                    bool free = true;
-                    if ((uint32_t)lane < round_len[0] && gstage <= g + NSLOTS)
-                        free = mbar_wait_bounded(&empty_bar[g % NSLOTS], (g / NSLOTS) & 1u, s_flags);
-                    if (!__all_sync(0xffffffffu, free)) {
-                        give_up();
-                        break;
-                    }
+                if (!round_free()) {
+                    give_up();
+                    break;
                 }
+                const int at_round = (int)(ground & (kB8Rounds - 1));
                 if (lane < kRoundBoxes) {
                     // a missing box has scale 0
                     const uint32_t at =
-                        smem_u32(&s_look->scales[ground & (kB8Rounds - 1)][lane / kBoxesPerStage][0]) +
-                                        (lane % kBoxesPerStage) * (BOX / kB8Scale) * 4;
+                        smem_u32(&s_look->scales[at_round][lane / kBoxesPerStage][0]) +
+                        (lane % kBoxesPerStage) * (BOX / kB8Scale) * 4;
 #pragma unroll
                     for (int h = 0; h < BOX / kB8Scale; ++h) {
                         cp_async_4(at + 4 * h, bp.k_scales + sc + h * sc_step, ok);
                         cp_async_4(at + 8 + 4 * h, bp.v_scales + sc + h * sc_step, ok);
                     }
                 }
-                cp_async_mbar_arrive_noinc(&s_look->scales_full[ground & (kB8Rounds - 1)]);
+                cp_async_mbar_arrive_noinc(&s_look->scales_full[at_round]);
                 ++ground;
-                s_look->lines[lane] = y;
-                __syncwarp();
                 const int stages_here = min(kB8Round, n_stages - base / kBoxesPerStage);
+                s_look->lines[at_round][lane] = y;
+                if (lane == 0) s_look->stages[at_round] = stages_here;
+                __syncwarp();
                 bool ok_stages = true;
                 if (lane == 0) {
-                    // one thread issues the round's copies
-                    for (int st = 0; st < stages_here; ++st) {
-                        const uint32_t gs = gstage + st;
-                        const uint32_t slot = gs % NSLOTS;
-                        int line[kBoxesPerStage];
-                        uint32_t bytes = 0;
-#pragma unroll
-                        for (int bx = 0; bx < kBoxesPerStage; ++bx) {
-                            line[bx] = s_look->lines[st * kBoxesPerStage + bx];
-                            bytes += line[bx] >= 0 ? 2u * BOX * kB8Line : 0u;
-                        }
-                        if (gs >= (uint32_t)NSLOTS &&
-                            !mbar_wait_bounded(&empty_bar[slot], ((gs / NSLOTS) - 1u) & 1u,
-                                               s_flags)) {
-                            ok_stages = false;
-                            gstage = gs;  // what was issued, for the drain
-                            break;
-                        }
-                        mbar_arrive_expect_tx(&full_bar[slot], bytes);
-                        uint8_t* dst = ring + (size_t)slot * kSlotBytes;
-#pragma unroll
-                        for (int bx = 0; bx < kBoxesPerStage; ++bx) {
-                            if (line[bx] >= 0) {
-                                tma_load_2d(dst + bx * BOX * kB8Line, &tmap_k, 0, line[bx],
-                                            &full_bar[slot], policy);
-                                tma_load_2d(dst + kB8Half + bx * BOX * kB8Line, &tmap_v, 0, line[bx],
-                                            &full_bar[slot], policy);
-                            }
-                        }
-                    }
+                    mbar_arrive(&s_look->lines_full[at_round]);
+                    uint32_t gs = gstage;
+                    ok_stages = copy_round(tmap_k, 0, s_look->lines[at_round], stages_here, gs);
+                    if (!ok_stages) gstage = gs;  // what was issued, for the drain
                 }
                 ok_stages = __shfl_sync(0xffffffffu, ok_stages, 0);
                 if (!ok_stages) {
@@ -337,17 +377,14 @@ __global__ void __launch_bounds__(kThreads, PKV_MIN_CTAS_PER_SM)
             cur = nxt;
             pid0 = nxt_pid;
         }
-        // Drain: every copy this warp issued lands before the CTA exits.
-        cp_async_wait_all();
-        if (lane == 0) {
-            const uint32_t first = gstage > (uint32_t)NSLOTS ? gstage - NSLOTS : 0u;
-            for (uint32_t g = first; g < gstage; ++g) {
-                if (!mbar_wait_bounded(&full_bar[g % NSLOTS], (g / NSLOTS) & 1u, nullptr)) {
-                    raise_error(p.error, kErrTimeout);
-                    break;
-                }
-            }
+        // the V copies end with a round of no stages
+        if (!aborted && round_free() && lane == 0) {
+            const int at = (int)(ground & (kB8Rounds - 1));
+            s_look->stages[at] = 0;
+            mbar_arrive(&s_look->lines_full[at]);
         }
+        cp_async_wait_all();
+        if (lane == 0) drain(gstage);
         return;
     }
 
