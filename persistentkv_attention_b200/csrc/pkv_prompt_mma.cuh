@@ -24,7 +24,7 @@ constexpr float kPmLazy = 8.0f;
 
 struct PmShared {
     uint64_t q_full, kv_full[kPmStages], kv_empty[kPmStages];
-    uint64_t s_full[2], p_full[2], o_full[2], tail, drained;
+    uint64_t s_full[2], p_full[2][2], o_full[2], tail, drained;
     uint32_t tmem;
     int abort;
     int seq, tile;  // this CTA's work
@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh->s_full[t], 1);
-            mbar_init(&sh->p_full[t], 128);
+            mbar_init(&sh->p_full[t][0], 128);
+            mbar_init(&sh->p_full[t][1], 128);
             mbar_init(&sh->o_full[t], 1);
         }
         mbar_init(&sh->tail, 1);
@@ -211,57 +212,78 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         }
     } else if (warp == 8) {
         // ------------------------------------------------------------ products
-        if (lane == 0 && n_blocks > 0) {
+        // The whole warp walks the loop, so that descriptors and addresses are
+        // uniform values; one elected lane issues the products and commits.
+        if (n_blocks > 0) {
             constexpr uint32_t kDescQk = mma_desc_f16(kPmTile, kPmTile, kBf16, false);
             constexpr uint32_t kDescPv = mma_desc_f16(kPmTile, kHeadDim, kBf16, true);
-            const uint32_t q_u32 = smem_u32(s_q), kv_u32 = smem_u32(s_kv);
+            const uint64_t q_desc = smem_desc_sw128(smem_u32(s_q), 16, 1024);
+            const uint64_t k_desc = smem_desc_sw128(smem_u32(s_kv), 16, 1024);
+            const uint64_t v_desc = smem_desc_sw128(smem_u32(s_kv), kPmHalfBytes, 1024);
+            constexpr uint32_t kTileStep = kPmTileBytes >> 4;  // in descriptor units
+            auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return __all_sync(0xffffffffu, pm_wait(p, sh, bar, parity));
+            };
+            // S of tile t from the K tile in stage st
             auto scores = [&](int t, int st) {
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t off = (ks >> 2) * kPmHalfBytes + (ks & 3) * 32;
-                    mma_f16_ss(tmem + t * 128,
-                               smem_desc_sw128(q_u32 + t * kPmTileBytes + off, 16, 1024),
-                               smem_desc_sw128(kv_u32 + st * kPmTileBytes + off, 16, 1024), kDescQk,
-                               ks > 0);
+                    const uint32_t off = ((ks >> 2) * kPmHalfBytes + (ks & 3) * 32) >> 4;
+                    mma_f16_ss(tmem + t * 128, q_desc + (t * kTileStep + off),
+                               k_desc + (st * kTileStep + off), kDescQk, ks > 0);
                 }
-                tc_commit(&sh->s_full[t]);
             };
-            auto output = [&](int t, int st, bool accumulate) {
+            // O of tile t plus keys 64 half .. 64 half + 63 of the V tile in stage st
+            auto output = [&](int t, int st, int half, bool accumulate) {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
+                for (int k = 0; k < 4; ++k) {
+                    const int ks = 4 * half + k;
                     mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8,
-                               smem_desc_sw128(kv_u32 + st * kPmTileBytes + ks * 2048, kPmHalfBytes,
-                                               1024),
-                               kDescPv, accumulate || ks > 0);
-                tc_commit(&sh->o_full[t]);
+                               v_desc + (st * kTileStep + ks * 128), kDescPv, accumulate || ks > 0);
+                }
             };
-            bool ok = pm_wait(p, sh, &sh->q_full, 0) && pm_wait(p, sh, &sh->kv_full[0], 0);
-            if (ok) {
-                for (int t = 0; t < n_tiles; ++t) scores(t, 0);
+            bool ok = wait(&sh->q_full, 0) && wait(&sh->kv_full[0], 0);
+            if (ok && elect_one()) {
+                for (int t = 0; t < n_tiles; ++t) {
+                    scores(t, 0);
+                    tc_commit(&sh->s_full[t]);
+                }
                 tc_commit(&sh->kv_empty[0]);
             }
+            __syncwarp();
             for (int j = 0; ok && j < n_blocks; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2;
                 const int sv = iv % kPmStages, sk = ik % kPmStages;
                 const bool more = j + 1 < n_blocks;
-                ok = pm_wait(p, sh, &sh->kv_full[sv], (iv / kPmStages) & 1);
-                if (ok && !more && tail < kPmTile) ok = pm_wait(p, sh, &sh->tail, 0);
+                ok = wait(&sh->kv_full[sv], (iv / kPmStages) & 1);
+                if (ok && !more && tail < kPmTile) ok = wait(&sh->tail, 0);
                 for (int t = 0; ok && t < n_tiles; ++t) {
-                    ok = pm_wait(p, sh, &sh->p_full[t], j & 1);
+                    const bool last = t == n_tiles - 1;
+                    ok = wait(&sh->p_full[t][0], j & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    output(t, sv, j > 0);
-                    if (t == n_tiles - 1) tc_commit(&sh->kv_empty[sv]);
-                    if (more) {
-                        if (t == 0) ok = pm_wait(p, sh, &sh->kv_full[sk], (ik / kPmStages) & 1);
-                        if (!ok) break;
-                        scores(t, sk);
-                        if (t == n_tiles - 1) tc_commit(&sh->kv_empty[sk]);
+                    if (elect_one()) output(t, sv, 0, j > 0);
+                    __syncwarp();
+                    ok = wait(&sh->p_full[t][1], j & 1);
+                    if (ok && more && t == 0) ok = wait(&sh->kv_full[sk], (ik / kPmStages) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        output(t, sv, 1, true);
+                        tc_commit(&sh->o_full[t]);
+                        if (last) tc_commit(&sh->kv_empty[sv]);
+                        if (more) {
+                            scores(t, sk);
+                            tc_commit(&sh->s_full[t]);
+                            if (last) tc_commit(&sh->kv_empty[sk]);
+                        }
                     }
+                    __syncwarp();
                 }
             }
             // the products in flight end before TMEM is freed (bounded)
-            tc_commit(&sh->drained);
+            if (elect_one()) tc_commit(&sh->drained);
+            __syncwarp();
             mbar_wait_bounded(&sh->drained, 0, nullptr);
         }
         __syncwarp();
@@ -299,7 +321,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 }
                 float mx[4] = {m, m, m, m};
 #pragma unroll
-                for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                for (int c = 0; c < 128; c += 2)
+                    mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], __uint_as_float(s[c])),
+                                             __uint_as_float(s[c + 1]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 // (a maximum of -inf: the difference is NaN, no move)
                 const bool move = (top - m) * p.scale_log2 > kPmLazy;
@@ -325,26 +349,33 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
+                const uint64_t base2 = pack_f32x2(-base, -base);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t w[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float a = fast_exp2(
-                            fmaf(__uint_as_float(s[64 * c + 2 * i]), p.scale_log2, -base));
-                        const float d = fast_exp2(
-                            fmaf(__uint_as_float(s[64 * c + 2 * i + 1]), p.scale_log2, -base));
-                        sum[(2 * i) & 3] += a;
-                        sum[(2 * i + 1) & 3] += d;
+                        const uint64_t x = fma_f32x2(
+                            pack_f32x2(__uint_as_float(s[64 * c + 2 * i]),
+                                       __uint_as_float(s[64 * c + 2 * i + 1])),
+                            scale2, base2);
+                        float a, d;
+                        unpack_f32x2(x, a, d);
+                        a = fast_exp2(a);
+                        d = fast_exp2(d);
+                        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, d));
                         w[i] = ElemOps<T>::pack(a, d);
                     }
                     tmem_st32(t_s + 32 * c, w);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&sh->p_full[t][c]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sh->p_full[t]);
+                float lo, hi;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
+                l += lo + hi;
             }
             // ---- output rows
             if (ok && n_blocks > 0)
