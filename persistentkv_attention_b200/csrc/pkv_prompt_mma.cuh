@@ -15,7 +15,7 @@ constexpr int kPmThreads = 320;  // 4 softmax warps per query tile, MMA warp, lo
 constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes + 256;
 // TMEM columns: scores of tile t at 128 t (its weights, 16 bit, in the first
 // 64 of them), output of tile t at 256 + 128 t.
-constexpr uint32_t kPmTmemColumns = 512;
+constexpr uint32_t kPmTmemColumns = 512;  // all there are
 // The running maximum that weights refer to is raised, and the output
 // rescaled, only when a row's maximum has grown by more than this many powers
 // of two: weights stay below 2^8, far inside both 16-bit types' range, and
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh->s_full[t], 1);
-            mbar_init(&sh->p_full[t][0], 128);
-            mbar_init(&sh->p_full[t][1], 128);
+            mbar_init(&sh->p_full[t][0], 4);  // one arrival per warp
+            mbar_init(&sh->p_full[t][1], 4);
             mbar_init(&sh->o_full[t], 1);
         }
         mbar_init(&sh->tail, 1);
@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh->tmem;
+    // all of TMEM: it starts at lane 0, column 0, and addresses are constants
+    constexpr uint32_t tmem = 0;
 
     if (warp == 9) {
         // ------------------------------------------------------------ loader
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     const uint32_t off = ((ks >> 2) * kPmHalfBytes + (ks & 3) * 32) >> 4;
-                    mma_f16_ss(tmem + t * 128, q_desc + (t * kTileStep + off),
+                    mma_f16_ss(t * 128, q_desc + (t * kTileStep + off),
                                k_desc + (st * kTileStep + off), kDescQk, ks > 0);
                 }
             };
@@ -238,35 +239,42 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int ks = 4 * half + k;
-                    mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8,
+                    mma_f16_ts(256 + t * 128, t * 128 + ks * 8,
                                v_desc + (st * kTileStep + ks * 128), kDescPv, accumulate || ks > 0);
                 }
             };
             bool ok = wait(&sh->q_full, 0) && wait(&sh->kv_full[0], 0);
             if (ok && elect_one()) {
-                for (int t = 0; t < n_tiles; ++t) {
-                    scores(t, 0);
-                    tc_commit(&sh->s_full[t]);
+                scores(0, 0);
+                tc_commit(&sh->s_full[0]);
+                if (n_tiles == 2) {
+                    scores(1, 0);
+                    tc_commit(&sh->s_full[1]);
                 }
                 tc_commit(&sh->kv_empty[0]);
             }
             __syncwarp();
-            for (int j = 0; ok && j < n_blocks; ++j) {
-                const int iv = 2 * j + 1, ik = 2 * j + 2;
-                const int sv = iv % kPmStages, sk = ik % kPmStages;
+            // One block; its V tile is in stage 1 or 3, the next block's K tile in
+            // stage 2 or 0: with stages and tiles known at compile time every
+            // operand of a product is a constant away from a loop invariant.
+            auto block = [&](int j, auto odd) -> bool {
+                constexpr int sv = decltype(odd)::value ? 3 : 1;
+                constexpr int sk = decltype(odd)::value ? 0 : 2;
+                const uint32_t ring = (uint32_t)(j >> 1) & 1u;  // (2 j + 1) / 4
+                const uint32_t ring_k = (uint32_t)((j + 1) >> 1) & 1u;
                 const bool more = j + 1 < n_blocks;
-                ok = wait(&sh->kv_full[sv], (iv / kPmStages) & 1);
-                if (ok && !more && tail < kPmTile) ok = wait(&sh->tail, 0);
-                for (int t = 0; ok && t < n_tiles; ++t) {
+                if (!wait(&sh->kv_full[sv], ring)) return false;
+                if (!more && tail < kPmTile && !wait(&sh->tail, 0)) return false;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t >= n_tiles) break;
                     const bool last = t == n_tiles - 1;
-                    ok = wait(&sh->p_full[t][0], j & 1);
-                    if (!ok) break;
+                    if (!wait(&sh->p_full[t][0], j & 1)) return false;
                     tc_fence_after();
                     if (elect_one()) output(t, sv, 0, j > 0);
                     __syncwarp();
-                    ok = wait(&sh->p_full[t][1], j & 1);
-                    if (ok && more && t == 0) ok = wait(&sh->kv_full[sk], (ik / kPmStages) & 1);
-                    if (!ok) break;
+                    if (!wait(&sh->p_full[t][1], j & 1)) return false;
+                    if (more && t == 0 && !wait(&sh->kv_full[sk], ring_k)) return false;
                     tc_fence_after();
                     if (elect_one()) {
                         output(t, sv, 1, true);
@@ -280,6 +288,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     }
                     __syncwarp();
                 }
+                return true;
+            };
+            static_assert(kPmStages == 4, "the stages of a block's tiles");
+            for (int j = 0; ok && j < n_blocks; j += 2) {
+                ok = block(j, std::integral_constant<bool, false>{});
+                if (ok && j + 1 < n_blocks) ok = block(j + 1, std::integral_constant<bool, true>{});
             }
             // the products in flight end before TMEM is freed (bounded)
             if (elect_one()) tc_commit(&sh->drained);
@@ -371,7 +385,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     tmem_st32(t_s + 32 * c, w);
                     tmem_wait_st();
                     tc_fence_before();
-                    mbar_arrive(&sh->p_full[t][c]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->p_full[t][c]);
                 }
                 float lo, hi;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
