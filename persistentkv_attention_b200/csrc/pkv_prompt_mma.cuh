@@ -11,8 +11,13 @@ constexpr int kPmTile = 128;                     // query rows of a tile, keys o
 constexpr int kPmTileBytes = kPmTile * kRowBytes;  // 32 KB: two 64-element halves of 16 KB
 constexpr int kPmHalfBytes = kPmTileBytes / 2;
 constexpr int kPmStages = 4;                     // K/V tiles in flight
-constexpr int kPmThreads = 320;  // 4 softmax warps per query tile, MMA warp, loader warp
-constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes + 256;
+// 8 softmax warps (tile, 32 rows each), then one warp each for the products,
+// the copies and the schedule.
+constexpr int kPmSoftmaxWarps = 8;
+constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10;
+constexpr int kPmThreads = 384;
+constexpr int kPmParts = 4;  // parts of a block's weights, 32 keys each, handed over one by one
+constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes + 512;
 // TMEM columns: scores of tile t at 128 t (its weights, 16 bit, in the first
 // 64 of them), output of tile t at 256 + 128 t.
 constexpr uint32_t kPmTmemColumns = 512;  // all there are
@@ -22,29 +27,68 @@ constexpr uint32_t kPmTmemColumns = 512;  // all there are
 // the division by the sum at the end takes the factor out again.
 constexpr float kPmLazy = 8.0f;
 
+// One item of work: two query tiles that read the same keys.
+struct PmWork {
+    int q0, k0, lq, lk;  // the sequence's first query row and key, and lengths
+    int row0;            // first query row of the item in its sequence; -1: no more items
+    int group;           // head or pair of heads
+    int pad[2];
+};
+constexpr int kPmWorks = 2;  // current item and the next
+
 struct PmShared {
-    uint64_t q_full, kv_full[kPmStages], kv_empty[kPmStages];
-    uint64_t s_full[2], p_full[2][2], o_full[2], tail, drained;
+    uint4 launch;  // answer of the launch control
+    PmWork work[kPmWorks];
+    uint64_t work_full[kPmWorks], work_empty[kPmWorks], launch_bar, issued;
+    uint64_t q_full, q_empty, kv_full[kPmStages], kv_empty[kPmStages];
+    uint64_t s_full[2], p_full[2][kPmParts], o_full[2], o_empty[2], drained;
     uint32_t tmem;
     int abort;
-    int seq, tile;  // this CTA's work
-    int warp_sum[kPmThreads / 32];
 };
-static_assert(sizeof(PmShared) <= 256, "prompt CTA's shared state");
+static_assert(sizeof(PmShared) <= 512, "prompt CTA's shared state");
 
-// The CTA's sequence and its query tile: tile number `rank` from the end over
-// all sequences' tiles of `rows` query rows, so the longest rows of each
-// sequence start first.  Whole CTA; seq = -1 if there are fewer tiles.
-__device__ __forceinline__ void pm_find_tile(const PromptParams& p, PmShared* sh, int rank,
-                                             int rows) {
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    if (t == 0) sh->seq = -1;
+// What follows from an item for every role.
+struct PmItem {
+    int q0, k0, lq, lk, row0, head0, kvh, n_tiles, n_blocks, tail, G;
+    // keys that row i of the sequence sees
+    __device__ __forceinline__ int visible(int i) const {
+        return max(0, min(lk, i + 1 + lk - lq));
+    }
+};
+
+__device__ __forceinline__ int pm_rows_per_item(int G) { return G == 1 ? 2 * kPmTile : kPmTile; }
+
+__device__ __forceinline__ PmItem pm_item(const PromptParams& p, const PmWork& w) {
+    PmItem it;
+    it.G = p.Hq / p.Hkv;
+    it.q0 = w.q0;
+    it.k0 = w.k0;
+    it.lq = w.lq;
+    it.lk = w.lk;
+    it.row0 = w.row0;
+    it.head0 = it.G == 1 ? w.group : 2 * w.group;
+    it.kvh = it.head0 / it.G;
+    it.n_tiles = (it.G == 1 && it.row0 + kPmTile >= it.lq) ? 1 : 2;
+    const int n_keys = it.visible(min(it.row0 + pm_rows_per_item(it.G), it.lq) - 1);
+    it.n_blocks = (n_keys + kPmTile - 1) / kPmTile;
+    it.tail = n_keys - (it.n_blocks - 1) * kPmTile;  // keys of the last block
+    return it;
+}
+
+// Whole warp: the query tile number `rank`, counted from the end over all
+// sequences' tiles of `rows` rows, so that the longest rows of a sequence start
+// first.  Returns 1 with the work filled in, 0 if there are fewer tiles, -1
+// for a tile of a sequence whose ranges are bad.
+__device__ __forceinline__ int pm_find(const PromptParams& p, int rank, int rows, PmWork& w) {
+    const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int base = 0; base < p.B; base += kPmThreads) {
-        const int b = p.B - 1 - base - t;
-        int n = 0;
+    for (int base = 0; base < p.B; base += 32) {
+        const int b = p.B - 1 - base - lane;
+        int q0 = 0, q1 = 0, n = 0;
         if (b >= 0) {
-            const long long len = (long long)__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b);
+            q0 = __ldg(p.cu_q + b);
+            q1 = __ldg(p.cu_q + b + 1);
+            const long long len = (long long)q1 - q0;
             n = len > 0 ? (int)min((len + rows - 1) / rows, (long long)p.Tq) : 0;
         }
         int x = n;
@@ -53,27 +97,38 @@ __device__ __forceinline__ void pm_find_tile(const PromptParams& p, PmShared* sh
             const int y = __shfl_up_sync(0xffffffffu, x, off);
             if (lane >= off) x += y;
         }
-        __syncthreads();
-        if (lane == 31) sh->warp_sum[warp] = x;
-        __syncthreads();
-        int first = before + x - n;
-#pragma unroll
-        for (int w = 0; w < kPmThreads / 32; ++w) {
-            const int s = sh->warp_sum[w];
-            first += w < warp ? s : 0;
-            before += s;
+        const int first = before + x - n;
+        const unsigned hit = __ballot_sync(0xffffffffu, rank >= first && rank < first + n);
+        if (hit != 0u) {
+            const int src = __ffs(hit) - 1;
+            const int bb = __shfl_sync(0xffffffffu, b, src);
+            w.q0 = __shfl_sync(0xffffffffu, q0, src);
+            q1 = __shfl_sync(0xffffffffu, q1, src);
+            w.row0 = __shfl_sync(0xffffffffu, n - 1 - (rank - first), src) * rows;
+            w.k0 = __ldg(p.cu_k + bb);
+            const int k1 = __ldg(p.cu_k + bb + 1);
+            w.lq = q1 - w.q0;
+            w.lk = k1 - w.k0;
+            return (w.q0 < 0 || q1 > p.Tq || w.k0 < 0 || k1 < w.k0 || k1 > p.Tk) ? -1 : 1;
         }
-        if (rank >= first && rank < first + n) {
-            sh->seq = b;
-            sh->tile = n - 1 - (rank - first);
-        }
-        if (rank < before) break;  // uniform
+        before = __shfl_sync(0xffffffffu, before + x, 31);
     }
-    __syncthreads();
+    return 0;
 }
 
-// One wait of the kernel: false after the time limit or once another thread
-// of the CTA has given up.
+// One wait of a converged warp: false after the time limit or once another
+// thread of the CTA has given up.
+__device__ __forceinline__ bool pm_wait_warp(const PromptParams& p, PmShared* sh, uint64_t* bar,
+                                             uint32_t parity) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) {
+        ok = mbar_wait_bounded(bar, parity, &sh->abort);
+        if (!ok && atomicExch(&sh->abort, 1) == 0) raise_error(p.error, kErrTimeout);
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+// One thread's wait.
 __device__ __forceinline__ bool pm_wait(const PromptParams& p, PmShared* sh, uint64_t* bar,
                                         uint32_t parity) {
     if (mbar_wait_bounded(bar, parity, &sh->abort)) return true;
@@ -81,17 +136,47 @@ __device__ __forceinline__ bool pm_wait(const PromptParams& p, PmShared* sh, uin
     return false;
 }
 
-// A CTA owns two query tiles of 128 rows that read the same keys: two heads of
+// Waits for item number n: false if there are no more (or on abort).
+__device__ __forceinline__ bool pm_wait_work(const PromptParams& p, PmShared* sh, uint32_t n) {
+    return pm_wait_warp(p, sh, &sh->work_full[n % kPmWorks], (n / kPmWorks) & 1u) &&
+           *(const volatile int*)&sh->work[n % kPmWorks].row0 >= 0;
+}
+
+// The warp needs item number n's place no longer.
+__device__ __forceinline__ void pm_release_work(PmShared* sh, uint32_t n) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->work_empty[n % kPmWorks]);
+}
+
+// Both, with the item copied.
+__device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uint32_t n,
+                                        PmItem& it) {
+    if (!pm_wait_work(p, sh, n)) return false;
+    it = pm_item(p, sh->work[n % kPmWorks]);
+    pm_release_work(sh, n);
+    return true;
+}
+
+// An item is two query tiles of 128 rows that read the same keys: two heads of
 // one KV group at the same positions, or (G = 1) two successive tiles of one
 // head.  K and V pass through shared memory in blocks of 128 keys (TMA, ring
 // of kPmStages tiles).  For each block, tile t's scores S = Q K^T and output
-// O += P V are tcgen05 products of one issuing thread with S, P and O in
-// TMEM; 128 softmax threads per tile, one per row, turn S into P in place
-// with the running maximum and sum in 32 bits.  The issue order
+// O += P V are tcgen05 products issued by one warp, with S, P and O in TMEM; 4
+// softmax warps per tile turn S into P in place, running maximum and sum in 32
+// bits, one row per thread.  The issue order
 //   S0 S1 | O0 S0' O1 S1' | O0' ...
-// keeps the tensor cores on one tile while the other's softmax runs.
-// Bound: the tensor cores (4 * 128 flops per query, key and head) and, close
-// behind, the 1 exponential per query and key of the special-function units.
+// keeps the tensor cores on one tile while the other's softmax runs, and the
+// weights of a block are handed over 32 keys at a time, so that its output
+// product starts before its last exponentials.
+//
+// The grid has one CTA per item; a resident CTA goes on with items whose CTA
+// has not started yet (launch control), so the next item's schedule, Q and
+// first keys arrive while the present one is computed, and its first scores
+// while the present one's output is written.
+//
+// Bound: the tensor cores (4 * 128 flops per query, key and head) under the
+// card's power cap, and next to it the 1 exponential per query and key of the
+// special-function units.
 template <typename T>
 __global__ void __launch_bounds__(kPmThreads, 1)
     pkv_prompt_mma_kernel(const __grid_constant__ PromptParams p,
@@ -101,243 +186,324 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* s_q = smem;                          // 2 tiles
-    uint8_t* s_kv = smem + 2 * kPmTileBytes;      // kPmStages tiles
+    uint8_t* s_q = smem;                      // 2 tiles
+    uint8_t* s_kv = smem + 2 * kPmTileBytes;  // kPmStages tiles
     PmShared* sh = reinterpret_cast<PmShared*>(s_kv + kPmStages * kPmTileBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int G = p.Hq / p.Hkv;
-    const int rows_per_cta = G == 1 ? 2 * kPmTile : kPmTile;
-    const int head_groups = G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
-    const int rank = (int)(blockIdx.x / head_groups), group = (int)(blockIdx.x % head_groups);
-    pm_find_tile(p, sh, rank, rows_per_cta);
-    const int b = sh->seq;
-    if (b < 0) return;
-    const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1);
-    const int k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
-    if (q0 < 0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk) {
-        if (threadIdx.x == 0) raise_error(p.error, kErrIndex);
-        return;
-    }
-    const int lq = q1 - q0, lk = k1 - k0;
-    const int row0 = sh->tile * rows_per_cta;  // first query row of the CTA in its sequence
-    const int head0 = G == 1 ? group : 2 * group;
-    const int kvh = head0 / G;
-    const int n_tiles = (G == 1 && row0 + kPmTile >= lq) ? 1 : 2;
-    // keys that row i of the sequence sees
-    auto visible = [lq, lk](int i) { return max(0, min(lk, i + 1 + lk - lq)); };
-    const int last_row = min(row0 + rows_per_cta, lq) - 1;
-    const int n_keys = visible(last_row);
-    const int n_blocks = (n_keys + kPmTile - 1) / kPmTile;
-    const int tail = n_keys - (n_blocks - 1) * kPmTile;  // keys of the last block
-
     if (threadIdx.x == 0) {
+        for (int i = 0; i < kPmWorks; ++i) {
+            mbar_init(&sh->work_full[i], 1);
+            mbar_init(&sh->work_empty[i], kPmSoftmaxWarps + 2);  // one arrival per reading warp
+        }
+        mbar_init(&sh->launch_bar, 1);
+        mbar_init(&sh->issued, 1);
         mbar_init(&sh->q_full, 1);
+        mbar_init(&sh->q_empty, 1);
         for (int i = 0; i < kPmStages; ++i) {
             mbar_init(&sh->kv_full[i], 1);
             mbar_init(&sh->kv_empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh->s_full[t], 1);
-            mbar_init(&sh->p_full[t][0], 4);  // one arrival per warp
-            mbar_init(&sh->p_full[t][1], 4);
+            for (int i = 0; i < kPmParts; ++i) mbar_init(&sh->p_full[t][i], 4);  // the warps
             mbar_init(&sh->o_full[t], 1);
+            mbar_init(&sh->o_empty[t], 4);
         }
-        mbar_init(&sh->tail, 1);
         mbar_init(&sh->drained, 1);
         sh->abort = 0;
         fence_mbar_init();
     }
-    if (warp == 8) tmem_alloc(&sh->tmem, kPmTmemColumns);
+    if (warp == kPmMmaWarp) tmem_alloc(&sh->tmem, kPmTmemColumns);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     // all of TMEM: it starts at lane 0, column 0, and addresses are constants
-    constexpr uint32_t tmem = 0;
 
-    if (warp == 9) {
-        // ------------------------------------------------------------ loader
-        if (lane == 0 && n_blocks > 0) {
+    if (warp == kPmPlanWarp) {
+        // ------------------------------------------------------------ schedule
+        const int G = p.Hq / p.Hkv;
+        const int groups = G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
+        int item = blockIdx.x;
+        uint32_t n = 0;  // items published
+        bool ok = true;
+        for (uint32_t round = 0; ok; ++round) {
+            PmWork w;
+            const int found = pm_find(p, item / groups, pm_rows_per_item(G), w);
+            w.group = item % groups;
+            if (found < 0 && lane == 0) raise_error(p.error, kErrIndex);
+            if (found > 0) {
+                if (n >= (uint32_t)kPmWorks)
+                    ok = pm_wait_warp(p, sh, &sh->work_empty[n % kPmWorks],
+                                      (n / kPmWorks - 1) & 1u);
+                if (!ok) break;
+                if (lane == 0) {
+                    sh->work[n % kPmWorks] = w;
+                    mbar_arrive(&sh->work_full[n % kPmWorks]);
+                }
+                __syncwarp();
+                ++n;
+                // The next item is asked for once the copies of this one's last
+                // blocks are under way: early enough that it is there when this
+                // one ends, late enough to be the fair one to take.
+                ok = pm_wait_warp(p, sh, &sh->issued, (n - 1) & 1u);
+                if (!ok) break;
+            }
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sh->launch_bar, 16);
+                launch_cancel_async(&sh->launch, &sh->launch_bar);
+            }
+            __syncwarp();
+            // (the answer lands in this CTA: its wait heeds no abort)
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh->launch_bar, round & 1u, nullptr));
+            if (!ok && lane == 0 && atomicExch(&sh->abort, 1) == 0) raise_error(p.error, kErrTimeout);
+            ok = ok && launch_cancelled(&sh->launch, item);
+            fence_proxy_async_smem();  // read before the next answer is written
+            __syncwarp();
+        }
+        if (n >= (uint32_t)kPmWorks)
+            pm_wait_warp(p, sh, &sh->work_empty[n % kPmWorks], (n / kPmWorks - 1) & 1u);
+        if (lane == 0) {
+            sh->work[n % kPmWorks].row0 = -1;
+            mbar_arrive(&sh->work_full[n % kPmWorks]);
+        }
+        __syncwarp();
+    } else if (warp == kPmLoadWarp) {
+        // ------------------------------------------------------------ copies
+        if (lane == 0) {
             tma_prefetch_map(&map_q);
             tma_prefetch_map(&map_k);
             tma_prefetch_map(&map_v);
-            auto load = [&](uint8_t* dst, const CUtensorMap* map, int head, int token,
-                            uint64_t* bar) {
-                tma_load_3d(dst, map, 0, head, token, bar);
-                tma_load_3d(dst + kPmHalfBytes, map, 64, head, token, bar);
-            };
-            mbar_arrive_expect_tx(&sh->q_full, n_tiles * kPmTileBytes);
-            for (int t = 0; t < n_tiles; ++t)
-                load(s_q + t * kPmTileBytes, &map_q, G == 1 ? head0 : head0 + t,
-                     q0 + row0 + (G == 1 ? t * kPmTile : 0), &sh->q_full);
-            int issued = 0;
-            bool ok = true;
-            for (int i = 0; i < 2 * n_blocks; ++i) {  // K0 V0 K1 V1 ...
-                const int st = i % kPmStages;
-                if (i >= kPmStages) {
-                    ok = pm_wait(p, sh, &sh->kv_empty[st], (i / kPmStages - 1) & 1);
+        }
+        auto load = [&](uint8_t* dst, const CUtensorMap& map, int head, int token, uint64_t* bar) {
+            tma_load_3d(dst, &map, 0, head, token, bar);
+            tma_load_3d(dst + kPmHalfBytes, &map, 64, head, token, bar);
+        };
+        PmItem it;
+        uint32_t i = 0;      // K/V tiles issued: K0 V0 K1 V1 ... of each item
+        uint32_t loads = 0;  // items with keys
+        bool ok = true;
+        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
+            if (it.n_blocks == 0) {
+                if (lane == 0) mbar_arrive(&sh->issued);
+                continue;
+            }
+            if (loads > 0) ok = pm_wait_warp(p, sh, &sh->q_empty, (loads - 1) & 1u);
+            if (!ok) break;
+            ++loads;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sh->q_full, it.n_tiles * kPmTileBytes);
+                for (int t = 0; t < it.n_tiles; ++t)
+                    load(s_q + t * kPmTileBytes, map_q, it.G == 1 ? it.head0 : it.head0 + t,
+                         it.q0 + it.row0 + (it.G == 1 ? t * kPmTile : 0), &sh->q_full);
+                for (int c = 0; ok && c < 2 * it.n_blocks; ++c, ++i) {
+                    const int st = i % kPmStages;
+                    if (i >= (uint32_t)kPmStages)
+                        ok = pm_wait(p, sh, &sh->kv_empty[st], (i / kPmStages - 1) & 1u);
                     if (!ok) break;
+                    mbar_arrive_expect_tx(&sh->kv_full[st], kPmTileBytes);
+                    if (c & 1)
+                        load(s_kv + st * kPmTileBytes, map_v, it.kvh, it.k0 + (c >> 1) * kPmTile,
+                             &sh->kv_full[st]);
+                    else
+                        load(s_kv + st * kPmTileBytes, map_k, it.kvh, it.k0 + (c >> 1) * kPmTile,
+                             &sh->kv_full[st]);
                 }
-                mbar_arrive_expect_tx(&sh->kv_full[st], kPmTileBytes);
-                load(s_kv + st * kPmTileBytes, (i & 1) ? &map_v : &map_k, kvh,
-                     k0 + (i >> 1) * kPmTile, &sh->kv_full[st]);
-                ++issued;
+                mbar_arrive(&sh->issued);
             }
-            // copies in flight land before the CTA ends (bounded)
-            if (!ok) {
-                mbar_wait_bounded(&sh->q_full, 0, nullptr);
-                for (int i = max(0, issued - kPmStages); i < issued; ++i)
-                    mbar_wait_bounded(&sh->kv_full[i % kPmStages], (i / kPmStages) & 1, nullptr);
-            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        // copies in flight land before the CTA ends (bounded)
+        if (lane == 0) {
+            bool landed = loads == 0 || mbar_wait_bounded(&sh->q_full, (loads - 1) & 1u, nullptr);
+            for (uint32_t c = i > (uint32_t)kPmStages ? i - kPmStages : 0u; landed && c < i; ++c)
+                landed = mbar_wait_bounded(&sh->kv_full[c % kPmStages], (c / kPmStages) & 1u, nullptr);
         }
         __syncwarp();
-        if (n_blocks > 0 && tail < kPmTile) {
-            // Rows of V behind the last key belong to other sequences or to
-            // nobody and may hold anything; their weights are 0, and 0 * NaN
-            // is not: zero them before the product reads the tile.
-            const int i = 2 * n_blocks - 1;
-            const int st = i % kPmStages;
-            bool ok = pm_wait(p, sh, &sh->kv_full[st], (i / kPmStages) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                uint8_t* tile = s_kv + st * kPmTileBytes;
-                for (int c = tail * 8 + lane; c < kPmTile * 8; c += 32) {
-                    *reinterpret_cast<uint4*>(tile + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(tile + kPmHalfBytes + c * 16) =
+    } else if (warp == kPmMmaWarp) {
+        // ------------------------------------------------------------ products
+        // The whole warp walks the loop, so that descriptors and addresses are
+        // uniform values; one elected lane issues the products and commits.
+        constexpr uint32_t kDescQk = mma_desc_f16(kPmTile, kPmTile, kBf16, false);
+        constexpr uint32_t kDescPv = mma_desc_f16(kPmTile, kHeadDim, kBf16, true);
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(s_q), 16, 1024);
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(s_kv), 16, 1024);
+        const uint64_t v_desc = smem_desc_sw128(smem_u32(s_kv), kPmHalfBytes, 1024);
+        constexpr uint32_t kTileStep = kPmTileBytes >> 4;  // in descriptor units
+        // S of tile t from the K tile in stage st
+        auto scores = [&](int t, int st) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                const uint32_t off = ((ks >> 2) * kPmHalfBytes + (ks & 3) * 32) >> 4;
+                mma_f16_ss(t * 128, q_desc + (t * kTileStep + off), k_desc + (st * kTileStep + off),
+                           kDescQk, ks > 0);
+            }
+        };
+        // O of tile t plus keys 32 part .. 32 part + 31 of the V tile in stage st
+        auto output = [&](int t, int st, int part, bool accumulate) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int ks = 2 * part + k;
+                mma_f16_ts(256 + t * 128, t * 128 + ks * 8, v_desc + (st * kTileStep + ks * 128),
+                           kDescPv, accumulate || ks > 0);
+            }
+        };
+        PmItem it{};
+        uint32_t gb = 0;               // blocks of the items before
+        uint32_t items = 0;            // items with keys
+        uint32_t blocks[2] = {0u, 0u}, outs[2] = {0u, 0u};  // each tile's blocks and items
+        // Block j of the item; its K tile is in stage 0 or 2, V in the next: with
+        // stages and tiles known at compile time every operand of a product is
+        // a constant away from a loop invariant.
+        auto block = [&](int j, auto odd) -> bool {
+            constexpr int sv = decltype(odd)::value ? 3 : 1;
+            constexpr int sk = decltype(odd)::value ? 0 : 2;
+            const uint32_t g = gb + j;  // its V tile is number 2 g + 1 of the ring
+            const bool more = j + 1 < it.n_blocks;
+            if (!pm_wait_warp(p, sh, &sh->kv_full[sv], (g >> 1) & 1u)) return false;
+            if (!more && it.tail < kPmTile) {
+                // Rows of V behind the last key belong to other sequences or to
+                // nobody and may hold anything; their weights are 0, and 0 * NaN
+                // is not: zero them (while the softmax is still at its weights).
+                uint8_t* tile = s_kv + sv * kPmTileBytes;
+                for (int x = it.tail * 8 + lane; x < kPmTile * 8; x += 32) {
+                    *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(tile + kPmHalfBytes + x * 16) =
                         make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->tail);
             }
-        }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ products
-        // The whole warp walks the loop, so that descriptors and addresses are
-        // uniform values; one elected lane issues the products and commits.
-        if (n_blocks > 0) {
-            constexpr uint32_t kDescQk = mma_desc_f16(kPmTile, kPmTile, kBf16, false);
-            constexpr uint32_t kDescPv = mma_desc_f16(kPmTile, kHeadDim, kBf16, true);
-            const uint64_t q_desc = smem_desc_sw128(smem_u32(s_q), 16, 1024);
-            const uint64_t k_desc = smem_desc_sw128(smem_u32(s_kv), 16, 1024);
-            const uint64_t v_desc = smem_desc_sw128(smem_u32(s_kv), kPmHalfBytes, 1024);
-            constexpr uint32_t kTileStep = kPmTileBytes >> 4;  // in descriptor units
-            auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-                return __all_sync(0xffffffffu, pm_wait(p, sh, bar, parity));
-            };
-            // S of tile t from the K tile in stage st
-            auto scores = [&](int t, int st) {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t off = ((ks >> 2) * kPmHalfBytes + (ks & 3) * 32) >> 4;
-                    mma_f16_ss(t * 128, q_desc + (t * kTileStep + off),
-                               k_desc + (st * kTileStep + off), kDescQk, ks > 0);
-                }
-            };
-            // O of tile t plus keys 64 half .. 64 half + 63 of the V tile in stage st
-            auto output = [&](int t, int st, int half, bool accumulate) {
+            for (int t = 0; t < 2; ++t) {
+                if (t >= it.n_tiles) break;
+                const bool last = t == it.n_tiles - 1;
+                // the item before has read its output
+                if (j == 0 && outs[t] > 0 &&
+                    !pm_wait_warp(p, sh, &sh->o_empty[t], (outs[t] - 1) & 1u))
+                    return false;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int ks = 4 * half + k;
-                    mma_f16_ts(256 + t * 128, t * 128 + ks * 8,
-                               v_desc + (st * kTileStep + ks * 128), kDescPv, accumulate || ks > 0);
-                }
-            };
-            bool ok = wait(&sh->q_full, 0) && wait(&sh->kv_full[0], 0);
-            if (ok && elect_one()) {
-                scores(0, 0);
-                tc_commit(&sh->s_full[0]);
-                if (n_tiles == 2) {
-                    scores(1, 0);
-                    tc_commit(&sh->s_full[1]);
-                }
-                tc_commit(&sh->kv_empty[0]);
-            }
-            __syncwarp();
-            // One block; its V tile is in stage 1 or 3, the next block's K tile in
-            // stage 2 or 0: with stages and tiles known at compile time every
-            // operand of a product is a constant away from a loop invariant.
-            auto block = [&](int j, auto odd) -> bool {
-                constexpr int sv = decltype(odd)::value ? 3 : 1;
-                constexpr int sk = decltype(odd)::value ? 0 : 2;
-                const uint32_t ring = (uint32_t)(j >> 1) & 1u;  // (2 j + 1) / 4
-                const uint32_t ring_k = (uint32_t)((j + 1) >> 1) & 1u;
-                const bool more = j + 1 < n_blocks;
-                if (!wait(&sh->kv_full[sv], ring)) return false;
-                if (!more && tail < kPmTile && !wait(&sh->tail, 0)) return false;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (t >= n_tiles) break;
-                    const bool last = t == n_tiles - 1;
-                    if (!wait(&sh->p_full[t][0], j & 1)) return false;
+                for (int i = 0; i + 1 < kPmParts; ++i) {
+                    if (!pm_wait_warp(p, sh, &sh->p_full[t][i], blocks[t] & 1u)) return false;
                     tc_fence_after();
-                    if (elect_one()) output(t, sv, 0, j > 0);
+                    if (elect_one()) output(t, sv, i, j > 0);
                     __syncwarp();
-                    if (!wait(&sh->p_full[t][1], j & 1)) return false;
-                    if (more && t == 0 && !wait(&sh->kv_full[sk], ring_k)) return false;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        output(t, sv, 1, true);
-                        tc_commit(&sh->o_full[t]);
-                        if (last) tc_commit(&sh->kv_empty[sv]);
-                        if (more) {
-                            scores(t, sk);
-                            tc_commit(&sh->s_full[t]);
-                            if (last) tc_commit(&sh->kv_empty[sk]);
+                }
+                if (!pm_wait_warp(p, sh, &sh->p_full[t][kPmParts - 1], blocks[t] & 1u)) return false;
+                ++blocks[t];
+                if (more && t == 0 && !pm_wait_warp(p, sh, &sh->kv_full[sk], ((g + 1) >> 1) & 1u))
+                    return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    output(t, sv, kPmParts - 1, true);
+                    tc_commit(&sh->o_full[t]);
+                    if (last) tc_commit(&sh->kv_empty[sv]);
+                    if (more) {
+                        scores(t, sk);
+                        tc_commit(&sh->s_full[t]);
+                        if (last) {
+                            tc_commit(&sh->kv_empty[sk]);
+                            if (j + 2 == it.n_blocks) tc_commit(&sh->q_empty);
                         }
                     }
-                    __syncwarp();
                 }
-                return true;
-            };
-            static_assert(kPmStages == 4, "the stages of a block's tiles");
-            for (int j = 0; ok && j < n_blocks; j += 2) {
-                ok = block(j, std::integral_constant<bool, false>{});
-                if (ok && j + 1 < n_blocks) ok = block(j + 1, std::integral_constant<bool, true>{});
+                __syncwarp();
+                if (!more) ++outs[t];
             }
-            // the products in flight end before TMEM is freed (bounded)
-            if (elect_one()) tc_commit(&sh->drained);
+            return true;
+        };
+        auto first = [&](auto odd) {
+            constexpr int sk = decltype(odd)::value ? 2 : 0;
+            if (elect_one()) {
+                scores(0, sk);
+                tc_commit(&sh->s_full[0]);
+                if (it.n_tiles == 2) {
+                    scores(1, sk);
+                    tc_commit(&sh->s_full[1]);
+                }
+                tc_commit(&sh->kv_empty[sk]);
+                if (it.n_blocks == 1) tc_commit(&sh->q_empty);
+            }
             __syncwarp();
-            mbar_wait_bounded(&sh->drained, 0, nullptr);
+        };
+        static_assert(kPmStages == 4, "the stages of a block's tiles");
+        const std::integral_constant<bool, false> kEven{};
+        const std::integral_constant<bool, true> kOdd{};
+        bool ok = true;
+        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
+            if (it.n_blocks == 0) continue;
+            const bool odd = (gb & 1u) != 0u;
+            ok = pm_wait_warp(p, sh, &sh->q_full, items & 1u) &&
+                 pm_wait_warp(p, sh, &sh->kv_full[odd ? 2 : 0], (gb >> 1) & 1u);
+            ++items;
+            if (!ok) break;
+            tc_fence_after();
+            if (odd) first(kOdd); else first(kEven);
+            for (int j = 0; ok && j < it.n_blocks; ++j) {
+                if (((gb + j) & 1u) != 0u) ok = block(j, kOdd); else ok = block(j, kEven);
+            }
+            gb += it.n_blocks;
         }
+        // the products in flight end before TMEM is freed (bounded)
+        if (elect_one()) tc_commit(&sh->drained);
         __syncwarp();
-    } else {
+        mbar_wait_bounded(&sh->drained, 0, nullptr);
+    } else if (warp < kPmSoftmaxWarps) {
         // ------------------------------------------------------------ softmax
         const int t = warp >> 2;  // query tile
-        const int r = threadIdx.x & 127;
-        const int qrow = row0 + (G == 1 ? t * kPmTile : 0) + r;  // row of the sequence
-        const int head = G == 1 ? head0 : head0 + t;
-        const bool real = t < n_tiles && qrow < lq;
-        if (t < n_tiles) {
-            const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 * (warp % 4) in bits 31..16
-            const uint32_t t_s = tmem + lanes + t * 128;
-            const uint32_t t_o = tmem + lanes + 256 + t * 128;
-            const int n = visible(qrow);
-            // blocks below need no mask for any row of the tile
-            const int clear = visible(qrow - r) / kPmTile;
+        const int r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 * (warp % 4) in bits 31..16
+        const uint32_t t_s = lanes + t * 128;
+        const uint32_t t_o = lanes + 256 + t * 128;
+        uint32_t blocks = 0;  // of this tile
+        bool ok = true;
+        for (uint32_t n = 0; ok && pm_wait_work(p, sh, n); ++n) {
+            // what the loop over the blocks needs; the rest is taken from the
+            // item again after it
+            int n_blocks, keys, clear;
+            bool mine;
+            {
+                const PmItem it = pm_item(p, sh->work[n % kPmWorks]);
+                mine = t < it.n_tiles;
+                const int tile0 = it.row0 + (it.G == 1 ? t * kPmTile : 0);
+                keys = it.visible(tile0 + r);
+                // blocks below need no mask for any row of the tile
+                clear = it.visible(tile0) / kPmTile;
+                n_blocks = it.n_blocks;
+            }
+            if (!mine) {
+                pm_release_work(sh, n);
+                continue;
+            }
             float m = -INFINITY;  // what the weights refer to (raw score units)
             float l = 0.f;
-            bool ok = true;
-            for (int j = 0; j < n_blocks; ++j) {
-                ok = __all_sync(0xffffffffu, pm_wait(p, sh, &sh->s_full[t], j & 1));
+            for (int j = 0; j < n_blocks; ++j, ++blocks) {
+                ok = pm_wait_warp(p, sh, &sh->s_full[t], blocks & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_wait_ld32(s + 32 * c);
-                if (j >= clear) {
-                    const int lim = n - j * kPmTile;
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c >= lim) s[c] = 0xff800000u;
-                }
                 float mx[4] = {m, m, m, m};
+                const int lim = keys - j * kPmTile;
+                tmem_ld32(t_s, s);
+                tmem_ld32(t_s + 32, s + 32);
 #pragma unroll
-                for (int c = 0; c < 128; c += 2)
-                    mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], __uint_as_float(s[c])),
-                                             __uint_as_float(s[c + 1]));
+                for (int h = 0; h < 2; ++h) {
+                    tmem_wait_ld32(s + 64 * h);
+                    tmem_wait_ld32(s + 64 * h + 32);
+                    if (h == 0) {
+                        tmem_ld32(t_s + 64, s + 64);
+                        tmem_ld32(t_s + 96, s + 96);
+                    }
+                    if (j >= clear) {
+#pragma unroll
+                        for (int c = 64 * h; c < 64 * h + 64; ++c)
+                            if (c >= lim) s[c] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int c = 64 * h; c < 64 * h + 64; c += 2)
+                        mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], __uint_as_float(s[c])),
+                                                 __uint_as_float(s[c + 1]));
+                }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 // (a maximum of -inf: the difference is NaN, no move)
                 const bool move = (top - m) * p.scale_log2 > kPmLazy;
@@ -347,18 +513,18 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     m = to;
                     l *= f;
                     if (j > 0) {
-                        ok = __all_sync(0xffffffffu, pm_wait(p, sh, &sh->o_full[t], (j - 1) & 1));
+                        ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + 32 * c, o);
-                            tmem_wait_ld32(o);
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + 16 * c, o);
+                            tmem_wait_ld16(o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
+                            for (int i = 0; i < 16; ++i)
                                 o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(t_o + 32 * c, o);
+                            tmem_st16(t_o + 16 * c, o);
                         }
                     }
                 }
@@ -367,13 +533,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 const uint64_t base2 = pack_f32x2(-base, -base);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[32];
+                for (int c = 0; c < kPmParts; ++c) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         const uint64_t x = fma_f32x2(
-                            pack_f32x2(__uint_as_float(s[64 * c + 2 * i]),
-                                       __uint_as_float(s[64 * c + 2 * i + 1])),
+                            pack_f32x2(__uint_as_float(s[32 * c + 2 * i]),
+                                       __uint_as_float(s[32 * c + 2 * i + 1])),
                             scale2, base2);
                         float a, d;
                         unpack_f32x2(x, a, d);
@@ -382,7 +548,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(a, d));
                         w[i] = ElemOps<T>::pack(a, d);
                     }
-                    tmem_st32(t_s + 32 * c, w);
+                    tmem_st16(t_s + 16 * c, w);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -392,72 +558,81 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
                 l += lo + hi;
             }
+            if (!ok) break;
             // ---- output rows
-            if (ok && n_blocks > 0)
-                ok = __all_sync(0xffffffffu,
-                                pm_wait(p, sh, &sh->o_full[t], (n_blocks - 1) & 1));
-            tc_fence_after();
-            if (ok) {
-                T* out = reinterpret_cast<T*>(p.out) +
-                         ((size_t)(q0 + min(qrow, lq - 1)) * p.Hq + head) * kHeadDim;
-                float* lse =
-                    p.lse != nullptr ? p.lse + (size_t)(q0 + min(qrow, lq - 1)) * p.Hq + head : nullptr;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                float worst = 0.f;  // NaN if any value of the row is not finite
+            const PmItem it = pm_item(p, sh->work[n % kPmWorks]);
+            const int qrow = it.row0 + (it.G == 1 ? t * kPmTile : 0) + r;  // of the sequence
+            const int head = it.G == 1 ? it.head0 : it.head0 + t;
+            const bool real = qrow < it.lq;
+            if (it.n_blocks > 0) {
+                ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const size_t at = (size_t)(it.q0 + min(qrow, it.lq - 1)) * p.Hq + head;
+            T* out = reinterpret_cast<T*>(p.out) + at * kHeadDim;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float worst = 0.f;  // NaN if any value is not finite
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    if (n_blocks > 0) {
-                        tmem_ld32(t_o + 32 * c, o);
-                        tmem_wait_ld32(o);
-                    } else {
+            for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                if (it.n_blocks > 0) {
+                    tmem_ld32(t_o + 32 * c, o);
+                    tmem_wait_ld32(o);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0u;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) worst = fmaf(__uint_as_float(o[i]), 0.f, worst);
-                    if (real) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 u;
-                            u.x = ElemOps<T>::pack(__uint_as_float(o[8 * i]) * inv,
-                                                   __uint_as_float(o[8 * i + 1]) * inv);
-                            u.y = ElemOps<T>::pack(__uint_as_float(o[8 * i + 2]) * inv,
-                                                   __uint_as_float(o[8 * i + 3]) * inv);
-                            u.z = ElemOps<T>::pack(__uint_as_float(o[8 * i + 4]) * inv,
-                                                   __uint_as_float(o[8 * i + 5]) * inv);
-                            u.w = ElemOps<T>::pack(__uint_as_float(o[8 * i + 6]) * inv,
-                                                   __uint_as_float(o[8 * i + 7]) * inv);
-                            reinterpret_cast<uint4*>(out)[4 * c + i] = u;
-                        }
-                    }
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;
                 }
-                if (real && lse != nullptr)
-                    *lse = l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
-                // A value that is not finite may come from a key the row does
-                // not see (weight 0 times an infinite or NaN V): such a row is
-                // computed again from its own keys alone.
-                __syncwarp();
-                unsigned again = __ballot_sync(0xffffffffu, real && worst != 0.f);
-                while (again != 0u) {
-                    const int i = __ffs(again) - 1;
-                    again &= again - 1;
-                    const int row = qrow - lane + i;  // of the sequence
-                    const size_t at = (size_t)(q0 + row) * p.Hq + head;
-                    prompt_row<T>(p, p.q + (q0 + row) * p.q_tok + head * p.q_head,
-                                  p.k + k0 * p.k_tok + kvh * p.k_head,
-                                  p.v + k0 * p.v_tok + kvh * p.v_head, visible(row),
-                                  reinterpret_cast<T*>(p.out) + at * kHeadDim,
-                                  p.lse != nullptr ? p.lse + at : nullptr, lane);
+                if (c == 3 && it.n_blocks > 0) {
+                    // TMEM has been read: the next item's output may start
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->o_empty[t]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) worst = fmaf(__uint_as_float(o[i]), 0.f, worst);
+                if (real) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 u;
+                        u.x = ElemOps<T>::pack(__uint_as_float(o[8 * i]) * inv,
+                                               __uint_as_float(o[8 * i + 1]) * inv);
+                        u.y = ElemOps<T>::pack(__uint_as_float(o[8 * i + 2]) * inv,
+                                               __uint_as_float(o[8 * i + 3]) * inv);
+                        u.z = ElemOps<T>::pack(__uint_as_float(o[8 * i + 4]) * inv,
+                                               __uint_as_float(o[8 * i + 5]) * inv);
+                        u.w = ElemOps<T>::pack(__uint_as_float(o[8 * i + 6]) * inv,
+                                               __uint_as_float(o[8 * i + 7]) * inv);
+                        reinterpret_cast<uint4*>(out)[4 * c + i] = u;
+                    }
                 }
             }
+            if (real && p.lse != nullptr)
+                p.lse[at] = l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
+            // A value that is not finite may come from a key the row does not see
+            // (weight 0 times an infinite or NaN V): such a row is computed again
+            // from its own keys alone.
+            __syncwarp();
+            unsigned again = __ballot_sync(0xffffffffu, real && worst != 0.f);
+            while (again != 0u) {
+                const int i = __ffs(again) - 1;
+                again &= again - 1;
+                const int row = qrow - lane + i;  // of the sequence
+                const size_t to = (size_t)(it.q0 + row) * p.Hq + head;
+                prompt_row<T>(p, p.q + (it.q0 + row) * p.q_tok + head * p.q_head,
+                              p.k + it.k0 * p.k_tok + it.kvh * p.k_head,
+                              p.v + it.k0 * p.v_tok + it.kvh * p.v_head, it.visible(row),
+                              reinterpret_cast<T*>(p.out) + to * kHeadDim,
+                              p.lse != nullptr ? p.lse + to : nullptr, lane);
+            }
+            pm_release_work(sh, n);
         }
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kPmMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, kPmTmemColumns);
+        tmem_dealloc(sh->tmem, kPmTmemColumns);
     }
 }
 

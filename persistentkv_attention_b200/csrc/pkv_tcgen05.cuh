@@ -104,6 +104,38 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
         : "memory");
 }
 
+// ---------------------------------------------------------------- launch control
+// Asks for a CTA of this grid that has not started: 16 bytes of answer to
+// `answer` (shared memory), as transaction bytes on `bar`.  Not asked again
+// once an answer was no.
+__device__ __forceinline__ void launch_cancel_async(void* answer, uint64_t* bar) {
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+        "[%0], [%1];" ::"r"(smem_u32(answer)),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Whether a CTA was given, and its blockIdx.x.
+__device__ __forceinline__ bool launch_cancelled(const void* answer, int& block) {
+    uint32_t yes, x;
+    asm volatile(
+        "{\n"
+        " .reg .pred p;\n"
+        " .reg .b128 a;\n"
+        " ld.shared.b128 a, [%2];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+        " selp.u32 %0, 1, 0, p;\n"
+        " mov.u32 %1, 0;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n"
+        "}\n"
+        : "=r"(yes), "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    if (yes != 0u) block = (int)x;
+    return yes != 0u;
+}
+
 // ---------------------------------------------------------------- pairs
 // Two fp32 values in one 64-bit register pair: one instruction for both.
 __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
@@ -147,6 +179,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
 #undef PKV_O
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+#define PKV_O(i) "=r"(r[i])
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : PKV_R16(PKV_O, 0)
+        : "r"(addr));
+#undef PKV_O
+}
+
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+#define PKV_O(i) "+r"(r[i])
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : PKV_R16(PKV_O, 0)::"memory");
+#undef PKV_O
+}
+
 // Waits for the thread's TMEM loads; the registers pass through so that no
 // use of them moves before the wait.
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
@@ -155,13 +203,12 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
 #undef PKV_O
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 #define PKV_O(i) "r"(r[i])
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::
-            PKV_R32(PKV_O, 0),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::PKV_R16(PKV_O,
+                                                                                            0),
         "r"(addr)
         : "memory");
 #undef PKV_O
