@@ -336,13 +336,13 @@ pkv_status pkv_paged_attention_auto_fp8_block(
  *   cu_seqlens [B + 1]; seq_lens[b] = cached + new (cached if not served);
  *   *free_left = *free_count less the pages taken (may be the same word).
  * A row is not served if its lengths are negative or exceed
- * max_pages * page_size (PKV_DEVERR_LOGICAL_PAGE), or if it needs pages and
- * the rows up to it need more than the stack holds (PKV_DEVERR_NO_PAGE).
+ * max_pages * page_size (PKV_DEVERR_LOGICAL_PAGE), if it needs pages and the
+ * rows up to it need more than the stack holds (PKV_DEVERR_NO_PAGE), or if its
+ * tokens do not fit into num_slots (PKV_DEVERR_SLOT).
  * free_pages NULL: every page is in block_table already (free_count,
  * free_left and counters are not used).  A page id that is negative or too
- * large for 32-bit slots gives slot -1 (PKV_DEVERR_PAGE_ID); more new tokens
- * than num_slots set PKV_DEVERR_SLOT, those beyond get no slot.  counters: one
- * zeroed int32, left zero.  No buffer written may overlap cached_lens or
+ * large for 32-bit slots gives slot -1 (PKV_DEVERR_PAGE_ID).  counters: one
+ * zeroed int32, left zero (used where free_left is free_count).  No buffer written may overlap cached_lens or
  * new_lens.  Two calls that overlap on the GPU must not share a stack or
  * counters. */
 pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,

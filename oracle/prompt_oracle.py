@@ -73,7 +73,8 @@ def prompt_slots(cached, new, table, num_slots, page, free=None, free_count=0):
         cu[r] = at
         fits = c >= 0 and n >= 0 and c + n <= width * page
         need = -(-(c + n) // page) - -(-c // page) if fits and free is not None else 0
-        served = fits and (need == 0 or asked + need <= free_count)
+        served = (fits and (need == 0 or asked + need <= free_count)
+                  and (n <= 0 or at + n <= num_slots))
         if served:
             for j in range(need):
                 table[r, -(-c // page) + j] = free[free_count - 1 - asked - j]
@@ -81,8 +82,7 @@ def prompt_slots(cached, new, table, num_slots, page, free=None, free_count=0):
                 taken = asked + need
             for i in range(n):
                 p = c + i
-                if at + i < num_slots:
-                    slots[at + i] = table[r, p // page] * page + p % page
+                slots[at + i] = table[r, p // page] * page + p % page
             seq[r] = c + n
         else:
             unserved.append(r)

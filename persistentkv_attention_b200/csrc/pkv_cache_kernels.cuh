@@ -4,6 +4,9 @@
 // and head.  Included by pkv_prompt.cu only.
 #pragma once
 
+#include <climits>
+#include <type_traits>
+
 #include "pkv_device.cuh"
 
 namespace pkv {
@@ -61,28 +64,37 @@ __device__ __forceinline__ unsigned long long slot_scan(unsigned long long v,
 // its own kSlotTokensPerCta tokens, and no CTA waits for another; the token's
 // row comes from a binary search in the scanned prefixes.  New pages are read
 // from the stack, never from block_table, where another CTA may still be
-// writing them.  Bound: launch and scan latency for a few rows (the work is a
-// few KB), the 4 B per token written for many.
+// writing them.  A thread finds the places of its tokens first, then loads
+// their pages together.  Bound: the latency of the chain lengths -> pages ->
+// slots, three trips to L2 (256 rows, 400k tokens: XXX us against 0.3 us for its
+// bytes).
 __global__ void __launch_bounds__(kSlotThreads)
     pkv_prompt_slots_kernel(const __grid_constant__ SlotsParams p) {
     __shared__ unsigned long long s_warp[kSlotThreads / 32];
     __shared__ int s_start[kSlotThreads], s_cached[kSlotThreads], s_need[kSlotThreads];
+    __shared__ int s_avail;
+    constexpr int kMine = kSlotTokensPerCta / kSlotThreads;  // tokens of a thread
     const int t = threadIdx.x;
     const long long limit = (long long)p.max_pages * p.page_size;
-    int avail = 0;
-    if (p.free_pages != nullptr) {
-        avail = *p.free_count;
-        if (avail < 0) avail = 0;
-        if (avail > p.free_capacity) {
-            if (blockIdx.x == 0 && t == 0) raise_error(p.error, kErrIndex);
-            avail = p.free_capacity;
+    const bool stack = p.free_pages != nullptr;
+    // A stack lowered in place: the CTA that counts last as having read it
+    // writes what is left.  The count travels while the work is done.
+    const bool in_place = stack && p.free_left == p.free_count;
+    int counted = 0;
+    if (stack && t == 0) {
+        int n = *(const volatile int32_t*)p.free_count;
+        if (in_place) counted = atom_add_acq_rel_gpu(p.counters, 1);
+        if (n > p.free_capacity) {
+            if (blockIdx.x == 0) raise_error(p.error, kErrIndex);
+            n = p.free_capacity;
         }
+        s_avail = max(n, 0);
     }
     const long long t0 = (long long)blockIdx.x * kSlotTokensPerCta;
     const long long t1 = min(t0 + kSlotTokensPerCta, (long long)p.num_slots);
     long long tokens = 0, pages = 0;  // of the rows before the current chunk
-    int taken = 0;
-    bool bad_len = false, no_page = false, bad_page = false;
+    int avail = 0, taken = 0;
+    bool bad_len = false, no_page = false, bad_page = false, no_room = false;
     for (int base = 0; base < p.B; base += kSlotThreads) {
         const int b = base + t;
         int c = 0, n = 0, need = 0;
@@ -93,18 +105,21 @@ __global__ void __launch_bounds__(kSlotThreads)
             valid = c >= 0 && n >= 0 && (long long)c + n <= limit;
             if (n < 0) n = 0;
             if (!valid) bad_len = true;
-            if (valid && p.free_pages != nullptr)
+            if (valid && stack)
                 need = (c + n + p.page_size - 1) / p.page_size -
                        (c + p.page_size - 1) / p.page_size;
         }
         unsigned long long total;
         const unsigned long long pre =
             slot_scan(((unsigned long long)(unsigned)n << 32) | (unsigned)need, s_warp, total);
+        if (stack) avail = s_avail;  // (written before the scan's barriers)
         const long long start = tokens + (long long)(pre >> 32);
         const long long before = pages + (long long)(pre & 0xffffffffull);
         const bool short_of = need > 0 && before + need > avail;
-        const bool served = valid && !short_of;
+        const bool beyond = n > 0 && start + n > p.num_slots;
+        const bool served = valid && !short_of && !beyond;
         if (short_of) no_page = true;
+        if (beyond) no_room = true;
         if (served && need > 0) taken = max(taken, (int)(before + need));
         if (b < p.B && blockIdx.x == 0) {
             p.cu_seqlens[b] = (int)min(start, (long long)INT_MAX);
@@ -118,36 +133,58 @@ __global__ void __launch_bounds__(kSlotThreads)
         const long long end = tokens + (long long)(total >> 32);
         const int rows = min(kSlotThreads, p.B - base);
         const long long lo = max(t0, tokens), hi = min(t1, end);
-        for (long long tok = lo + t; tok < hi; tok += kSlotThreads) {
-            // the last row that starts at or before tok (rows of no tokens that
-            // start there come before it)
-            int a = 0, z = rows;
-            while (z - a > 1) {
-                const int m = (a + z) >> 1;
-                if ((long long)s_start[m] <= tok) a = m; else z = m;
+        // tokens t0 + t + 256 i of this chunk's rows
+        const int32_t* from[kMine];  // where the page of the token stands
+        int32_t* opened[kMine];      // block-table entry that the token opens
+        int off[kMine];
+        bool here[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const long long tok = t0 + t + i * kSlotThreads;
+            here[i] = tok >= lo && tok < hi;
+            from[i] = nullptr;
+            opened[i] = nullptr;
+            off[i] = 0;
+            if (here[i]) {
+                // the last row that starts at or before tok (rows of no tokens
+                // that start there come before it)
+                int a = 0, z = rows;
+                while (z - a > 1) {
+                    const int m = (a + z) >> 1;
+                    if ((long long)s_start[m] <= tok) a = m; else z = m;
+                }
+                const int cached = s_cached[a];
+                if (cached >= 0) {
+                    const int pos = cached + (int)(tok - s_start[a]);
+                    const int j = pos / p.page_size;
+                    off[i] = pos - j * p.page_size;
+                    int32_t* entry = p.block_table + (size_t)(base + a) * p.max_pages + j;
+                    const int first = (cached + p.page_size - 1) / p.page_size;
+                    if (stack && j >= first) {
+                        from[i] = p.free_pages + (avail - 1 - s_need[a] - (j - first));
+                        if (off[i] == 0) opened[i] = entry;
+                    } else {
+                        from[i] = entry;
+                    }
+                }
             }
-            const int cached = s_cached[a];
+        }
+        int page[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            page[i] = from[i] != nullptr ? *(const volatile int32_t*)from[i] : 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (!here[i]) continue;
             int slot = -1;
-            if (cached >= 0) {
-                const int pos = cached + (int)(tok - s_start[a]);
-                const int j = pos / p.page_size;
-                const int off = pos - j * p.page_size;
-                int32_t* entry = p.block_table + (size_t)(base + a) * p.max_pages + j;
-                const int first = (cached + p.page_size - 1) / p.page_size;
-                int page;
-                if (p.free_pages != nullptr && j >= first) {
-                    page = __ldg(p.free_pages + (avail - 1 - s_need[a] - (j - first)));
-                    if (off == 0) *entry = page;
-                } else {
-                    page = *entry;
-                }
-                if (page < 0 || page > (INT_MAX - p.page_size) / p.page_size) {
+            if (from[i] != nullptr) {
+                if (opened[i] != nullptr) *opened[i] = page[i];
+                if (page[i] < 0 || page[i] > (INT_MAX - p.page_size) / p.page_size)
                     bad_page = true;
-                } else {
-                    slot = page * p.page_size + off;
-                }
+                else
+                    slot = page[i] * p.page_size + off[i];
             }
-            p.slots[tok] = slot;
+            p.slots[t0 + t + i * kSlotThreads] = slot;
         }
         tokens = end;
         pages += (long long)(total & 0xffffffffull);
@@ -158,25 +195,18 @@ __global__ void __launch_bounds__(kSlotThreads)
     if (blockIdx.x == 0) {
         if (bad_len) raise_error(p.error, kErrLogicalPage);
         if (no_page) raise_error(p.error, kErrNoPage);
-        if (t == 0) {
-            if (tokens > p.num_slots) raise_error(p.error, kErrSlot);
-            p.cu_seqlens[p.B] = (int)min(tokens, (long long)INT_MAX);
-        }
+        if (no_room) raise_error(p.error, kErrSlot);
+        if (t == 0) p.cu_seqlens[p.B] = (int)min(tokens, (long long)INT_MAX);
     }
-    if (p.free_pages != nullptr) {
-        // every thread has read *free_count; the last CTA to get here writes
-        // what is left (free_left may be the same word)
+    if (stack && (in_place || blockIdx.x == 0)) {
         taken = __reduce_max_sync(0xffffffffu, taken);
         if ((t & 31) == 0) s_start[t >> 5] = taken;
         __syncthreads();
-        if (t == 0) {
+        if (t == 0 && (!in_place || counted == (int)gridDim.x - 1)) {
 #pragma unroll
             for (int w = 1; w < kSlotThreads / 32; ++w) taken = max(taken, s_start[w]);
-            __threadfence();
-            if (atomicAdd(p.counters, 1) == (int)gridDim.x - 1) {
-                *p.counters = 0;
-                *p.free_left = avail - taken;
-            }
+            if (in_place) *p.counters = 0;
+            *p.free_left = s_avail - taken;
         }
     }
 }
@@ -194,6 +224,7 @@ struct WriteParams {
     long long k_tok, k_head, v_tok, v_head;
     long long num_slots;  // P * page
     int T, Hkv, page_size, block;
+    int split;  // warps that share a window of tokens (e4m3 write)
 };
 
 constexpr int kWriteThreads = 256;
@@ -225,8 +256,8 @@ __global__ void __launch_bounds__(kWriteThreads)
 
 // ------------------------------------------------------------ e4m3 block write
 // The tokens of a call that fall into one block of the cache (`block` slots of
-// one page) are a run of consecutive tokens.  One warp takes one run of one
-// head's K or V: the block's scale is the least power of two, at least 2^-24,
+// one page) are a run of consecutive tokens.  A warp takes a run of one head's
+// K or V: the block's scale is the least power of two, at least 2^-24,
 // that brings the run's largest magnitude to e4m3's 448 or below, and, when
 // the run starts inside the block, at least the block's old scale, whose
 // earlier tokens stay.  A power of two makes x / scale and the move of old
@@ -254,10 +285,14 @@ __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t x) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
 }
 
-// |x| where it is finite, else 0: infinities and NaN do not set a scale.
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = fabsf(x);
-    return a < INFINITY ? a : 0.f;
+// The magnitude bits of 16-bit floats order as integers; the first that is not
+// finite:
+template <typename T>
+constexpr unsigned kInf16 = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+
+template <typename T>
+__device__ __forceinline__ float from_bits16(unsigned bits) {
+    return to_float2<T>(bits).x;
 }
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -274,18 +309,25 @@ __device__ __forceinline__ uint32_t rescale_e4m3x2(uint32_t codes, float ratio) 
 
 constexpr int kRunRows = 16;  // tokens held in registers at a time
 
-// Warp w of the grid: window of 16 tokens w / (2 Hkv), head (w / 2) % Hkv, K or
-// V by w % 2; it takes the runs that start in its window.  Lane l holds 16
-// bytes (8 elements) of tokens l / 16 + 2 i: 8 loads in flight, 4 KB a warp.
+// A window of 16 tokens of one head's K or V belongs to `split` warps: the
+// runs that start in it go to them in turn.  Long prompts start about one run
+// per window (split = 1); the new tokens of a decode step are a run each, and
+// one warp would take them one after another (64 rows: 27.9 us; with a warp
+// each 5.5 us).  Lane l holds 16 bytes (8 elements) of tokens l / 16 + 2 i: 8 loads
+// in flight, 4 KB a warp.  Bound: HBM for long prompts (reads 2 bytes, writes 1
+// per element), the chain slots -> tokens -> codes for short ones.
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads)
+__global__ void __launch_bounds__(kWriteThreads, 4)
     pkv_kv_write_block_kernel(const __grid_constant__ WriteParams p) {
     const int lane = threadIdx.x & 31;
     const long long w = ((long long)blockIdx.x * kWriteThreads + threadIdx.x) >> 5;
-    const long long window = w / (2 * p.Hkv);
+    const int per_window = 2 * p.Hkv * p.split;
+    const long long window = w / per_window;
     const long long t0 = window * kRunRows;
     if (t0 >= p.T) return;
-    const int r = (int)(w - window * (2 * p.Hkv));
+    int r = (int)(w - window * per_window);
+    const int sub = r % p.split;
+    r /= p.split;
     const int h = r >> 1;
     const bool is_v = (r & 1) != 0;
     const uint8_t* src = is_v ? p.v + h * p.v_head : p.k + h * p.k_head;
@@ -293,43 +335,47 @@ __global__ void __launch_bounds__(kWriteThreads)
     uint8_t* pool = is_v ? p.v_pages : p.k_pages;
     float* scales = is_v ? p.v_scales : p.k_scales;
     const int nblk = p.page_size / p.block;
-    // blocks of the window's tokens and of the token before it; -1 is padding
-    auto block_of = [&](long long t) -> int {
-        if (t < 0 || t >= p.T) return -1;
-        const int s = __ldg(p.slots + t);
-        if (s < 0) return -1;
-        if (s >= p.num_slots) {
-            if (r == 0) raise_error(p.error, kErrSlot);
-            return -1;
-        }
-        return s / p.block;
+    // slots and blocks of the tokens t0 - 1 .. t0 + 30; block -1 is padding
+    auto slot_of = [&](long long t) -> int {
+        return t >= 0 && t < p.T ? __ldg(p.slots + t) : -1;
     };
-    const int blk = block_of(t0 + lane - 1);  // lane 0: the token before the window
+    auto block_of = [&](int slot) -> int {
+        return slot >= 0 && slot < p.num_slots ? slot / p.block : -1;
+    };
+    const int slot = slot_of(t0 + lane - 1);
+    if (slot >= p.num_slots && r == 0) raise_error(p.error, kErrSlot);
+    const int blk = block_of(slot);
     const int prev = __shfl_up_sync(0xffffffffu, blk, 1);
     unsigned starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= kRunRows && blk >= 0 &&
                                                      blk != prev);
     const int half = lane >> 4, piece = lane & 15;
-    while (starts != 0u) {
+    for (int turn = 0; starts != 0u; ++turn) {
         const int sl = __ffs(starts) - 1;
         starts &= starts - 1;
+        if (turn % p.split != sub) continue;
         const int run_blk = __shfl_sync(0xffffffffu, blk, sl);
+        const int kept = __shfl_sync(0xffffffffu, slot, sl) - run_blk * p.block;
         const long long first = t0 + sl - 1;
-        // length of the run
-        int n = 0;
-        while (true) {
-            const unsigned same =
-                __ballot_sync(0xffffffffu, block_of(first + n + lane) == run_blk);
-            const int more = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
-            n += more;
-            if (more < 32) break;
+        // length of the run: the tokens in hand hold any run of 16, longer ones
+        // are followed
+        int n = __ffs(~(__ballot_sync(0xffffffffu, blk == run_blk) >> sl)) - 1;
+        if (n < 0 || n > 32 - sl) n = 32 - sl;
+        if (n == 32 - sl && p.block > kRunRows) {
+            while (true) {
+                const unsigned same = __ballot_sync(
+                    0xffffffffu, block_of(slot_of(first + n + lane)) == run_blk);
+                const int more = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+                n += more;
+                if (more < 32) break;
+            }
         }
         const int page = run_blk / nblk, g = run_blk % nblk;
         float* scale_at = scales + ((size_t)page * p.Hkv + h) * nblk + g;
         uint8_t* block_base =
             pool + (((size_t)page * p.Hkv + h) * p.page_size + (size_t)g * p.block) * kHeadDim;
-        const int kept = __ldg(p.slots + first) - run_blk * p.block;
+        float old = 0.f;
+        if (kept > 0) old = *scale_at;
         uint4 x[kRunRows / 2];
-        float amax = 0.f;
         auto load = [&](int base) {
 #pragma unroll
             for (int i = 0; i < kRunRows / 2; ++i) {
@@ -339,22 +385,39 @@ __global__ void __launch_bounds__(kWriteThreads)
                                : make_uint4(0u, 0u, 0u, 0u);
             }
         };
+        // the largest magnitude, two elements at a time on their bits
+        unsigned top2 = 0u;
         for (int base = 0; base < n; base += kRunRows) {
             load(base);
 #pragma unroll
             for (int i = 0; i < kRunRows / 2; ++i) {
-                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = to_float2<T>(u[j]);
-                    amax = fmaxf(amax, fmaxf(finite_abs(f.x), finite_abs(f.y)));
-                }
+                top2 = __vmaxu2(top2, x[i].x & 0x7fff7fffu);
+                top2 = __vmaxu2(top2, x[i].y & 0x7fff7fffu);
+                top2 = __vmaxu2(top2, x[i].z & 0x7fff7fffu);
+                top2 = __vmaxu2(top2, x[i].w & 0x7fff7fffu);
             }
         }
-        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-        float scale = block_scale(amax);
+        unsigned top = __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16));
+        if (top >= kInf16<T>) {
+            // infinities and NaN do not set a scale: again without them
+            top = 0u;
+            for (int base = 0; base < n; base += kRunRows) {
+                load(base);
+#pragma unroll
+                for (int i = 0; i < kRunRows / 2; ++i) {
+                    const unsigned u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const unsigned a = (u[j >> 1] >> (16 * (j & 1))) & 0x7fffu;
+                        if (a < kInf16<T>) top = max(top, a);
+                    }
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (n > kRunRows) load(0);
+        }
+        float scale = block_scale(from_bits16<T>(top));
         if (kept > 0) {
-            const float old = *scale_at;
             if (old > scale) {
                 scale = old;
             } else if (old < scale) {
@@ -378,14 +441,16 @@ __global__ void __launch_bounds__(kWriteThreads)
 #pragma unroll
             for (int i = 0; i < kRunRows / 2; ++i) {
                 const int row = base + half + 2 * i;
+                const int near = __shfl_sync(0xffffffffu, slot, (sl + row) & 31);
                 if (row >= n) continue;
-                const int off = __ldg(p.slots + first + row) - run_blk * p.block;
+                const int to = sl + row < 32 ? near : __ldg(p.slots + first + row);
                 const float2 a = to_float2<T>(x[i].x), b = to_float2<T>(x[i].y);
                 const float2 c = to_float2<T>(x[i].z), d = to_float2<T>(x[i].w);
                 uint2 out;
                 out.x = e4m3x2(a.x * inv, a.y * inv) | (e4m3x2(b.x * inv, b.y * inv) << 16);
                 out.y = e4m3x2(c.x * inv, c.y * inv) | (e4m3x2(d.x * inv, d.y * inv) << 16);
-                reinterpret_cast<uint2*>(block_base + (size_t)off * kHeadDim)[piece] = out;
+                reinterpret_cast<uint2*>(block_base + (size_t)(to - run_blk * p.block) * kHeadDim)[piece] =
+                    out;
             }
         }
     }

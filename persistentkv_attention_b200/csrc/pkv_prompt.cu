@@ -80,6 +80,7 @@ pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_p
     wp.Hkv = Hkv;
     wp.page_size = page_size;
     wp.block = page_size;
+    wp.split = 1;
     return PKV_OK;
 }
 
@@ -239,8 +240,11 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
     unsigned grid = 0;
+    // up to a warp per token while the card has room for them (32 warps an SM)
     const long long windows = ((long long)T + kRunRows - 1) / kRunRows;
-    st = grid_of(windows * 2 * Hkv * 32, kWriteThreads, &grid);
+    wp.split = 1;
+    while (wp.split < kRunRows && windows * 2 * Hkv * wp.split * 2 <= 32ll * sms) wp.split *= 2;
+    st = grid_of(windows * 2 * Hkv * wp.split * 32, kWriteThreads, &grid);
     if (st != PKV_OK) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PKV_DTYPE_F16)

@@ -35,6 +35,7 @@ HEAD_DIM = 128
 STATE_STRIDE = HEAD_DIM + 2
 
 _DTYPES = {torch.float16: _native.PKV_DTYPE_F16, torch.bfloat16: _native.PKV_DTYPE_BF16}
+_SUPPORTED_G = (1, 2, 4, 8)
 
 
 def _check_tensor(tensor: torch.Tensor, name: str, dtype, dims: int) -> None:
@@ -554,12 +555,24 @@ def kv_append(k_new, v_new, k_pages, v_pages, block_table, positions, free_pages
         k_pages.size(2), block_table.size(1), _DTYPES[dt], _stream()))
 
 
+# The calls below are a few microseconds of GPU work at their smallest, so their
+# checks are two: one expression over everything a call needs, and, where it
+# fails, the checks that say what is wrong.
+
+
 def _check_current_device(*tensors) -> None:
     """Kernels launch on the current device: every operand must live there."""
     device = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise RuntimeError(f"operands must be on the current device, cuda:{device}")
+
+
+def _stream_of(device: int) -> int:
+    """Raw stream of ``device``, which is the current one."""
+    if _raw_stream is not None:
+        return _raw_stream(device)
+    return torch.cuda.current_stream().cuda_stream
 
 
 def _check_packed(t, name: str, dtype) -> None:
@@ -590,14 +603,8 @@ def _check_block_scales(k_pages, k_scales, v_scales) -> int:
     return page_size // blocks
 
 
-def paged_attention_auto_fp8_block(q_source, k_pages, v_pages, k_scales, v_scales, block_table,
-                                   seq_lens, output, workspace, q_indices=None, out_indices=None,
-                                   merge_counters=None) -> None:
-    """``paged_attention_auto`` over an e4m3 (``torch.float8_e4m3fn``) K/V cache
-    with one float32 scale per block of tokens and head: ``k_scales`` /
-    ``v_scales`` [P, Hkv, page_size / block], block a multiple of 16 tokens.  q
-    and output are fp16 or bf16.  Half the cache's bytes, read at the same
-    rate.  No counterpart in the reference."""
+def _check_block_decode(q_source, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens,
+                        output, workspace, q_indices, out_indices, merge_counters) -> None:
     _check_tensor(q_source, "q_source", tuple(_DTYPES), 3)
     _check_tensor(k_pages, "k_pages", torch.float8_e4m3fn, 4)
     _check_tensor(v_pages, "v_pages", torch.float8_e4m3fn, 4)
@@ -606,9 +613,9 @@ def paged_attention_auto_fp8_block(q_source, k_pages, v_pages, k_scales, v_scale
     _check_tensor(output, "output", q_source.dtype, 3)
     if v_pages.shape != k_pages.shape or k_pages.size(3) != HEAD_DIM:
         raise RuntimeError("k_pages / v_pages shape mismatch")
-    physical_pages, hkv, page_size, _ = k_pages.shape
-    block = _check_block_scales(k_pages, k_scales, v_scales)
-    b, max_pages = block_table.shape
+    hkv = k_pages.size(1)
+    _check_block_scales(k_pages, k_scales, v_scales)
+    b = block_table.size(0)
     q_rows, hq, d = q_source.shape
     if d != HEAD_DIM:
         raise RuntimeError("PersistentKV extension currently requires d=128")
@@ -616,33 +623,97 @@ def paged_attention_auto_fp8_block(q_source, k_pages, v_pages, k_scales, v_scale
         raise RuntimeError("seq_lens batch mismatch")
     if output.size(1) != hq or output.size(2) != d:
         raise RuntimeError("output shape must match q head dimensions")
-    ptrs = []
     for name, t in (("q_indices", q_indices), ("out_indices", out_indices)):
-        if t is None:
-            ptrs.append(None)
-        else:
+        if t is not None:
             _check_tensor(t, name, torch.int32, 1)
             if t.size(0) != b:
                 raise RuntimeError(f"{name} batch mismatch")
-            ptrs.append(t.data_ptr())
     # without an index tensor row b reads q_source[b] and writes output[b]
     if (q_indices is None and q_rows < b) or (out_indices is None and output.size(0) < b):
         raise RuntimeError("q_source and output need a row per block_table row")
-    ctr = None
     if merge_counters is not None:
         _check_tensor(merge_counters, "merge_counters", torch.int32, 2)
         if merge_counters.size(0) != b or merge_counters.size(1) != hkv:
             raise RuntimeError("merge_counters shape mismatch")
-        ctr = merge_counters.data_ptr()
     _check_supported_gqa(hq, hkv)
-    ws_ptr, ws_bytes = _workspace(workspace)
+    _workspace(workspace)
     _check_current_device(q_source, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens,
                           output, workspace, q_indices, out_indices, merge_counters)
+
+
+def paged_attention_auto_fp8_block(q_source, k_pages, v_pages, k_scales, v_scales, block_table,
+                                   seq_lens, output, workspace, q_indices=None, out_indices=None,
+                                   merge_counters=None) -> None:
+    """``paged_attention_auto`` over an e4m3 (``torch.float8_e4m3fn``) K/V cache
+    with one float32 scale per block of tokens and head: ``k_scales`` /
+    ``v_scales`` [P, Hkv, page_size / block], block a multiple of 16 tokens.  q
+    and output are fp16 or bf16.  Half the cache's bytes, read at the same
+    rate.  No counterpart in the reference."""
+    dt, pool, scale, table = q_source.dtype, k_pages.shape, k_scales.shape, block_table.shape
+    qs, outs, dev = q_source.shape, output.shape, q_source.get_device()
+    i32, f8 = torch.int32, torch.float8_e4m3fn
+    if not (
+        dev >= 0 and dt in _DTYPES and output.dtype is dt and k_pages.dtype is f8
+        and v_pages.dtype is f8 and k_scales.dtype is torch.float32
+        and v_scales.dtype is torch.float32 and block_table.dtype is i32 and seq_lens.dtype is i32
+        and len(qs) == 3 and len(outs) == 3 and len(pool) == 4 and len(scale) == 3
+        and len(table) == 2 and seq_lens.shape == table[:1] and qs[1:] == outs[1:]
+        and qs[2] == HEAD_DIM and pool[3] == HEAD_DIM and v_pages.shape == pool
+        and v_scales.shape == scale and scale[:2] == pool[:2] and scale[2] > 0
+        and pool[2] % (16 * scale[2]) == 0 and pool[1] > 0 and qs[1] % pool[1] == 0
+        and qs[1] // pool[1] in _SUPPORTED_G
+        and q_indices is None and out_indices is None and qs[0] >= table[0] and outs[0] >= table[0]
+        and q_source.is_contiguous() and output.is_contiguous() and k_pages.is_contiguous()
+        and v_pages.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+        and block_table.is_contiguous() and seq_lens.is_contiguous()
+        and workspace.is_contiguous() and k_pages.get_device() == dev
+        and v_pages.get_device() == dev and k_scales.get_device() == dev
+        and v_scales.get_device() == dev and block_table.get_device() == dev
+        and seq_lens.get_device() == dev and output.get_device() == dev
+        and workspace.get_device() == dev and torch.cuda.current_device() == dev
+        and (merge_counters is None or (
+            merge_counters.dtype is i32 and merge_counters.shape == (table[0], pool[1])
+            and merge_counters.is_contiguous() and merge_counters.get_device() == dev))
+    ):
+        _check_block_decode(q_source, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens,
+                            output, workspace, q_indices, out_indices, merge_counters)
+    ws_bytes = workspace.numel() * workspace.element_size()
     _native.check(_native.load().pkv_paged_attention_auto_fp8_block(
         q_source.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
-        v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ptrs[0], ptrs[1],
-        output.data_ptr(), ws_ptr, ws_bytes, ctr, b, q_rows, output.size(0), hq, hkv, d,
-        physical_pages, page_size, max_pages, block, _DTYPES[q_source.dtype], _stream()))
+        v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        None if q_indices is None else q_indices.data_ptr(),
+        None if out_indices is None else out_indices.data_ptr(), output.data_ptr(),
+        workspace.data_ptr() if ws_bytes else None, ws_bytes,
+        None if merge_counters is None else merge_counters.data_ptr(), table[0], qs[0], outs[0],
+        qs[1], pool[1], HEAD_DIM, pool[0], pool[2], table[1], pool[2] // scale[2], _DTYPES[dt],
+        _stream_of(dev)))
+
+
+def _check_prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens,
+                        free_pages, free_count, free_left, counters, page_size) -> None:
+    _check_tensor(cached_lens, "cached_lens", torch.int32, 1)
+    _check_tensor(new_lens, "new_lens", torch.int32, 1)
+    _check_tensor(block_table, "block_table", torch.int32, 2)
+    _check_tensor(slots, "slots", torch.int32, 1)
+    _check_tensor(cu_seqlens, "cu_seqlens", torch.int32, 1)
+    _check_tensor(seq_lens, "seq_lens", torch.int32, 1)
+    b = block_table.size(0)
+    if cached_lens.size(0) != b or new_lens.size(0) != b or seq_lens.size(0) != b:
+        raise RuntimeError("cached_lens / new_lens / seq_lens batch mismatch")
+    if cu_seqlens.size(0) != b + 1:
+        raise RuntimeError("cu_seqlens must hold B + 1 values")
+    _positive(page_size, "page_size")
+    if free_pages is not None:
+        _check_tensor(free_pages, "free_pages", torch.int32, 1)
+        if free_count is None or free_left is None or counters is None:
+            raise RuntimeError("a free-page list needs free_count, free_left and counters")
+        for name, t in (("free_count", free_count), ("free_left", free_left),
+                        ("counters", counters)):
+            _check_tensor(t, name, torch.int32, 1)
+            if t.size(0) < 1:
+                raise RuntimeError(f"{name} must hold one value")
+    _check_current_device(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens,
+                          free_pages, free_count, free_left, counters)
 
 
 def prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens, free_pages,
@@ -659,41 +730,43 @@ def prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens
     ``free_pages`` None every page is in ``block_table`` already.  See
     ``pkv_prompt_slots`` for the rows that are not served.  No counterpart in
     the reference."""
-    _check_tensor(cached_lens, "cached_lens", torch.int32, 1)
-    _check_tensor(new_lens, "new_lens", torch.int32, 1)
-    _check_tensor(block_table, "block_table", torch.int32, 2)
-    _check_tensor(slots, "slots", torch.int32, 1)
-    _check_tensor(cu_seqlens, "cu_seqlens", torch.int32, 1)
-    _check_tensor(seq_lens, "seq_lens", torch.int32, 1)
-    b, max_pages = block_table.shape
-    if cached_lens.size(0) != b or new_lens.size(0) != b or seq_lens.size(0) != b:
-        raise RuntimeError("cached_lens / new_lens / seq_lens batch mismatch")
-    if cu_seqlens.size(0) != b + 1:
-        raise RuntimeError("cu_seqlens must hold B + 1 values")
-    _positive(page_size, "page_size")
+    i32, dev, table, n = torch.int32, cached_lens.get_device(), block_table.shape, slots.shape
+    rows = cached_lens.shape
+    if not (
+        dev >= 0 and cached_lens.dtype is i32 and new_lens.dtype is i32
+        and block_table.dtype is i32 and slots.dtype is i32 and cu_seqlens.dtype is i32
+        and seq_lens.dtype is i32 and len(rows) == 1 and len(table) == 2 and len(n) == 1
+        and table[0] == rows[0] and new_lens.shape == rows and seq_lens.shape == rows
+        and cu_seqlens.shape == (rows[0] + 1,) and page_size > 0
+        and cached_lens.is_contiguous() and new_lens.is_contiguous()
+        and block_table.is_contiguous() and slots.is_contiguous() and cu_seqlens.is_contiguous()
+        and seq_lens.is_contiguous() and new_lens.get_device() == dev
+        and block_table.get_device() == dev and slots.get_device() == dev
+        and cu_seqlens.get_device() == dev and seq_lens.get_device() == dev
+        and torch.cuda.current_device() == dev
+        and (free_pages is None or (
+            free_count is not None and free_left is not None and counters is not None
+            and free_pages.dtype is i32 and free_count.dtype is i32 and free_left.dtype is i32
+            and counters.dtype is i32 and free_pages.dim() == 1 and free_count.shape == (1,)
+            and free_left.shape == (1,) and counters.shape == (1,) and free_pages.is_contiguous()
+            and free_pages.get_device() == dev and free_count.get_device() == dev
+            and free_left.get_device() == dev and counters.get_device() == dev))
+    ):
+        _check_prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens,
+                            free_pages, free_count, free_left, counters, page_size)
     fp = fc = fl = ctr = None
     capacity = 0
     if free_pages is not None:
-        _check_tensor(free_pages, "free_pages", torch.int32, 1)
-        if free_count is None or free_left is None or counters is None:
-            raise RuntimeError("a free-page list needs free_count, free_left and counters")
-        for name, t in (("free_count", free_count), ("free_left", free_left),
-                        ("counters", counters)):
-            _check_tensor(t, name, torch.int32, 1)
-            if t.size(0) < 1:
-                raise RuntimeError(f"{name} must hold one value")
         fp, fc = free_pages.data_ptr(), free_count.data_ptr()
         fl, ctr = free_left.data_ptr(), counters.data_ptr()
-        capacity = free_pages.size(0)
-    _check_current_device(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens,
-                          free_pages, free_count, free_left, counters)
+        capacity = free_pages.numel()
     _native.check(_native.load().pkv_prompt_slots(
         cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), slots.data_ptr(),
-        cu_seqlens.data_ptr(), seq_lens.data_ptr(), fp, fc, fl, ctr, b, max_pages,
-        int(page_size), slots.size(0), capacity, _stream()))
+        cu_seqlens.data_ptr(), seq_lens.data_ptr(), fp, fc, fl, ctr, table[0], table[1],
+        int(page_size), n[0], capacity, _stream_of(dev)))
 
 
-def _check_write(k, v, k_pages, v_pages, slots, pool_dtype):
+def _check_write(k, v, k_pages, v_pages, slots, pool_dtype) -> None:
     _check_packed(k, "k", tuple(_DTYPES))
     _check_packed(v, "v", k.dtype)
     _check_tensor(k_pages, "k_pages", pool_dtype, 4)
@@ -711,12 +784,24 @@ def kv_write(k, v, k_pages, v_pages, slots) -> None:
     """Writes packed tokens ``k`` / ``v`` [T, Hkv, 128] into 16-bit pools of their
     dtype at ``slots`` [T] (page * page_size + offset; negative skips a token).
     No counterpart in the reference."""
-    _check_write(k, v, k_pages, v_pages, slots, k.dtype)
-    _check_current_device(k, v, k_pages, v_pages, slots)
+    dt, ks, pool, dev = k.dtype, k.shape, k_pages.shape, k.get_device()
+    kst, vst = k.stride(), v.stride()
+    if not (
+        dev >= 0 and dt in _DTYPES and v.dtype is dt and k_pages.dtype is dt
+        and v_pages.dtype is dt and slots.dtype is torch.int32 and len(ks) == 3 and len(pool) == 4
+        and v.shape == ks and v_pages.shape == pool and slots.shape == ks[:1]
+        and pool[1] == ks[1] and ks[2] == HEAD_DIM and pool[3] == HEAD_DIM and kst[2] == 1
+        and vst[2] == 1 and k_pages.is_contiguous() and v_pages.is_contiguous()
+        and slots.is_contiguous() and v.get_device() == dev and k_pages.get_device() == dev
+        and v_pages.get_device() == dev and slots.get_device() == dev
+        and torch.cuda.current_device() == dev
+    ):
+        _check_write(k, v, k_pages, v_pages, slots, dt)
+        _check_current_device(k, v, k_pages, v_pages, slots)
     _native.check(_native.load().pkv_kv_write(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(),
-        k.size(0), k.size(1), HEAD_DIM, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        k_pages.size(0), k_pages.size(2), _DTYPES[k.dtype], _stream()))
+        ks[0], ks[1], HEAD_DIM, kst[0], kst[1], vst[0], vst[1], pool[0], pool[2], _DTYPES[dt],
+        _stream_of(dev)))
 
 
 def kv_write_fp8_block(k, v, k_pages, v_pages, k_scales, v_scales, slots) -> None:
@@ -725,14 +810,53 @@ def kv_write_fp8_block(k, v, k_pages, v_pages, k_scales, v_scales, slots) -> Non
     touches gets the least power of two that holds its new tokens, and its
     earlier tokens if the call starts inside it.  The tokens of one block must
     be consecutive and in slot order.  No counterpart in the reference."""
-    _check_write(k, v, k_pages, v_pages, slots, torch.float8_e4m3fn)
-    block = _check_block_scales(k_pages, k_scales, v_scales)
-    _check_current_device(k, v, k_pages, v_pages, k_scales, v_scales, slots)
+    dt, ks, pool, dev = k.dtype, k.shape, k_pages.shape, k.get_device()
+    kst, vst, scale, f8 = k.stride(), v.stride(), k_scales.shape, torch.float8_e4m3fn
+    if not (
+        dev >= 0 and dt in _DTYPES and v.dtype is dt and k_pages.dtype is f8
+        and v_pages.dtype is f8 and slots.dtype is torch.int32 and len(ks) == 3 and len(pool) == 4
+        and k_scales.dtype is torch.float32 and v_scales.dtype is torch.float32
+        and len(scale) == 3 and v_scales.shape == scale and scale[:2] == pool[:2] and scale[2] > 0
+        and pool[2] % (16 * scale[2]) == 0
+        and v.shape == ks and v_pages.shape == pool and slots.shape == ks[:1]
+        and pool[1] == ks[1] and ks[2] == HEAD_DIM and pool[3] == HEAD_DIM and kst[2] == 1
+        and vst[2] == 1 and k_pages.is_contiguous() and v_pages.is_contiguous()
+        and k_scales.is_contiguous() and v_scales.is_contiguous() and slots.is_contiguous()
+        and v.get_device() == dev and k_pages.get_device() == dev and v_pages.get_device() == dev
+        and k_scales.get_device() == dev and v_scales.get_device() == dev
+        and slots.get_device() == dev and torch.cuda.current_device() == dev
+    ):
+        _check_write(k, v, k_pages, v_pages, slots, f8)
+        _check_block_scales(k_pages, k_scales, v_scales)
+        _check_current_device(k, v, k_pages, v_pages, k_scales, v_scales, slots)
     _native.check(_native.load().pkv_kv_write_fp8_block(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
-        v_scales.data_ptr(), slots.data_ptr(), k.size(0), k.size(1), HEAD_DIM, k.stride(0),
-        k.stride(1), v.stride(0), v.stride(1), k_pages.size(0), k_pages.size(2), block,
-        _DTYPES[k.dtype], _stream()))
+        v_scales.data_ptr(), slots.data_ptr(), ks[0], ks[1], HEAD_DIM, kst[0], kst[1], vst[0],
+        vst[1], pool[0], pool[2], pool[2] // scale[2], _DTYPES[dt], _stream_of(dev)))
+
+
+def _check_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse) -> None:
+    _check_packed(q, "q", tuple(_DTYPES))
+    _check_packed(k, "k", q.dtype)
+    _check_packed(v, "v", q.dtype)
+    _check_tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+    _check_tensor(output, "output", q.dtype, 3)
+    if v.shape != k.shape:
+        raise RuntimeError("v shape must match k")
+    if output.shape != q.shape:
+        raise RuntimeError("output shape must match q")
+    if cu_seqlens_q.size(0) < 1:
+        raise RuntimeError("cu_seqlens_q must hold B + 1 values")
+    if cu_seqlens_k is not None:
+        _check_tensor(cu_seqlens_k, "cu_seqlens_k", torch.int32, 1)
+        if cu_seqlens_k.size(0) != cu_seqlens_q.size(0):
+            raise RuntimeError("cu_seqlens_k batch mismatch")
+    if lse is not None:
+        _check_tensor(lse, "lse", torch.float32, 2)
+        if lse.size(0) != q.size(0) or lse.size(1) != q.size(1):
+            raise RuntimeError("lse must have shape [Tq, Hq]")
+    _check_supported_gqa(q.size(1), k.size(1))
+    _check_current_device(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse)
 
 
 def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse=None) -> None:
@@ -746,38 +870,29 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse=None) -> N
     (optional, float32 [Tq, Hq]) gets each row's log-sum-exp.  A row that sees
     no key gives zeros and -inf; rows of no sequence are left as they were.  No
     counterpart in the reference."""
-    _check_packed(q, "q", tuple(_DTYPES))
-    _check_packed(k, "k", q.dtype)
-    _check_packed(v, "v", q.dtype)
-    _check_tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
-    _check_tensor(output, "output", q.dtype, 3)
-    tq, hq, d = q.shape
-    tk, hkv, _ = k.shape
-    if v.shape != k.shape:
-        raise RuntimeError("v shape must match k")
-    if output.shape != q.shape:
-        raise RuntimeError("output shape must match q")
-    b = cu_seqlens_q.size(0) - 1
-    if b < 0:
-        raise RuntimeError("cu_seqlens_q must hold B + 1 values")
-    ck = None
-    if cu_seqlens_k is not None:
-        _check_tensor(cu_seqlens_k, "cu_seqlens_k", torch.int32, 1)
-        if cu_seqlens_k.size(0) != b + 1:
-            raise RuntimeError("cu_seqlens_k batch mismatch")
-        ck = cu_seqlens_k.data_ptr()
-    ls = None
-    if lse is not None:
-        _check_tensor(lse, "lse", torch.float32, 2)
-        if lse.size(0) != tq or lse.size(1) != hq:
-            raise RuntimeError("lse must have shape [Tq, Hq]")
-        ls = lse.data_ptr()
-    _check_supported_gqa(hq, hkv)
-    _check_current_device(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse)
+    dt, qs, ks, dev, cq = q.dtype, q.shape, k.shape, q.get_device(), cu_seqlens_q.shape
+    qst, kst, vst = q.stride(), k.stride(), v.stride()
+    if not (
+        dev >= 0 and dt in _DTYPES and k.dtype is dt and v.dtype is dt and output.dtype is dt
+        and cu_seqlens_q.dtype is torch.int32 and len(qs) == 3 and len(ks) == 3 and len(cq) == 1
+        and cq[0] > 0 and v.shape == ks and output.shape == qs and qs[2] == HEAD_DIM
+        and ks[2] == HEAD_DIM and ks[1] > 0 and qs[1] % ks[1] == 0
+        and qs[1] // ks[1] in _SUPPORTED_G and qst[2] == 1 and kst[2] == 1 and vst[2] == 1
+        and output.is_contiguous() and cu_seqlens_q.is_contiguous() and k.get_device() == dev
+        and v.get_device() == dev and output.get_device() == dev
+        and cu_seqlens_q.get_device() == dev and torch.cuda.current_device() == dev
+        and (cu_seqlens_k is None or (
+            cu_seqlens_k.dtype is torch.int32 and cu_seqlens_k.shape == cq
+            and cu_seqlens_k.is_contiguous() and cu_seqlens_k.get_device() == dev))
+        and (lse is None or (lse.dtype is torch.float32 and lse.shape == qs[:2]
+                             and lse.is_contiguous() and lse.get_device() == dev))
+    ):
+        _check_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse)
     _native.check(_native.load().pkv_prompt_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(), ck, output.data_ptr(),
-        ls, b, tq, tk, hq, hkv, d, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-        v.stride(0), v.stride(1), _DTYPES[q.dtype], _stream()))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(),
+        None if cu_seqlens_k is None else cu_seqlens_k.data_ptr(), output.data_ptr(),
+        None if lse is None else lse.data_ptr(), cq[0] - 1, qs[0], ks[0], qs[1], ks[1], HEAD_DIM,
+        qst[0], qst[1], kst[0], kst[1], vst[0], vst[1], _DTYPES[dt], _stream_of(dev)))
 
 
 def auto_workspace_bytes(batch: int, hq: int, hkv: int, sm_count: int = 0) -> int:

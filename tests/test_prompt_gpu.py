@@ -313,9 +313,14 @@ def test_slots_without_a_stack_and_with_bad_rows():
         assert np.array_equal(got.cpu().numpy(), w)
     d, left, code = run_slots([0], [20], np.zeros((1, 4)), 20, 16, free, 999)
     assert code == 0x10 and left == 18 and d["t"][0, :2].tolist() == [119, 118]
-    # fewer places than tokens; a page id that cannot be a slot
-    d, left, code = run_slots([0], [20], np.zeros((1, 4)), 12, 16, free, 20)
-    assert code == 0x8 and d["s"].tolist() == [119 * 16 + i for i in range(12)]
+    # fewer places than tokens: the row that does not fit is not served; a page id
+    # that cannot be a slot
+    cached, new = [0, 0, 3], [7, 20, 0]
+    d, left, code = run_slots(cached, new, np.zeros((3, 4)), 12, 16, free, 20)
+    want = pr.prompt_slots(cached, new, np.zeros((3, 4)), 12, 16, free, 20)
+    assert code == 0x8 and left == want[4] == 19 and want[5] == [1]
+    for got, w in zip((d["t"], d["s"], d["cu"], d["seq"]), want):
+        assert np.array_equal(got.cpu().numpy(), w)
     d, left, code = run_slots([0], [20], np.zeros((1, 4)), 20, 16, [-1, 3], 2)
     assert code == 0x4 >> 2 and d["s"].tolist() == [48 + i for i in range(16)] + [-1] * 4
 
