@@ -227,7 +227,7 @@ struct WriteParams {
     int split;  // warps that share a window of tokens (e4m3 write)
 };
 
-constexpr int kWriteThreads = 256;
+constexpr int kWriteThreads = 128;
 
 // One thread moves one 16-byte piece of a token's K and the same piece of its
 // V.  A copy: HBM-bound for long prompts.
@@ -317,7 +317,7 @@ constexpr int kRunRows = 16;  // tokens held in registers at a time
 // in flight, 4 KB a warp.  Bound: HBM for long prompts (reads 2 bytes, writes 1
 // per element), the chain slots -> tokens -> codes for short ones.
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads, 4)
+__global__ void __launch_bounds__(kWriteThreads, 8)
     pkv_kv_write_block_kernel(const __grid_constant__ WriteParams p) {
     const int lane = threadIdx.x & 31;
     const long long w = ((long long)blockIdx.x * kWriteThreads + threadIdx.x) >> 5;
@@ -342,6 +342,12 @@ __global__ void __launch_bounds__(kWriteThreads, 4)
     auto block_of = [&](int slot) -> int {
         return slot >= 0 && slot < p.num_slots ? slot / p.block : -1;
     };
+    if (lane >= 1 && lane <= kRunRows && t0 + lane - 1 < p.T) {
+        // the window's tokens come to L2 while their slots are looked up
+        const uint8_t* row = src + (t0 + lane - 1) * tok_stride;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(row));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(row + 128));
+    }
     const int slot = slot_of(t0 + lane - 1);
     if (slot >= p.num_slots && r == 0) raise_error(p.error, kErrSlot);
     const int blk = block_of(slot);

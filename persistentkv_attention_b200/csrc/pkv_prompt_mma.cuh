@@ -17,7 +17,9 @@ constexpr int kPmSoftmaxWarps = 8;
 constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10;
 constexpr int kPmThreads = 384;
 constexpr int kPmParts = 4;  // parts of a block's weights, 32 keys each, handed over one by one
-constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes + 512;
+constexpr int kPmStageOut = 32 * 64;  // a softmax warp's 32 rows x 32 output dims
+constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes +
+                                kPmSoftmaxWarps * kPmStageOut + 512;
 // TMEM columns: scores of tile t at 128 t (its weights, 16 bit, in the first
 // 64 of them), output of tile t at 256 + 128 t.
 constexpr uint32_t kPmTmemColumns = 512;  // all there are
@@ -192,7 +194,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* s_q = smem;                      // 2 tiles
     uint8_t* s_kv = smem + 2 * kPmTileBytes;  // kPmStages tiles
-    PmShared* sh = reinterpret_cast<PmShared*>(s_kv + kPmStages * kPmTileBytes);
+    uint8_t* s_out = s_kv + kPmStages * kPmTileBytes;
+    PmShared* sh = reinterpret_cast<PmShared*>(s_out + kPmSoftmaxWarps * kPmStageOut);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -573,10 +576,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
             }
-            const size_t at = (size_t)(it.q0 + min(qrow, it.lq - 1)) * p.Hq + head;
-            T* out = reinterpret_cast<T*>(p.out) + at * kHeadDim;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float worst = 0.f;  // NaN if any value is not finite
+            // Through shared memory, 32 dims at a time, so that a warp stores 64
+            // bytes of 8 rows at once: a thread writing its own row touches 32
+            // lines an instruction, and the stores took longer than a block.
+            // 16-byte piece i of row r stands at i ^ (r / 2): no bank conflicts.
+            uint8_t* stage = s_out + warp * kPmStageOut;
+            const int srow = lane >> 2, spiece = lane & 3;  // row of 8 and piece it stores
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -595,24 +602,36 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) worst = fmaf(__uint_as_float(o[i]), 0.f, worst);
-                if (real) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 u;
-                        u.x = ElemOps<T>::pack(__uint_as_float(o[8 * i]) * inv,
-                                               __uint_as_float(o[8 * i + 1]) * inv);
-                        u.y = ElemOps<T>::pack(__uint_as_float(o[8 * i + 2]) * inv,
-                                               __uint_as_float(o[8 * i + 3]) * inv);
-                        u.z = ElemOps<T>::pack(__uint_as_float(o[8 * i + 4]) * inv,
-                                               __uint_as_float(o[8 * i + 5]) * inv);
-                        u.w = ElemOps<T>::pack(__uint_as_float(o[8 * i + 6]) * inv,
-                                               __uint_as_float(o[8 * i + 7]) * inv);
-                        reinterpret_cast<uint4*>(out)[4 * c + i] = u;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    uint4 u;
+                    u.x = ElemOps<T>::pack(__uint_as_float(o[8 * i]) * inv,
+                                           __uint_as_float(o[8 * i + 1]) * inv);
+                    u.y = ElemOps<T>::pack(__uint_as_float(o[8 * i + 2]) * inv,
+                                           __uint_as_float(o[8 * i + 3]) * inv);
+                    u.z = ElemOps<T>::pack(__uint_as_float(o[8 * i + 4]) * inv,
+                                           __uint_as_float(o[8 * i + 5]) * inv);
+                    u.w = ElemOps<T>::pack(__uint_as_float(o[8 * i + 6]) * inv,
+                                           __uint_as_float(o[8 * i + 7]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = u;
                 }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 8 * k + srow;  // of the warp
+                    const uint4 u = *reinterpret_cast<const uint4*>(
+                        stage + row * 64 + ((spiece ^ ((row >> 1) & 3)) << 4));
+                    const int seq_row = qrow - lane + row;
+                    if (seq_row < it.lq)
+                        reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
+                                                 ((size_t)(it.q0 + seq_row) * p.Hq + head) *
+                                                     kHeadDim)[4 * c + spiece] = u;
+                }
+                __syncwarp();
             }
             if (real && p.lse != nullptr)
-                p.lse[at] = l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
+                p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
+                    l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
             // A value that is not finite may come from a key the row does not see
             // (weight 0 times an infinite or NaN V): such a row is computed again
             // from its own keys alone.
