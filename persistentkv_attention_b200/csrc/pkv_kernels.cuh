@@ -767,7 +767,7 @@ __device__ __forceinline__ bool plan_init(const DecodeParams& p, int lane, AutoC
     const int row = word(4), row_end = word(5), P = word(6), O = word(7);
     const long long limit = (long long)p.max_pages * p.page_size;
     const bool ok = word(0) == kPlanMagic && word(1) == p.auto_groups && word(2) == p.B && T >= 0 &&
-                    row < p.B && row_end <= p.B && (row < 0 || (row_end > row && P >= 0 && O >= 0));
+                    row < p.B && row_end <= p.B && (row < 0 || (row_end >= row && P >= 0 && O >= 0));
     if (!ok) {
         if (report) raise_error(p.error, kErrWorkItem);
         return false;
@@ -778,11 +778,13 @@ __device__ __forceinline__ bool plan_init(const DecodeParams& p, int lane, AutoC
     c.kvh = (int)blockIdx.x % p.Hkv;
     c.T = T;
     c.sd.init(T, c.NG);
-    c.b = row;
-    c.b_end = row < 0 ? row : row_end;
+    // with more groups than tiles a group may hold no row piece (row_end == row)
+    const bool none = row < 0 || row_end == row;
+    c.b = none ? -1 : row;
+    c.b_end = none ? -1 : row_end;
     c.P = P;
     c.O = O;
-    if (row < 0) return true;
+    if (none) return true;
     int seq = word(8);
     seq = seq < 0 ? 0 : ((long long)seq > limit ? (int)limit : seq);
     const int n = (seq + kTileTokens - 1) / kTileTokens;
