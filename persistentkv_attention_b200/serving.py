@@ -72,6 +72,23 @@ class HostPlan:
 
 
 @dataclass
+class PageStack:
+    """Free pages of a pool on the device, as ``ops.prompt_slots`` and
+    ``ops.kv_append`` take them: the top is ``free_pages[free_count - 1]``."""
+
+    free_pages: torch.Tensor   # int32 [capacity]
+    free_count: torch.Tensor   # int32 [1]
+    counters: torch.Tensor     # int32 [1], zero between calls
+
+    @classmethod
+    def full(cls, pages: int, device) -> "PageStack":
+        """Every page of a pool, page 0 on top."""
+        i32 = dict(dtype=torch.int32, device=device)
+        return cls(torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32),
+                   torch.zeros(1, **i32))
+
+
+@dataclass
 class StepPlan:
     """Device-resident metadata of one decode step."""
 
@@ -95,9 +112,14 @@ class DecodeEngine:
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, hq: int,
                  router: Router | None = None, policy: str = "device", fused: bool = True,
                  requested_splits: int = 0, kv_scales: tuple[float, float] | None = None,
-                 use_plan: bool = True, groups: int | str = "router"):
+                 use_plan: bool = True, groups: int | str = "router",
+                 kv_block_scales: tuple[torch.Tensor, torch.Tensor] | None = None,
+                 q_dtype: torch.dtype = torch.float16):
         """``kv_scales`` = (k_scale, v_scale) for ``torch.float8_e4m3fn`` pools
-        (q and output are then fp16; device schedule only).  ``use_plan``: with
+        (q and output are then fp16; device schedule only), or
+        ``kv_block_scales`` = (k_scales, v_scales), float32 [P, Hkv, page_size /
+        block], for e4m3 pools with a scale per block of tokens and head
+        (``q_dtype``: that of q and the output, fp16 or bf16).  ``use_plan``: with
         the device schedule, each step carries a host plan of the schedule
         (``scheduler.build_auto_plan``) uploaded with its other metadata.
         ``groups``: the device schedule's group count -- "router" (default) the
@@ -110,9 +132,15 @@ class DecodeEngine:
         self.page_size = k_pages.shape[2]
         self.kv8 = k_pages.dtype == torch.float8_e4m3fn
         self.dtype = torch.float16 if self.kv8 else k_pages.dtype
-        if self.kv8 and (kv_scales is None or policy != "device"):
-            raise RuntimeError("an e4m3 K/V cache needs kv_scales and the device schedule")
+        if self.kv8 and ((kv_scales is None) == (kv_block_scales is None) or policy != "device"):
+            raise RuntimeError("an e4m3 K/V cache needs kv_scales or kv_block_scales, and the "
+                               "device schedule")
+        if kv_block_scales is not None:
+            if not self.kv8:
+                raise RuntimeError("kv_block_scales belong to an e4m3 K/V cache")
+            self.dtype = q_dtype
         self.kv_scales = kv_scales
+        self.kv_block_scales = kv_block_scales
         self.device = k_pages.device
         if router is None:
             sms = torch.cuda.get_device_properties(self.device).multi_processor_count
@@ -216,6 +244,12 @@ class DecodeEngine:
     def run(self, plan: StepPlan, q_source: torch.Tensor, out: torch.Tensor) -> None:
         f = plan.fields
         counters = self._counters[: plan.batch * self.hkv].view(plan.batch, self.hkv)
+        if self.kv_block_scales is not None:
+            ops.paged_attention_auto_fp8_block(
+                q_source, self.k_pages, self.v_pages, *self.kv_block_scales, f["block_table"],
+                f["seq_lens"], out, self._workspace, f["q_indices"], f["out_indices"],
+                counters if self.fused else None)
+            return
         if self.kv8:
             ops.paged_attention_auto_fp8(
                 q_source, self.k_pages, self.v_pages, self.kv_scales[0], self.kv_scales[1],
@@ -232,6 +266,36 @@ class DecodeEngine:
             q_source, self.k_pages, self.v_pages, f["block_table"], f["seq_lens"],
             f["work_items"], f["split_offsets"], counters, f["q_indices"], f["out_indices"], out,
             self._workspace, plan.host.bucket, self.page_size, plan.host.total_slots, self.fused)
+
+    def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, new_lens: torch.Tensor,
+                block_table: torch.Tensor, out: torch.Tensor, stack: "PageStack | None" = None,
+                lse: torch.Tensor | None = None) -> torch.Tensor:
+        """A batch of whole prompts: their pages, their K/V into the cache and
+        their attention, all on the GPU; returns the rows' lengths (int32 [B]).
+
+        ``q`` [T, Hq, 128] and ``k`` / ``v`` [T, Hkv, 128] hold the prompts' tokens
+        one row after another, ``new_lens`` (int32 [B], device) their lengths; T
+        may exceed their sum (padding).  Pages come from ``stack`` into
+        ``block_table`` [B, max_pages], or are in it already (None).  ``out`` gets
+        the attention of each row over its own tokens, computed from the packed
+        16-bit K/V.  A row that finds no pages (length 0 in the result) keeps
+        none of its K/V."""
+        b = block_table.size(0)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        slots, cu = torch.empty(k.size(0), **i32), torch.empty(b + 1, **i32)
+        seq_lens = torch.empty(b, **i32)
+        ops.prompt_slots(torch.zeros(b, **i32), new_lens, block_table, slots, cu, seq_lens,
+                         *((None,) * 4 if stack is None else
+                           (stack.free_pages, stack.free_count, stack.free_count, stack.counters)),
+                         self.page_size)
+        if self.kv_block_scales is not None:
+            ops.kv_write_fp8_block(k, v, self.k_pages, self.v_pages, *self.kv_block_scales, slots)
+        elif self.kv8:
+            raise RuntimeError("prefill writes 16-bit caches and e4m3 caches with block scales")
+        else:
+            ops.kv_write(k, v, self.k_pages, self.v_pages, slots)
+        ops.prompt_attention(q, k, v, cu, None, out, lse=lse)
+        return seq_lens
 
     def run_state(self, plan: StepPlan, q_source: torch.Tensor, state_out: torch.Tensor) -> None:
         """One decode of this GPU's pages into the (m, l, acc) state [B, Hq, 130]."""

@@ -16,6 +16,7 @@ import torch
 
 from oracle import prompt_oracle as pr
 from persistentkv_attention_b200 import _native, ops
+from persistentkv_attention_b200.serving import DecodeEngine, PageStack
 
 pytestmark = pytest.mark.gpu
 
@@ -688,3 +689,62 @@ def test_prompt_then_decode_over_one_cache(dtype):
                 off = np.abs(got - hk.double().numpy())
                 assert (off <= 2.0 ** -4 * np.abs(hk.double().numpy()) + 2.0 ** -9).all()
     no_error()
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "block-f16", "block-bf16"])
+def test_engine_prefill_then_steps(cache):
+    """The engine's own path: prompts through ``prefill``, then decode steps over
+    what it wrote, for 16-bit caches and e4m3 ones with block scales."""
+    dtype = cache.rsplit("-")[-1]
+    hq, hkv, page, pool, width = 16, 4, 32, 40, 12
+    gen = torch.Generator().manual_seed(9)
+    new = lambda n, h: torch.randn(n, h, 128, generator=gen).to(DT[dtype])  # noqa: E731
+    if cache.startswith("block"):
+        kp, ks = empty_cache(pool, hkv, page, 16)
+        vp, vs = empty_cache(pool, hkv, page, 16)
+        engine = DecodeEngine(kp, vp, hq, kv_block_scales=(ks, vs), q_dtype=DT[dtype])
+    else:
+        kp = torch.zeros(pool, hkv, page, 128, dtype=DT[dtype], device="cuda")
+        vp = torch.zeros_like(kp)
+        engine = DecodeEngine(kp, vp, hq)
+    stack = PageStack.full(pool, "cuda")
+    lens = [130, 1, 300, 0]
+    total, pad = sum(lens), 9
+    q, k, v = new(total + pad, hq), new(total + pad, hkv), new(total + pad, hkv)
+    table = torch.zeros(4, width, dtype=torch.int32, device="cuda")
+    out = torch.full((total + pad, hq, 128), 7.0, dtype=DT[dtype], device="cuda")
+    lse = torch.full((total + pad, hq), 7.0, device="cuda")
+    seq = engine.prefill(q.cuda(), k.cuda(), v.cuda(), i32(lens), table, out, stack, lse)
+    no_error()
+    assert seq.tolist() == lens and stack.free_count.item() == pool - 5 - 1 - 10
+    cu = np.cumsum([0] + lens)
+    check_prompt(q, k, v, cu, cu, dtype, out, lse)
+    plan = engine.upload(engine.plan_step(lens, table.cpu().numpy()))
+    dq = new(4, hq)
+    step = torch.zeros(4, hq, 128, dtype=DT[dtype], device="cuda")
+    engine.run(plan, dq.cuda(), step)
+    no_error()
+    t = table.cpu().numpy()
+    if cache.startswith("block"):
+        check_decode(step, dq, kp, ks, vp, vs, t, lens, dtype)
+    else:
+        one = np.ones((pool, hkv, 1))
+        want, mag, size, _ = pr.paged_decode(dq.double().numpy(), kp.double().cpu().numpy(),
+                                             vp.double().cpu().numpy(), one, t, lens)
+        check_close(step, want, mag, size, 1e3, dtype)
+
+
+def test_engine_refuses_caches_it_cannot_fill():
+    p8, s8 = empty_cache(4, 2, 16, 16)
+    p16 = torch.zeros(4, 2, 16, 128, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="kv_scales or kv_block_scales"):
+        DecodeEngine(p8, p8, 4)
+    with pytest.raises(RuntimeError, match="kv_scales or kv_block_scales"):
+        DecodeEngine(p8, p8, 4, kv_scales=(1.0, 1.0), kv_block_scales=(s8, s8))
+    with pytest.raises(RuntimeError, match="belong to an e4m3"):
+        DecodeEngine(p16, p16, 4, kv_block_scales=(s8, s8))
+    x = torch.zeros(3, 2, 128, dtype=torch.float16, device="cuda")
+    q = torch.zeros(3, 4, 128, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="prefill writes"):
+        DecodeEngine(p8, p8, 4, kv_scales=(1.0, 1.0)).prefill(
+            q, x, x, i32([3]), i32([[0]]), torch.empty_like(q))
