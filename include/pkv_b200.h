@@ -303,7 +303,7 @@ pkv_status pkv_paged_attention_auto_fp8(
  * K = k_scales[p][h][t / block_tokens] * value, V likewise; scales are
  * [P][Hkv][page_size / block_tokens], block_tokens a multiple of 16 that
  * divides page_size.  A scale is positive and finite, or zero for a block of
- * zeros.  q and output are fp16 or bf16 (dtype).  Pages and scales of tokens
+ * zeros; a V scale below 2^-60 counts as 2^-60.  q and output are fp16 or bf16 (dtype).  Pages and scales of tokens
  * past a row's length are never used, whatever they hold.  No counterpart in
  * the reference. */
 pkv_status pkv_paged_attention_auto_fp8_block(
@@ -356,7 +356,8 @@ pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
  * strides (elements, multiples of 8), into 16-bit pools: token t of head h
  * goes to slot slots[t] = page * page_size + offset.  A negative slot skips
  * its token; one beyond the pool skips it and sets PKV_DEVERR_SLOT.  Of two
- * tokens with one slot either may stay. */
+ * tokens with one slot either may stay.  The pools and the tokens must not
+ * overlap. */
 pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pages,
                         const int32_t* slots, int T, int Hkv, int head_dim, long long k_stride,
                         long long k_head_stride, long long v_stride, long long v_head_stride,
@@ -384,12 +385,14 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
  * sees its last key, so row i of lq sees the keys j <= i + lk - lq of lk, and a
  * row that sees none gives zeros.  q [q_tokens][Hq][128], k / v
  * [k_tokens][Hkv][128] with the given strides (elements, multiples of 8),
- * output [q_tokens][Hq][128] contiguous; softmax scale 1 / sqrt(128).  lse
+ * output [q_tokens][Hq][128] contiguous, apart from the inputs; softmax scale
+ * 1 / sqrt(128).  lse
  * (or NULL): [q_tokens][Hq] natural log of each row's sum of exponentials,
  * -inf for a row that sees no key.  Rows of no sequence are left as they
  * were, and a row's result depends on no key that it does not see, whatever
- * those hold.  A sequence whose ranges lie outside the tokens is skipped and
- * sets PKV_DEVERR_INDEX. */
+ * those hold.  A sequence whose ranges lie outside the tokens or run backwards
+ * is skipped and sets PKV_DEVERR_INDEX; the others' rows are computed only if
+ * every range is in order. */
 pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 void* output, float* lse, int B, int q_tokens, int k_tokens,

@@ -48,6 +48,9 @@ struct B8Lookups {
 // math falls behind HBM (64 rows up to 32768 tokens: 197 us, two threads 175 us).
 constexpr int kB8Threads = kThreads + 32;
 
+// V scales below this count as this.
+constexpr float kB8LeastScale = 0x1p-60f;
+
 template <int G, int NSLOTS>
 constexpr size_t block8_smem_bytes() {
     return decode_smem_bytes<G, NSLOTS>() + sizeof(B8Lookups);
@@ -573,9 +576,9 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
                 }
                 const float ks = i == 0 ? scales.x : scales.y;
                 const float vs = i == 0 ? scales.z : scales.w;
-                // a block of zeros (scale 0) still counts in the sum: its scale
-                // becomes 2^-100, far below any weight's contribution
-                const float lg = vs == 0.f ? -100.f : fast_log2(vs);
+                // a block of zeros (scale 0) still counts in the sum, as one of scale
+                // 2^-60: its weights stay 66 powers of two above fp32's least
+                const float lg = vs < kB8LeastScale ? -60.f : fast_log2(vs);
                 const float f0 = qs[0] * ks, f1 = qs[1] * ks;
                 if (ks == 0.f) c[0] = c[1] = c[2] = c[3] = 0.f;  // K = 0, whatever the codes
                 const bool ok0 = 16 * i + g8 < valid, ok1 = 16 * i + g8 + 8 < valid;
@@ -617,7 +620,7 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
                 const float vs = i == 0 ? scales.z : scales.w;
                 // (a masked block's scale may be anything: fmaxf drops a NaN, and a
                 // weight of 0 must not meet an infinity)
-                const float inv = 1.f / fmaxf(vs, 0x1p-100f);
+                const float inv = 1.f / fmaxf(vs, kB8LeastScale);
                 float pr[4];
                 pr[0] = fast_exp2(sc[i][0] - b0);
                 pr[1] = fast_exp2(sc[i][1] - b1);

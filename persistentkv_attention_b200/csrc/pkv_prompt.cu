@@ -84,6 +84,32 @@ pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_p
     return PKV_OK;
 }
 
+// The bytes of a [T][H][128] 16-bit operand, from its first element to its last.
+struct Range {
+    const char* begin;
+    long long bytes;
+};
+Range operand_range(const void* base, int T, int H, long long tok_bytes, long long head_bytes) {
+    return {static_cast<const char*>(base),
+            T > 0 ? (T - 1) * tok_bytes + (H - 1) * head_bytes + kRowBytes : 0};
+}
+bool overlap(const Range& a, const Range& b) {
+    return a.bytes > 0 && b.bytes > 0 && a.begin < b.begin + b.bytes && b.begin < a.begin + a.bytes;
+}
+
+// K and V go to pools of their own, apart from the tokens that are read.
+pkv_status check_apart(const WriteParams& wp, int physical_pages, int elem_bytes) {
+    const long long pool = (long long)physical_pages * wp.Hkv * wp.page_size * kHeadDim * elem_bytes;
+    const Range kp{reinterpret_cast<const char*>(wp.k_pages), pool};
+    const Range vp{reinterpret_cast<const char*>(wp.v_pages), pool};
+    const Range k = operand_range(wp.k, wp.T, wp.Hkv, wp.k_tok, wp.k_head);
+    const Range v = operand_range(wp.v, wp.T, wp.Hkv, wp.v_tok, wp.v_head);
+    if (overlap(kp, vp) || overlap(kp, k) || overlap(kp, v) || overlap(vp, k) || overlap(vp, v))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                        "k_pages, v_pages and the tokens written must not overlap");
+    return PKV_OK;
+}
+
 pkv_status grid_of(long long threads, int per_cta, unsigned* grid) {
     const long long n = (threads + per_cta - 1) / per_cta;
     if (n > INT_MAX) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many tokens for one launch");
@@ -204,6 +230,8 @@ pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pag
                                  page_size, dtype);
     if (st != PKV_OK) return st;
     if (T == 0) return ok();
+    st = check_apart(wp, physical_pages, 2);
+    if (st != PKV_OK) return st;
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
@@ -236,6 +264,10 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     wp.v_scales = v_scales;
     wp.block = block_tokens;
     if (T == 0) return ok();
+    st = check_apart(wp, physical_pages, 1);
+    if (st != PKV_OK) return st;
+    if (k_scales == v_scales)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must not overlap");
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
@@ -309,6 +341,11 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
     pp.Hq = Hq;
     pp.Hkv = Hkv;
     pp.scale_log2 = (1.0f / sqrtf((float)kHeadDim)) * kLog2e;
+    const Range o = operand_range(output, q_tokens, Hq, (long long)Hq * kRowBytes, kRowBytes);
+    if (overlap(o, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
+        overlap(o, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
+        overlap(o, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "output must not overlap q, k or v");
     int sms = 0;
     st = device_state(&sms, &pp.error);
     if (st != PKV_OK) return st;

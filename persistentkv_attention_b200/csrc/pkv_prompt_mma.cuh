@@ -12,9 +12,9 @@ constexpr int kPmTileBytes = kPmTile * kRowBytes;  // 32 KB: two 64-element halv
 constexpr int kPmHalfBytes = kPmTileBytes / 2;
 constexpr int kPmStages = 4;                     // K/V tiles in flight
 // 8 softmax warps (tile, 32 rows each), then one warp each for the products,
-// the copies and the schedule.
+// the copies and the schedule, and one that looks the ranges over.
 constexpr int kPmSoftmaxWarps = 8;
-constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10;
+constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10, kPmCheckWarp = 11;
 constexpr int kPmThreads = 384;
 constexpr int kPmParts = 4;  // parts of a block's weights, 32 keys each, handed over one by one
 constexpr int kPmStageOut = 32 * 64;  // a softmax warp's 32 rows x 32 output dims
@@ -238,8 +238,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             PmWork w;
             const int found = pm_find(p, item / groups, pm_rows_per_item(G), w);
             w.group = item % groups;
-            if (found < 0 && lane == 0) raise_error(p.error, kErrIndex);
-            if (found > 0) {
+            if (found > 0) {  // (a bad sequence is reported by the checking warp)
                 if (n >= (uint32_t)kPmWorks)
                     ok = pm_wait_warp(p, sh, &sh->work_empty[n % kPmWorks],
                                       (n / kPmWorks - 1) & 1u);
@@ -275,6 +274,17 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             mbar_arrive(&sh->work_full[n % kPmWorks]);
         }
         __syncwarp();
+    } else if (warp == kPmCheckWarp) {
+        // ------------------------------------------------------------ ranges
+        if (blockIdx.x == 0) {
+            bool bad = false;
+            for (int b = lane; b < p.B; b += 32) {
+                const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1);
+                const int k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
+                bad = bad || q0 < 0 || q1 < q0 || q1 > p.Tq || k0 < 0 || k1 < k0 || k1 > p.Tk;
+            }
+            if (bad) raise_error(p.error, kErrIndex);
+        }
     } else if (warp == kPmLoadWarp) {
         // ------------------------------------------------------------ copies
         if (lane == 0) {

@@ -107,6 +107,24 @@ def test_prompt_validation(lib, kw, status, msg):
     assert msg in lib.pkv_last_error_message().decode()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(), dict(vp=FAKE + (1 << 20), k=FAKE2), dict(kp=FAKE2, vp=FAKE + 4096),
+    dict(kp=FAKE - 4096, vp=FAKE2 + (1 << 24))])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_write_refuses_overlaps(lib, fp8, kw):
+    # pools of 2 MB (1 MB of e4m3), tokens of 8 KB at FAKE
+    assert write(lib, fp8, **kw) == 1
+    assert b"overlap" in lib.pkv_last_error_message()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(q=FAKE - 16, k=1 << 30, v=1 << 30), dict(q=1 << 30, k=FAKE + 1024, v=1 << 30),
+    dict(q=1 << 30, k=1 << 30, out=1 << 24, v=(1 << 24) - 80 * 1024 + 16)])
+def test_prompt_refuses_overlaps(lib, kw):
+    assert prompt(lib, **kw) == 1
+    assert b"output must not overlap" in lib.pkv_last_error_message()
+
+
 def test_nothing_to_do_is_no_error(lib):
     assert prompt(lib, B=0) == 0
     assert prompt(lib, q=None, out=None, Tq=0) == 0
