@@ -28,7 +28,9 @@ struct SlotsParams {
 };
 
 constexpr int kSlotThreads = 256;
-constexpr int kSlotTokensPerCta = 1024;
+// 256 rows, 400k tokens: 8.5 us (with 1024: 7.8, 2048: 10.0); 8 rows, 3k tokens:
+// 3.5 us (4.6, 6.9).
+constexpr int kSlotTokensPerCta = 512;
 
 // Sum over the CTA of one 64-bit value per thread, exclusive prefix returned,
 // total in `total`.  Both 32-bit halves are sums of non-negative values below
@@ -66,7 +68,7 @@ __device__ __forceinline__ unsigned long long slot_scan(unsigned long long v,
 // from the stack, never from block_table, where another CTA may still be
 // writing them.  A thread finds the places of its tokens first, then loads
 // their pages together.  Bound: the latency of the chain lengths -> pages ->
-// slots, three trips to L2 (256 rows, 400k tokens: XXX us against 0.3 us for its
+// slots, three trips to L2 (256 rows, 400k tokens: 8.5 us against 0.3 us for its
 // bytes).
 __global__ void __launch_bounds__(kSlotThreads)
     pkv_prompt_slots_kernel(const __grid_constant__ SlotsParams p) {
@@ -224,13 +226,14 @@ struct WriteParams {
     long long k_tok, k_head, v_tok, v_head;
     long long num_slots;  // P * page
     int T, Hkv, page_size, block;
-    int split;  // warps that share a window of tokens (e4m3 write)
+    int split_log2;  // warps that share a window of tokens (e4m3 write)
 };
 
 constexpr int kWriteThreads = 128;
 
 // One thread moves one 16-byte piece of a token's K and the same piece of its
-// V.  A copy: HBM-bound for long prompts.
+// V.  A copy: HBM-bound for long prompts (22.8k tokens of 8 heads, 187 MB: 31 us,
+// 6.0 TB/s), launch latency for short ones (37 tokens: 1.6 us).
 __global__ void __launch_bounds__(kWriteThreads)
     pkv_kv_write_kernel(const __grid_constant__ WriteParams p) {
     constexpr int kPieces = kRowBytes / 16;
@@ -299,6 +302,16 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// Four 16-bit values times a factor as e4m3 codes.
+template <typename T>
+__device__ __forceinline__ uint32_t e4m3x4(uint32_t lo, uint32_t hi, uint64_t factor2) {
+    const float2 a = to_float2<T>(lo), b = to_float2<T>(hi);
+    float ax, ay, bx, by;
+    unpack_f32x2(mul_f32x2(pack_f32x2(a.x, a.y), factor2), ax, ay);
+    unpack_f32x2(mul_f32x2(pack_f32x2(b.x, b.y), factor2), bx, by);
+    return __byte_perm(e4m3x2(ax, ay), e4m3x2(bx, by), 0x5410);
+}
+
 // Two e4m3 codes times a power of two, rounded back to e4m3.
 __device__ __forceinline__ uint32_t rescale_e4m3x2(uint32_t codes, float ratio) {
     const __half2_raw h =
@@ -309,25 +322,25 @@ __device__ __forceinline__ uint32_t rescale_e4m3x2(uint32_t codes, float ratio) 
 
 constexpr int kRunRows = 16;  // tokens held in registers at a time
 
-// A window of 16 tokens of one head's K or V belongs to `split` warps: the
+// A window of 16 tokens of one head's K or V belongs to 2^split_log2 warps: the
 // runs that start in it go to them in turn.  Long prompts start about one run
-// per window (split = 1); the new tokens of a decode step are a run each, and
+// per window (one warp); the new tokens of a decode step are a run each, and
 // one warp would take them one after another (64 rows: 27.9 us; with a warp
-// each 5.5 us).  Lane l holds 16 bytes (8 elements) of tokens l / 16 + 2 i: 8 loads
-// in flight, 4 KB a warp.  Bound: HBM for long prompts (reads 2 bytes, writes 1
-// per element), the chain slots -> tokens -> codes for short ones.
+// each 4.5 us).  Lane l holds 16 bytes (8 elements) of tokens l / 16 + 2 i: 8 loads
+// in flight, 4 KB a warp, 28 warps an SM (72 registers; at 24 or 32 warps it took
+// 39 and 32 us where this takes 29.6).  Bound: issue slots and HBM for long
+// prompts (2 bytes read, 1 written per element; 23k tokens of 8 heads, 143 MB:
+// 29.6 us, 4.8 TB/s), the chain slots -> tokens -> codes for short ones.
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads, 8)
+__global__ void __launch_bounds__(kWriteThreads, 7)
     pkv_kv_write_block_kernel(const __grid_constant__ WriteParams p) {
     const int lane = threadIdx.x & 31;
-    const long long w = ((long long)blockIdx.x * kWriteThreads + threadIdx.x) >> 5;
-    const int per_window = 2 * p.Hkv * p.split;
-    const long long window = w / per_window;
-    const long long t0 = window * kRunRows;
-    if (t0 >= p.T) return;
-    int r = (int)(w - window * per_window);
-    const int sub = r % p.split;
-    r /= p.split;
+    const long long t0 = (long long)blockIdx.x * kRunRows;
+    const int role = blockIdx.y * (kWriteThreads / 32) + (threadIdx.x >> 5);
+    if (role >= (2 * p.Hkv) << p.split_log2) return;
+    const int split = 1 << p.split_log2;
+    const int sub = role & (split - 1);
+    const int r = role >> p.split_log2;
     const int h = r >> 1;
     const bool is_v = (r & 1) != 0;
     const uint8_t* src = is_v ? p.v + h * p.v_head : p.k + h * p.k_head;
@@ -358,7 +371,7 @@ __global__ void __launch_bounds__(kWriteThreads, 8)
     for (int turn = 0; starts != 0u; ++turn) {
         const int sl = __ffs(starts) - 1;
         starts &= starts - 1;
-        if (turn % p.split != sub) continue;
+        if ((turn & (split - 1)) != sub) continue;
         const int run_blk = __shfl_sync(0xffffffffu, blk, sl);
         const int kept = __shfl_sync(0xffffffffu, slot, sl) - run_blk * p.block;
         const long long first = t0 + sl - 1;
@@ -382,13 +395,14 @@ __global__ void __launch_bounds__(kWriteThreads, 8)
         float old = 0.f;
         if (kept > 0) old = *scale_at;
         uint4 x[kRunRows / 2];
+        const uint8_t* from = src + (first + half) * tok_stride + 16 * piece;
         auto load = [&](int base) {
+            const uint8_t* at = from + base * tok_stride;
 #pragma unroll
             for (int i = 0; i < kRunRows / 2; ++i) {
-                const int row = base + half + 2 * i;
-                x[i] = row < n ? __ldg(reinterpret_cast<const uint4*>(src + (first + row) * tok_stride) +
-                                       piece)
-                               : make_uint4(0u, 0u, 0u, 0u);
+                x[i] = base + half + 2 * i < n ? __ldg(reinterpret_cast<const uint4*>(at))
+                                               : make_uint4(0u, 0u, 0u, 0u);
+                at += 2 * tok_stride;
             }
         };
         // the largest magnitude, two elements at a time on their bits
@@ -407,20 +421,18 @@ __global__ void __launch_bounds__(kWriteThreads, 8)
         if (top >= kInf16<T>) {
             // infinities and NaN do not set a scale: again without them
             top = 0u;
-            for (int base = 0; base < n; base += kRunRows) {
-                load(base);
+            for (int row = half; row < n; row += 2) {
+                const uint4 y = __ldg(reinterpret_cast<const uint4*>(from + (row - half) * tok_stride));
+                const unsigned u[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int i = 0; i < kRunRows / 2; ++i) {
-                    const unsigned u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const unsigned a = (u[j >> 1] >> (16 * (j & 1))) & 0x7fffu;
-                        if (a < kInf16<T>) top = max(top, a);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned lo = u[j] & 0x7fffu, hi = (u[j] >> 16) & 0x7fffu;
+                    if (lo < kInf16<T>) top = max(top, lo);
+                    if (hi < kInf16<T>) top = max(top, hi);
                 }
             }
+            __syncwarp();
             top = __reduce_max_sync(0xffffffffu, top);
-            if (n > kRunRows) load(0);
         }
         float scale = block_scale(from_bits16<T>(top));
         if (kept > 0) {
@@ -441,7 +453,7 @@ __global__ void __launch_bounds__(kWriteThreads, 8)
         __syncwarp();
         if (lane == 0) *scale_at = scale;
         // 1 / scale: exact for a power of two (an old scale may be any value)
-        const float inv = 1.0f / scale;
+        const uint64_t inv2 = pack_f32x2(1.0f / scale, 1.0f / scale);
         for (int base = 0; base < n; base += kRunRows) {
             if (n > kRunRows) load(base);
 #pragma unroll
@@ -450,13 +462,10 @@ __global__ void __launch_bounds__(kWriteThreads, 8)
                 const int near = __shfl_sync(0xffffffffu, slot, (sl + row) & 31);
                 if (row >= n) continue;
                 const int to = sl + row < 32 ? near : __ldg(p.slots + first + row);
-                const float2 a = to_float2<T>(x[i].x), b = to_float2<T>(x[i].y);
-                const float2 c = to_float2<T>(x[i].z), d = to_float2<T>(x[i].w);
-                uint2 out;
-                out.x = e4m3x2(a.x * inv, a.y * inv) | (e4m3x2(b.x * inv, b.y * inv) << 16);
-                out.y = e4m3x2(c.x * inv, c.y * inv) | (e4m3x2(d.x * inv, d.y * inv) << 16);
-                reinterpret_cast<uint2*>(block_base + (size_t)(to - run_blk * p.block) * kHeadDim)[piece] =
-                    out;
+                const uint2 out = make_uint2(e4m3x4<T>(x[i].x, x[i].y, inv2),
+                                             e4m3x4<T>(x[i].z, x[i].w, inv2));
+                *reinterpret_cast<uint2*>(block_base + (to - run_blk * p.block) * kHeadDim +
+                                          8 * piece) = out;
             }
         }
     }

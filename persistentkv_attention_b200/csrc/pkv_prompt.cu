@@ -80,7 +80,7 @@ pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_p
     wp.Hkv = Hkv;
     wp.page_size = page_size;
     wp.block = page_size;
-    wp.split = 1;
+    wp.split_log2 = 0;
     return PKV_OK;
 }
 
@@ -271,13 +271,16 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
-    unsigned grid = 0;
     // up to a warp per token while the card has room for them (32 warps an SM)
     const long long windows = ((long long)T + kRunRows - 1) / kRunRows;
-    wp.split = 1;
-    while (wp.split < kRunRows && windows * 2 * Hkv * wp.split * 2 <= 32ll * sms) wp.split *= 2;
-    st = grid_of(windows * 2 * Hkv * wp.split * 32, kWriteThreads, &grid);
-    if (st != PKV_OK) return st;
+    wp.split_log2 = 0;
+    while ((1 << wp.split_log2) < kRunRows &&
+           (windows * 2 * Hkv << (wp.split_log2 + 1)) <= 32ll * sms)
+        ++wp.split_log2;
+    const long long roles = (2ll * Hkv) << wp.split_log2;
+    const long long rows = (roles + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
+    if (rows > 65535) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many heads for one launch");
+    const dim3 grid((unsigned)windows, (unsigned)rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PKV_DTYPE_F16)
         pkv_kv_write_block_kernel<__half><<<grid, kWriteThreads, 0, s>>>(wp);

@@ -180,9 +180,10 @@ __device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uin
 // first keys arrive while the present one is computed, and its first scores
 // while the present one's output is written.
 //
-// Bound: the tensor cores (4 * 128 flops per query, key and head) under the
-// card's power cap, and next to it the 1 exponential per query and key of the
-// special-function units.
+// Bound: a tile's chain scores -> softmax -> output.  One prompt of 16384 tokens
+// (32 heads, bf16) takes 2.0 ms, 1.09 PFLOP/s, 3750 cycles per pair of tiles and
+// block at 1.67 GHz under the card's power cap; the products alone take 2580,
+// the exponentials 2050, and the tensor cores' nominal rate would be 2048.
 template <typename T>
 __global__ void __launch_bounds__(kPmThreads, 1)
     pkv_prompt_mma_kernel(const __grid_constant__ PromptParams p,
