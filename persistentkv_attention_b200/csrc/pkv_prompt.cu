@@ -39,6 +39,11 @@ pkv_status check_strides(const char* name, int T, int H, long long* tok, long lo
     return PKV_OK;
 }
 
+// Key blocks that a CTA of a split item gets at the least (prompt attention).  A
+// join costs about 8 us, a block 2: 16 queries over 8016 keys (32 heads) take
+// 114 us in one CTA per item and 47 in eight, 256 over 256 keys 12 and, in two, 21.
+constexpr int kPmSplitBlocks = 4;
+
 // Shared checks of the two writes; fills everything but the scales.
 pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_pages,
                         void* v_pages, const int32_t* slots, int T, int Hkv, int head_dim,
@@ -138,8 +143,27 @@ pkv_status token_map(CUtensorMap* map, const void* base, int T, int H, long long
     return PKV_OK;
 }
 
+// Shared-memory limit of a kernel, once per device.
+template <typename K>
+pkv_status set_smem(K kern, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPmSmemBytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail_fmt(PKV_ERR_CUDA, "cudaFuncSetAttribute failed: %s",
+                            cudaGetErrorString(e));
+        }
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    return PKV_OK;
+}
+
 template <typename T>
-pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, cudaStream_t stream) {
+pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, int sms, cudaStream_t stream) {
     CUtensorMap mq, mk, mv;
     pkv_status st = token_map(&mq, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
     // without keys no block is ever loaded: any valid map does
@@ -150,30 +174,50 @@ pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, cudaStream_t s
         st = pp.Tk > 0 ? token_map(&mv, pp.v, pp.Tk, pp.Hkv, pp.v_tok, pp.v_head, dtype)
                        : token_map(&mv, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
     if (st != PKV_OK) return st;
-    auto kern = pkv_prompt_mma_kernel<T>;
-    static std::atomic<unsigned long long> attr_done{0ull};  // devices already set up
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(attr_done.load(std::memory_order_acquire) & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(
-            kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPmSmemBytes);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return fail_fmt(PKV_ERR_CUDA, "cudaFuncSetAttribute failed: %s",
-                            cudaGetErrorString(e));
-        }
-        attr_done.fetch_or(bit, std::memory_order_acq_rel);
-    }
     const int G = pp.Hq / pp.Hkv;
     const int rows = G == 1 ? 2 * kPmTile : kPmTile;
     // every sequence has at most one tile that is not full
     const long long tiles = std::min<long long>((long long)pp.Tq / rows + pp.B, pp.Tq);
+    const long long items = tiles * (G == 1 ? pp.Hq : pp.Hq / 2);
+    // A cluster per item where that still leaves SMs free and each CTA gets
+    // at least kPmSplitBlocks key blocks of an average sequence.
+    int split = 1;
+    while (split < 8 && items * split * 2 <= sms &&
+           (long long)pp.Tk / pp.B >= (long long)kPmTile * kPmSplitBlocks * split * 2)
+        split *= 2;
     unsigned grid = 0;
-    st = grid_of(tiles * (G == 1 ? pp.Hq : pp.Hq / 2), 1, &grid);
+    st = grid_of(items * split, 1, &grid);
     if (st != PKV_OK) return st;
-    kern<<<grid, kPmThreads, kPmSmemBytes, stream>>>(pp, mq, mk, mv);
-    return launched("prompt attention");
+    if (split == 1) {
+        static std::atomic<unsigned long long> done{0ull};
+        auto kern = pkv_prompt_mma_kernel<T, false>;
+        st = set_smem(kern, done);
+        if (st != PKV_OK) return st;
+        kern<<<grid, kPmThreads, kPmSmemBytes, stream>>>(pp, mq, mk, mv);
+        return launched("prompt attention");
+    }
+    static std::atomic<unsigned long long> done{0ull};
+    auto kern = pkv_prompt_mma_kernel<T, true>;
+    st = set_smem(kern, done);
+    if (st != PKV_OK) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kPmThreads);
+    cfg.dynamicSmemBytes = kPmSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, pp, mq, mk, mv);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail_fmt(PKV_ERR_CUDA, "prompt attention launch failed: %s", cudaGetErrorString(e));
+    }
+    return ok();
 }
 
 }  // namespace
@@ -353,8 +397,8 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
     st = device_state(&sms, &pp.error);
     if (st != PKV_OK) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return dtype == PKV_DTYPE_F16 ? launch_prompt<__half>(pp, dtype, s)
-                                  : launch_prompt<__nv_bfloat16>(pp, dtype, s);
+    return dtype == PKV_DTYPE_F16 ? launch_prompt<__half>(pp, dtype, sms, s)
+                                  : launch_prompt<__nv_bfloat16>(pp, dtype, sms, s);
 }
 
 }  // extern "C"

@@ -55,7 +55,9 @@ static_assert(sizeof(PmShared) <= 512, "prompt CTA's shared state");
 
 // What follows from an item for every role.
 struct PmItem {
-    int q0, k0, lq, lk, row0, head0, kvh, n_tiles, n_blocks, tail, G;
+    int q0, k0, lq, lk, row0, head0, kvh, n_tiles, G;
+    int first, n_blocks;  // this CTA's key blocks
+    int tail;             // keys of the last of them
     // keys that row i of the sequence sees
     __device__ __forceinline__ int visible(int i) const {
         return max(0, min(lk, i + 1 + lk - lq));
@@ -64,6 +66,8 @@ struct PmItem {
 
 __device__ __forceinline__ int pm_rows_per_item(int G) { return G == 1 ? 2 * kPmTile : kPmTile; }
 
+// kSplit: the CTAs of a cluster share the item, its key blocks in equal parts.
+template <bool kSplit>
 __device__ __forceinline__ PmItem pm_item(const PromptParams& p, const PmWork& w) {
     PmItem it;
     it.G = p.Hq / p.Hkv;
@@ -76,8 +80,15 @@ __device__ __forceinline__ PmItem pm_item(const PromptParams& p, const PmWork& w
     it.kvh = it.head0 / it.G;
     it.n_tiles = (it.G == 1 && it.row0 + kPmTile >= it.lq) ? 1 : 2;
     const int n_keys = it.visible(min(it.row0 + pm_rows_per_item(it.G), it.lq) - 1);
+    it.first = 0;
     it.n_blocks = (n_keys + kPmTile - 1) / kPmTile;
-    it.tail = n_keys - (it.n_blocks - 1) * kPmTile;  // keys of the last block
+    it.tail = n_keys - (it.n_blocks - 1) * kPmTile;
+    if (kSplit) {
+        const int all = it.n_blocks, rank = (int)cluster_rank(), n = (int)cluster_size();
+        it.first = all * rank / n;
+        it.n_blocks = all * (rank + 1) / n - it.first;
+        if (it.first + it.n_blocks < all) it.tail = kPmTile;
+    }
     return it;
 }
 
@@ -155,12 +166,72 @@ __device__ __forceinline__ void pm_release_work(PmShared* sh, uint32_t n) {
 }
 
 // Both, with the item copied.
+template <bool kSplit>
 __device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uint32_t n,
                                         PmItem& it) {
     if (!pm_wait_work(p, sh, n)) return false;
-    it = pm_item(p, sh->work[n % kPmWorks]);
+    it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
     pm_release_work(sh, n);
     return true;
+}
+
+// The cluster's parts of an item joined: softmax warp w of CTA `rank` takes every
+// n-th of its rows, lane l dims 4l .. 4l + 3, and reads the n CTAs' states through
+// their shared memory.
+template <typename T>
+__device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uint8_t* s_kv,
+                                        float2* s_state) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const PmWork w = sh->work[0];
+    if (*(const volatile int*)&sh->work[0].row0 < 0 || *(const volatile int*)&sh->abort != 0) return;
+    const PmItem it = pm_item<false>(p, w);
+    const int n = (int)cluster_size();
+    const uint32_t o_u32 = smem_u32(s_kv), st_u32 = smem_u32(s_state);
+    for (int i = warp + kPmSoftmaxWarps * (int)cluster_rank(); i < it.n_tiles * kPmTile;
+         i += kPmSoftmaxWarps * n) {
+        const int t = i / kPmTile;
+        const int row = it.row0 + (it.G == 1 ? i : i - t * kPmTile);  // of the sequence
+        if (row >= it.lq) continue;
+        const int head = it.G == 1 ? it.head0 : it.head0 + t;
+        float2 st[8];
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            st[c] = c < n ? ld_cluster_f2(cluster_addr(st_u32 + i * 8, c))
+                          : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, st[c].x);
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        const uint32_t piece = o_u32 + i * (kHeadDim * 4) + ((lane ^ (i & 31)) << 4);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            // (a part that saw no key holds nothing; a NaN maximum passes on)
+            if (c >= n || st[c].x == -INFINITY) continue;
+            const float f = fast_exp2((st[c].x - top) * p.scale_log2);
+            const float4 x = ld_cluster_f4(cluster_addr(piece, c));
+            l = fmaf(f, st[c].y, l);
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const size_t at = (size_t)(it.q0 + row) * p.Hq + head;
+        T* out = reinterpret_cast<T*>(p.out) + at * kHeadDim;
+        const float worst = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, fmaf(o.w, 0.f, l * 0.f))));
+        if (__any_sync(0xffffffffu, worst != 0.f)) {
+            prompt_row<T>(p, p.q + (it.q0 + row) * p.q_tok + head * p.q_head,
+                          p.k + it.k0 * p.k_tok + it.kvh * p.k_head,
+                          p.v + it.k0 * p.v_tok + it.kvh * p.v_head, it.visible(row), out,
+                          p.lse != nullptr ? p.lse + at : nullptr, lane);
+            continue;
+        }
+        reinterpret_cast<uint2*>(out)[lane] =
+            make_uint2(ElemOps<T>::pack(o.x * inv, o.y * inv), ElemOps<T>::pack(o.z * inv, o.w * inv));
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[at] = l == 0.f ? -INFINITY : top * p.scale_log2 * kLn2 + logf(l);
+    }
 }
 
 // An item is two query tiles of 128 rows that read the same keys: two heads of
@@ -180,11 +251,15 @@ __device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uin
 // first keys arrive while the present one is computed, and its first scores
 // while the present one's output is written.
 //
+// kSplit: few rows and many keys.  A cluster of 2 to 8 CTAs takes an item, each a
+// part of its key blocks, and joins the parts through distributed shared memory,
+// without a workspace.
+//
 // Bound: a tile's chain scores -> softmax -> output.  One prompt of 16384 tokens
 // (32 heads, bf16) takes 2.0 ms, 1.09 PFLOP/s, 3750 cycles per pair of tiles and
 // block at 1.67 GHz under the card's power cap; the products alone take 2580,
 // the exponentials 2050, and the tensor cores' nominal rate would be 2048.
-template <typename T>
+template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kPmThreads, 1)
     pkv_prompt_mma_kernel(const __grid_constant__ PromptParams p,
                           const __grid_constant__ CUtensorMap map_q,
@@ -197,6 +272,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
     uint8_t* s_kv = smem + 2 * kPmTileBytes;  // kPmStages tiles
     uint8_t* s_out = s_kv + kPmStages * kPmTileBytes;
     PmShared* sh = reinterpret_cast<PmShared*>(s_out + kPmSoftmaxWarps * kPmStageOut);
+    float2* s_state = reinterpret_cast<float2*>(s_out);  // [2][128] m and l (kSplit)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -232,7 +308,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         // ------------------------------------------------------------ schedule
         const int G = p.Hq / p.Hkv;
         const int groups = G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
-        int item = blockIdx.x;
+        int item = kSplit ? blockIdx.x / cluster_size() : blockIdx.x;
         uint32_t n = 0;  // items published
         bool ok = true;
         for (uint32_t round = 0; ok; ++round) {
@@ -250,12 +326,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 }
                 __syncwarp();
                 ++n;
+                if (kSplit) break;  // a cluster has one item
                 // The next item is asked for once the copies of this one's last
                 // blocks are under way: early enough that it is there when this
                 // one ends, late enough to be the fair one to take.
                 ok = pm_wait_warp(p, sh, &sh->issued, (n - 1) & 1u);
                 if (!ok) break;
             }
+            if (kSplit) break;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&sh->launch_bar, 16);
                 launch_cancel_async(&sh->launch, &sh->launch_bar);
@@ -301,7 +379,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         uint32_t i = 0;      // K/V tiles issued: K0 V0 K1 V1 ... of each item
         uint32_t loads = 0;  // items with keys
         bool ok = true;
-        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
+        for (uint32_t n = 0; ok && pm_next<kSplit>(p, sh, n, it); ++n) {
             if (it.n_blocks == 0) {
                 if (lane == 0) mbar_arrive(&sh->issued);
                 continue;
@@ -321,10 +399,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     if (!ok) break;
                     mbar_arrive_expect_tx(&sh->kv_full[st], kPmTileBytes);
                     if (c & 1)
-                        load(s_kv + st * kPmTileBytes, map_v, it.kvh, it.k0 + (c >> 1) * kPmTile,
+                        load(s_kv + st * kPmTileBytes, map_v, it.kvh, it.k0 + (it.first + (int)(c >> 1)) * kPmTile,
                              &sh->kv_full[st]);
                     else
-                        load(s_kv + st * kPmTileBytes, map_k, it.kvh, it.k0 + (c >> 1) * kPmTile,
+                        load(s_kv + st * kPmTileBytes, map_k, it.kvh, it.k0 + (it.first + (int)(c >> 1)) * kPmTile,
                              &sh->kv_full[st]);
                 }
                 mbar_arrive(&sh->issued);
@@ -448,7 +526,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         const std::integral_constant<bool, false> kEven{};
         const std::integral_constant<bool, true> kOdd{};
         bool ok = true;
-        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
+        for (uint32_t n = 0; ok && pm_next<kSplit>(p, sh, n, it); ++n) {
             if (it.n_blocks == 0) continue;
             const bool odd = (gb & 1u) != 0u;
             ok = pm_wait_warp(p, sh, &sh->q_full, items & 1u) &&
@@ -481,12 +559,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             int n_blocks, keys, clear;
             bool mine;
             {
-                const PmItem it = pm_item(p, sh->work[n % kPmWorks]);
+                const PmItem it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
                 mine = t < it.n_tiles;
                 const int tile0 = it.row0 + (it.G == 1 ? t * kPmTile : 0);
-                keys = it.visible(tile0 + r);
+                keys = it.visible(tile0 + r) - it.first * kPmTile;
                 // blocks below need no mask for any row of the tile
-                clear = it.visible(tile0) / kPmTile;
+                clear = it.visible(tile0) / kPmTile - it.first;
                 n_blocks = it.n_blocks;
             }
             if (!mine) {
@@ -578,7 +656,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             }
             if (!ok) break;
             // ---- output rows
-            const PmItem it = pm_item(p, sh->work[n % kPmWorks]);
+            const PmItem it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
             const int qrow = it.row0 + (it.G == 1 ? t * kPmTile : 0) + r;  // of the sequence
             const int head = it.G == 1 ? it.head0 : it.head0 + t;
             const bool real = qrow < it.lq;
@@ -586,6 +664,29 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
+            }
+            if (kSplit) {
+                // this CTA's part of the rows, for the cluster: O in 32 bits where
+                // the keys were (both tiles' products have read them), m and l
+                if (it.n_blocks > 0 && it.n_tiles == 2) {
+                    ok = pm_wait_warp(p, sh, &sh->o_full[t ^ 1], (blocks - 1) & 1u);
+                    if (!ok) break;
+                }
+                if (it.n_blocks > 0) {
+                    uint8_t* mine_o = s_kv + (t * kPmTile + r) * (kHeadDim * 4);
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + 32 * c, o);
+                        tmem_wait_ld32(o);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(mine_o + (((8 * c + i) ^ lane) << 4)) =
+                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+                s_state[t * kPmTile + r] = make_float2(m, l);
+                continue;  // (the item's place is not needed again)
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float worst = 0.f;  // NaN if any value is not finite
@@ -662,6 +763,15 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             pm_release_work(sh, n);
         }
         tc_fence_before();
+    }
+    if (kSplit) {
+        // Every thread of every CTA of the cluster passes both barriers, whatever
+        // happened before.
+        __syncwarp();
+        cluster_sync();
+        if (warp < kPmSoftmaxWarps) pm_join<T>(p, sh, s_kv, s_state);
+        __syncwarp();
+        cluster_sync();  // the others' parts have been read
     }
     __syncthreads();
     if (warp == kPmMmaWarp) {

@@ -122,6 +122,39 @@ def test_prompt_heads(hq, hkv, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lq,lk,hq,hkv", [
+    ([1], [600], 2, 1), ([3], [4000], 2, 1), ([1], [2049], 2, 2), ([130], [3000], 4, 2),
+    ([257], [2300], 3, 3), ([200, 7], [70, 5000], 2, 1), ([16, 16], [2048, 2048], 8, 1),
+    ([700], [1100], 2, 2), ([300], [2200], 1, 1)])
+def test_prompt_few_rows_many_keys(lq, lk, hq, hkv, dtype):
+    """Key blocks shared by the CTAs of a cluster, some of which get none."""
+    q, k, v, cq, ck = packed(lq, lk, hq, hkv, dtype, seed=sum(lk), tail=2)
+    check_prompt(q, k, v, cq, ck, dtype, *run_prompt(q, k, v, cq, ck))
+    a, _ = run_prompt(q, k, v, cq, ck, lse=False)
+    b, _ = run_prompt(q, k, v, cq, ck)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_prompt_few_rows_ignore_what_they_do_not_see(bad):
+    lq, lk = [40, 20], [1500, 1500]
+    q, k, v, cq, ck = packed(lq, lk, 2, 1, "bf16", seed=3, tail=9)
+    want, _ = run_prompt(q, k, v, cq, ck)
+    k2, v2 = k.clone(), v.clone()
+    for t in (k2, v2):
+        t[ck[2]:] = bad
+        t[ck[2] - 5:ck[2]] = bad       # the last keys: rows before them do not see them
+    got, _ = run_prompt(q, k2, v2, cq, ck)
+    seen = list(range(55))
+    _, _, mag, size = pr.prompt_attention(q.double().numpy(), k.double().numpy(),
+                                          v.double().numpy(), cq, ck)
+    w = np.full(want.shape, np.nan)
+    w[seen] = want.double().cpu().numpy()[seen]
+    check_close(got, w, 2 * np.nan_to_num(mag), size, 1e3, "bf16")
+    assert not torch.isfinite(got[55:60].float()).all(-1).any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_prompt_many_short_sequences(dtype):
     lens = [(7 * i) % 23 for i in range(300)]
     q, k, v, cq, ck = packed(lens, lens, 2, 2, dtype, seed=4, tail=1)
