@@ -125,7 +125,8 @@ def test_prompt_heads(hq, hkv, dtype):
 @pytest.mark.parametrize("lq,lk,hq,hkv", [
     ([1], [600], 2, 1), ([3], [4000], 2, 1), ([1], [2049], 2, 2), ([130], [3000], 4, 2),
     ([257], [2300], 3, 3), ([200, 7], [70, 5000], 2, 1), ([16, 16], [2048, 2048], 8, 1),
-    ([700], [1100], 2, 2), ([300], [2200], 1, 1)])
+    ([700], [1100], 2, 2), ([300], [2200], 1, 1),
+    ([2], [4500], 2, 1), ([9], [4097], 1, 1)])
 def test_prompt_few_rows_many_keys(lq, lk, hq, hkv, dtype):
     """Key blocks shared by the CTAs of a cluster, some of which get none."""
     q, k, v, cq, ck = packed(lq, lk, hq, hkv, dtype, seed=sum(lk), tail=2)
