@@ -303,9 +303,9 @@ pkv_status pkv_paged_attention_auto_fp8(
  * K = k_scales[p][h][t / block_tokens] * value, V likewise; scales are
  * [P][Hkv][page_size / block_tokens], block_tokens a multiple of 16 that
  * divides page_size.  A scale is positive and finite, or zero for a block of
- * zeros; a V scale below 2^-60 counts as 2^-60.  q and output are fp16 or bf16 (dtype).  Pages and scales of tokens
- * past a row's length are never used, whatever they hold.  No counterpart in
- * the reference. */
+ * zeros; a V scale below 2^-60 counts as 2^-60.  q and output are fp16 or bf16
+ * (dtype).  Pages and scales of tokens past a row's length are never used,
+ * whatever they hold.  No counterpart in the reference. */
 pkv_status pkv_paged_attention_auto_fp8_block(
     const void* q_source, const void* k_pages, const void* v_pages, const float* k_scales,
     const float* v_scales, const int32_t* block_table, const int32_t* seq_lens,
@@ -342,8 +342,8 @@ pkv_status pkv_paged_attention_auto_fp8_block(
  * free_pages NULL: every page is in block_table already (free_count,
  * free_left and counters are not used).  A page id that is negative or too
  * large for 32-bit slots gives slot -1 (PKV_DEVERR_PAGE_ID).  counters: one
- * zeroed int32, left zero (used where free_left is free_count).  No buffer written may overlap cached_lens or
- * new_lens.  Two calls that overlap on the GPU must not share a stack or
+ * zeroed int32, left zero (used where free_left is free_count).  No buffer
+ * written may overlap cached_lens or new_lens.  Two calls that overlap on the GPU must not share a stack or
  * counters. */
 pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
                             int32_t* block_table, int32_t* slots, int32_t* cu_seqlens,
@@ -355,9 +355,9 @@ pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
 /* Writes T packed tokens, k / v [T][Hkv][128] with the given token and head
  * strides (elements, multiples of 8), into 16-bit pools: token t of head h
  * goes to slot slots[t] = page * page_size + offset.  A negative slot skips
- * its token; one beyond the pool skips it and sets PKV_DEVERR_SLOT.  Of two
- * tokens with one slot either may stay.  The pools and the tokens must not
- * overlap. */
+ * its token; one beyond the pool skips it and sets PKV_DEVERR_SLOT.  The slots
+ * of a call are distinct: of two tokens with one slot, any 16-byte pieces of
+ * either may stay.  The pools and the tokens must not overlap. */
 pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pages,
                         const int32_t* slots, int T, int Hkv, int head_dim, long long k_stride,
                         long long k_head_stride, long long v_stride, long long v_head_stride,
@@ -371,7 +371,8 @@ pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pag
  * and at least the old scale if the first of them is not the block's first
  * token: the earlier tokens stay, moved to the new scale if it grew.  Values
  * are rounded to nearest, ties to even.  Infinities and NaN do not set a
- * scale: the first are stored as +-448, the second as NaN. */
+ * scale: the first are stored as +-448, the second as NaN.  Scales, pools and
+ * tokens must not overlap. */
 pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, void* v_pages,
                                   float* k_scales, float* v_scales, const int32_t* slots, int T,
                                   int Hkv, int head_dim, long long k_stride,
@@ -386,8 +387,7 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
  * row that sees none gives zeros.  q [q_tokens][Hq][128], k / v
  * [k_tokens][Hkv][128] with the given strides (elements, multiples of 8),
  * output [q_tokens][Hq][128] contiguous, apart from the inputs; softmax scale
- * 1 / sqrt(128).  lse
- * (or NULL): [q_tokens][Hq] natural log of each row's sum of exponentials,
+ * 1 / sqrt(128).  lse (or NULL, apart from all): [q_tokens][Hq] natural log of each row's sum of exponentials,
  * -inf for a row that sees no key.  Rows of no sequence are left as they
  * were, and a row's result depends on no key that it does not see, whatever
  * those hold.  A sequence whose ranges lie outside the tokens or run backwards

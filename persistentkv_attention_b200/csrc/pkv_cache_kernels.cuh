@@ -32,32 +32,34 @@ constexpr int kSlotThreads = 256;
 // 3.5 us (4.6, 6.9).
 constexpr int kSlotTokensPerCta = 512;
 
-// Sum over the CTA of one 64-bit value per thread, exclusive prefix returned,
-// total in `total`.  Both 32-bit halves are sums of non-negative values below
-// 2^31, so they do not carry into one another.
-__device__ __forceinline__ unsigned long long slot_scan(unsigned long long v,
-                                                        unsigned long long* s_warp,
-                                                        unsigned long long& total) {
+// Exclusive prefix sums over the CTA of two non-negative values per thread, and
+// their totals in `total`.  Sums stop at INT_MAX: lengths may hold anything, and
+// a row behind so many tokens or pages is not served whatever their number.
+__device__ __forceinline__ int2 slot_scan(int2 v, int2* s_warp, int2& total) {
+    auto add = [](int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)INT_MAX); };
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    unsigned long long x = v;
+    int2 x = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
+        const int yx = __shfl_up_sync(0xffffffffu, x.x, off);
+        const int yy = __shfl_up_sync(0xffffffffu, x.y, off);
+        if (lane >= off) x = make_int2(add(x.x, yx), add(x.y, yy));
     }
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    unsigned long long before = 0;
-    total = 0;
+    int2 before = make_int2(0, 0);
+    total = make_int2(0, 0);
 #pragma unroll
     for (int w = 0; w < kSlotThreads / 32; ++w) {
-        const unsigned long long t = s_warp[w];
-        before += w < warp ? t : 0ull;
-        total += t;
+        const int2 t = s_warp[w];
+        if (w < warp) before = make_int2(add(before.x, t.x), add(before.y, t.y));
+        total = make_int2(add(total.x, t.x), add(total.y, t.y));
     }
     __syncthreads();
-    return before + x - v;
+    x.x = __shfl_up_sync(0xffffffffu, x.x, 1);
+    x.y = __shfl_up_sync(0xffffffffu, x.y, 1);
+    return lane > 0 ? make_int2(add(before.x, x.x), add(before.y, x.y)) : before;
 }
 
 // Everything a token's slot depends on is a prefix sum over the rows before
@@ -72,7 +74,7 @@ __device__ __forceinline__ unsigned long long slot_scan(unsigned long long v,
 // bytes).
 __global__ void __launch_bounds__(kSlotThreads)
     pkv_prompt_slots_kernel(const __grid_constant__ SlotsParams p) {
-    __shared__ unsigned long long s_warp[kSlotThreads / 32];
+    __shared__ int2 s_warp[kSlotThreads / 32];
     __shared__ int s_start[kSlotThreads], s_cached[kSlotThreads], s_need[kSlotThreads];
     __shared__ int s_avail;
     constexpr int kMine = kSlotTokensPerCta / kSlotThreads;  // tokens of a thread
@@ -111,12 +113,11 @@ __global__ void __launch_bounds__(kSlotThreads)
                 need = (c + n + p.page_size - 1) / p.page_size -
                        (c + p.page_size - 1) / p.page_size;
         }
-        unsigned long long total;
-        const unsigned long long pre =
-            slot_scan(((unsigned long long)(unsigned)n << 32) | (unsigned)need, s_warp, total);
+        int2 total;
+        const int2 pre = slot_scan(make_int2(n, need), s_warp, total);
         if (stack) avail = s_avail;  // (written before the scan's barriers)
-        const long long start = tokens + (long long)(pre >> 32);
-        const long long before = pages + (long long)(pre & 0xffffffffull);
+        const long long start = tokens + pre.x;
+        const long long before = pages + pre.y;
         const bool short_of = need > 0 && before + need > avail;
         const bool beyond = n > 0 && start + n > p.num_slots;
         const bool served = valid && !short_of && !beyond;
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(kSlotThreads)
         s_cached[t] = served ? c : -1;
         s_need[t] = (int)min(before, (long long)INT_MAX);
         __syncthreads();
-        const long long end = tokens + (long long)(total >> 32);
+        const long long end = tokens + total.x;
         const int rows = min(kSlotThreads, p.B - base);
         const long long lo = max(t0, tokens), hi = min(t1, end);
         // tokens t0 + t + 256 i of this chunk's rows
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kSlotThreads)
             p.slots[t0 + t + i * kSlotThreads] = slot;
         }
         tokens = end;
-        pages += (long long)(total & 0xffffffffull);
+        pages += total.y;
         __syncthreads();
     }
     for (long long tok = max(t0, tokens) + t; tok < t1; tok += kSlotThreads) p.slots[tok] = -1;

@@ -247,7 +247,8 @@ pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
                         "seq_lens and cu_seqlens must not be the tensors they are made from");
     if (B < 0 || max_pages <= 0 || page_size <= 0 || num_slots < 0 || free_capacity < 0)
         return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid slot map shape");
-    if ((long long)max_pages * page_size >= (1ll << 31))
+    // (a length rounded up to pages fits into 32 bits too)
+    if (((long long)max_pages + 1) * page_size > (1ll << 31))
         return fail_fmt(PKV_ERR_UNSUPPORTED, "max_pages * page_size exceeds 32-bit positions");
     int sms = 0;
     unsigned* error = nullptr;
@@ -310,8 +311,19 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     if (T == 0) return ok();
     st = check_apart(wp, physical_pages, 1);
     if (st != PKV_OK) return st;
-    if (k_scales == v_scales)
+    const long long pool = (long long)physical_pages * Hkv * page_size * kHeadDim;
+    const Range scales[2] = {
+        {reinterpret_cast<const char*>(k_scales), pool / kHeadDim / block_tokens * 4},
+        {reinterpret_cast<const char*>(v_scales), pool / kHeadDim / block_tokens * 4}};
+    if (overlap(scales[0], scales[1]))
         return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must not overlap");
+    for (const Range& sc : scales)
+        if (overlap(sc, {static_cast<const char*>(k_pages), pool}) ||
+            overlap(sc, {static_cast<const char*>(v_pages), pool}) ||
+            overlap(sc, operand_range(k, T, Hkv, wp.k_tok, wp.k_head)) ||
+            overlap(sc, operand_range(v, T, Hkv, wp.v_tok, wp.v_head)))
+            return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                            "the scales must not overlap the pools or the tokens written");
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
@@ -393,6 +405,11 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
         overlap(o, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
         overlap(o, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
         return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "output must not overlap q, k or v");
+    const Range l{reinterpret_cast<const char*>(lse), lse ? (long long)q_tokens * Hq * 4 : 0};
+    if (overlap(l, o) || overlap(l, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
+        overlap(l, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
+        overlap(l, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "lse must not overlap output, q, k or v");
     int sms = 0;
     st = device_state(&sms, &pp.error);
     if (st != PKV_OK) return st;

@@ -95,11 +95,15 @@ __device__ __forceinline__ PmItem pm_item(const PromptParams& p, const PmWork& w
 // Whole warp: the query tile number `rank`, counted from the end over all
 // sequences' tiles of `rows` rows, so that the longest rows of a sequence start
 // first.  Returns 1 with the work filled in, 0 if there are fewer tiles, -1
-// for a tile of a sequence whose ranges are bad.
-__device__ __forceinline__ int pm_find(const PromptParams& p, int rank, int rows, PmWork& w) {
+// for a tile of a sequence whose ranges are bad.  `seen` sequences hold the
+// first `before` tiles: a CTA's items come in ascending order, so the search goes
+// on where the last one ended.
+__device__ __forceinline__ int pm_find(const PromptParams& p, int rank, int rows, PmWork& w,
+                                       int& seen, int& before) {
     const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int base = 0; base < p.B; base += 32) {
+    if (rank < before) seen = before = 0;
+    for (; seen < p.B; seen += 32) {
+        const int base = seen;
         const int b = p.B - 1 - base - lane;
         int q0 = 0, q1 = 0, n = 0;
         if (b >= 0) {
@@ -206,8 +210,9 @@ __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uin
         const uint32_t piece = o_u32 + i * (kHeadDim * 4) + ((lane ^ (i & 31)) << 4);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            // (a part that saw no key holds nothing; a NaN maximum passes on)
-            if (c >= n || st[c].x == -INFINITY) continue;
+            // (a part that saw no key holds nothing; one whose scores are all NaN has
+            // no maximum either, and its sum is NaN)
+            if (c >= n || (st[c].x == -INFINITY && st[c].y == 0.f)) continue;
             const float f = fast_exp2((st[c].x - top) * p.scale_log2);
             const float4 x = ld_cluster_f4(cluster_addr(piece, c));
             l = fmaf(f, st[c].y, l);
@@ -309,11 +314,12 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         const int G = p.Hq / p.Hkv;
         const int groups = G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
         int item = kSplit ? blockIdx.x / cluster_size() : blockIdx.x;
+        int seen = 0, before = 0;
         uint32_t n = 0;  // items published
         bool ok = true;
         for (uint32_t round = 0; ok; ++round) {
             PmWork w;
-            const int found = pm_find(p, item / groups, pm_rows_per_item(G), w);
+            const int found = pm_find(p, item / groups, pm_rows_per_item(G), w, seen, before);
             w.group = item % groups;
             if (found > 0) {  // (a bad sequence is reported by the checking warp)
                 if (n >= (uint32_t)kPmWorks)

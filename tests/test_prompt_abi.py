@@ -30,6 +30,7 @@ def slots(lib, **kw):
     (dict(page=0), 1, "invalid slot map shape"),
     (dict(B=-1), 1, "invalid slot map shape"),
     (dict(maxp=1 << 27), 2, "32-bit positions"),
+    (dict(maxp=178956970, page=12), 2, "32-bit positions"),  # 2^31 - 8: rounded up, too many
 ])
 def test_slots_validation(lib, kw, status, msg):
     assert slots(lib, **kw) == status
@@ -123,6 +124,23 @@ def test_write_refuses_overlaps(lib, fp8, kw):
 def test_prompt_refuses_overlaps(lib, kw):
     assert prompt(lib, **kw) == 1
     assert b"output must not overlap" in lib.pkv_last_error_message()
+
+
+@pytest.mark.parametrize("lse", [1 << 24, (1 << 30) + 40 * 8192 - 16, (1 << 31) - 16, 1 << 32])
+def test_prompt_refuses_an_lse_in_its_operands(lib, lse):
+    kw = dict(out=1 << 24, q=1 << 30, k=1 << 31, v=1 << 32, lse=lse)
+    assert prompt(lib, **kw) == 1
+    assert b"lse must not overlap" in lib.pkv_last_error_message()
+
+
+@pytest.mark.parametrize("ks,vs,msg", [
+    (1 << 34, (1 << 34) + 2044, b"k_scales and v_scales"),  # 64 pages x 8 heads: 2 KB
+    (1 << 30, 1 << 34, b"the scales"), (1 << 34, (1 << 31) - 4, b"the scales"),
+    ((1 << 32) + 8000, 1 << 34, b"the scales"), (1 << 34, (1 << 33) - 4, b"the scales")])
+def test_block_write_refuses_scales_in_its_operands(lib, ks, vs, msg):
+    kw = dict(kp=1 << 30, vp=1 << 31, k=1 << 32, v=1 << 33, ks=ks, vs=vs)
+    assert write(lib, True, **kw) == 1
+    assert msg in lib.pkv_last_error_message()
 
 
 def test_nothing_to_do_is_no_error(lib):

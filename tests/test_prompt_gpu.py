@@ -163,6 +163,13 @@ def test_prompt_many_short_sequences(dtype):
     check_prompt(q, k, v, cq, cq, dtype, out, ls)
 
 
+def test_prompt_thousands_of_sequences():
+    """Many more items than CTAs, most of the grid without a tile of its own."""
+    lens = [1 + (i % 3) for i in range(4000)] + [0] * 90 + [150]
+    q, k, v, cq, ck = packed(lens, lens, 4, 4, "f16", seed=5)
+    check_prompt(q, k, v, cq, ck, "f16", *run_prompt(q, k, v, cq, ck))
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_prompt_large_scores(dtype):
     """Scores of hundreds: the running maximum moves far, later and earlier."""
@@ -200,6 +207,41 @@ def test_prompt_ignores_what_it_does_not_see(dtype, bad):
     torch.testing.assert_close(ls[seen], ls0[seen], rtol=1e-5, atol=1e-5)
     # rows that see them say so
     assert not torch.isfinite(got[cq[2] + 64:cq[3]].float()).all(-1).any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hkv", [1, 4])
+def test_prompt_split_keys_pass_nan_on(dtype, hkv):
+    """Rows whose keys are split among CTAs: a NaN that a row sees reaches it,
+    one in a part of its own, in one key or in the query."""
+    lq, lk = 6, 4500
+    q, k, v, cq, ck = packed([lq], [lk], 4, hkv, dtype, seed=21)
+    nan = float("nan")
+    want, lse = run_prompt(q, k, v, cq, ck)
+    assert want.isfinite().all()
+    for lo, hi in ((0, 2000), (777, 778), (4000, 4494), (0, lk)):
+        k2 = k.clone()
+        k2[lo:hi, 0] = nan
+        got, ls = run_prompt(q, k2, v, cq, ck)
+        g = 4 // hkv  # the heads that read KV head 0
+        assert got[:, :g].isnan().all() and ls[:, :g].isnan().all()
+        assert torch.equal(got[:, g:], want[:, g:]) and torch.equal(ls[:, g:], lse[:, g:])
+    q2 = q.clone()
+    q2[2] = nan
+    got, ls = run_prompt(q2, k, v, cq, ck)
+    rest = [0, 1, 3, 4, 5]
+    assert got[2].isnan().all() and ls[2].isnan().all()
+    assert torch.equal(got[rest], want[rest]) and torch.equal(ls[rest], lse[rest])
+    # the keys of the last position, which only the last row sees
+    k2, v2 = k.clone(), v.clone()
+    k2[-1] = v2[-1] = nan
+    got, ls = run_prompt(q, k2, v2, cq, ck)
+    assert got[-1].isnan().all() and ls[-1].isnan().all()
+    w = np.full(want.shape, np.nan)
+    w[:-1] = want.double().cpu().numpy()[:-1]
+    _, _, mag, size = pr.prompt_attention(q.double().numpy(), k.double().numpy(),
+                                          v.double().numpy(), cq, ck)
+    check_close(got, w, 2 * mag, size, 1e3, dtype)
 
 
 def test_prompt_strided_operands():
@@ -360,6 +402,25 @@ def test_slots_without_a_stack_and_with_bad_rows():
         assert np.array_equal(got.cpu().numpy(), w)
     d, left, code = run_slots([0], [20], np.zeros((1, 4)), 20, 16, [-1, 3], 2)
     assert code == 0x4 >> 2 and d["s"].tolist() == [48 + i for i in range(16)] + [-1] * 4
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_slots_of_lengths_that_hold_anything(page):
+    """Sums of lengths beyond 32 bits, in one chunk of rows and over all: what comes
+    before them is served, no token behind them is."""
+    big = 2 ** 31 - 1
+    new = [5, 3] + [big] * 9 + [4, 0, 2] + [big - 7] * 260 + [6, 0]
+    cached = [0, 2] + [0, 9, 0, -1, 0, 0, 3, 0, 0] + [1, 2, 3] + [0] * 260 + [0, 1]
+    width = 64
+    free = list(range(50))
+    table = np.arange(len(new) * width).reshape(len(new), width) % 40
+    for stack, count in ((free, 50), (None, 0)):
+        d, left, code = run_slots(cached, new, table, 1500, page, stack, count)
+        want = pr.prompt_slots(cached, new, table, 1500, page, stack, count)
+        assert code == 0x2 | 0x8 and (stack is None or left == want[4])
+        assert np.array_equal(d["cu"].cpu().numpy(), np.minimum(want[2], big))
+        for got, w in ((d["t"], want[0]), (d["s"], want[1]), (d["seq"], want[3])):
+            assert np.array_equal(got.cpu().numpy(), w)
 
 
 def test_slots_of_no_rows():
