@@ -280,18 +280,22 @@ class DecodeEngine:
         the attention of each row over its own tokens, computed from the packed
         16-bit K/V.  A row that finds no pages (length 0 in the result) keeps
         none of its K/V."""
+        if self.kv8 and self.kv_block_scales is None:
+            raise RuntimeError("prefill writes 16-bit caches and e4m3 caches with block scales")
         b = block_table.size(0)
         i32 = dict(dtype=torch.int32, device=self.device)
         slots, cu = torch.empty(k.size(0), **i32), torch.empty(b + 1, **i32)
         seq_lens = torch.empty(b, **i32)
+        # wrong tensors are refused before pages are taken
+        ops._check_prompt(q, k, v, cu, None, out, lse)
+        ops._check_write(k, v, self.k_pages, self.v_pages, slots,
+                         self.k_pages.dtype if self.kv8 else k.dtype)
         ops.prompt_slots(torch.zeros(b, **i32), new_lens, block_table, slots, cu, seq_lens,
                          *((None,) * 4 if stack is None else
                            (stack.free_pages, stack.free_count, stack.free_count, stack.counters)),
                          self.page_size)
         if self.kv_block_scales is not None:
             ops.kv_write_fp8_block(k, v, self.k_pages, self.v_pages, *self.kv_block_scales, slots)
-        elif self.kv8:
-            raise RuntimeError("prefill writes 16-bit caches and e4m3 caches with block scales")
         else:
             ops.kv_write(k, v, self.k_pages, self.v_pages, slots)
         ops.prompt_attention(q, k, v, cu, None, out, lse=lse)

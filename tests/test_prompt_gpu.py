@@ -244,6 +244,38 @@ def test_prompt_split_keys_pass_nan_on(dtype, hkv):
     check_close(got, w, 2 * mag, size, 1e3, dtype)
 
 
+def test_prompt_split_keys_in_a_graph():
+    """The split is chosen by shapes; a replay follows the lengths on the device,
+    down to none."""
+    q, k, v, cq, ck = packed([6], [4500], 4, 1, "bf16", seed=31)
+    dev = [t.cuda() for t in (q, k, v)]
+    c, d, out = i32([0, 6]), i32([0, 4500]), torch.zeros_like(dev[0])
+    ls = torch.zeros(6, 4, device="cuda")
+    ops.prompt_attention(*dev, c, d, out, lse=ls)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.prompt_attention(*dev, c, d, out, lse=ls)
+    for cq, ck in (([0, 6], [0, 4500]), ([1, 4], [100, 130]), ([0, 6], [7, 7]), ([2, 2], [0, 4500]),
+                   ([0, 5], [0, 4499]), ([0, 6], [4490, 4500])):
+        c.copy_(i32(cq)), d.copy_(i32(ck))
+        out.fill_(7.0), ls.fill_(7.0)
+        graph.replay()
+        no_error()
+        check_prompt(q, k, v, cq, ck, "bf16", out, ls)
+    # two at once, on two streams
+    c.copy_(i32([0, 6])), d.copy_(i32([0, 4500]))
+    want = out.clone()
+    ops.prompt_attention(*dev, c, d, want)
+    outs = [torch.zeros_like(out) for _ in range(8)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        with torch.cuda.stream(streams[i % 2]):
+            ops.prompt_attention(*dev, c, d, o)
+    no_error()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_prompt_strided_operands():
     """Slices of one fused projection: token strides beyond heads * 128, and
     head-major storage."""
@@ -863,3 +895,101 @@ def test_engine_refuses_caches_it_cannot_fill():
     with pytest.raises(RuntimeError, match="prefill writes"):
         DecodeEngine(p8, p8, 4, kv_scales=(1.0, 1.0)).prefill(
             q, x, x, i32([3]), i32([[0]]), torch.empty_like(q))
+
+
+def test_engine_refuses_before_it_takes_pages():
+    p8, s8 = empty_cache(4, 2, 16, 16)
+    p16 = torch.zeros(4, 2, 16, 128, dtype=torch.float16, device="cuda")
+    x = torch.zeros(3, 2, 128, dtype=torch.float16, device="cuda")
+    q = torch.zeros(3, 4, 128, dtype=torch.float16, device="cuda")
+    stack, table, new = PageStack.full(4, "cuda"), i32([[-1]]), i32([3])
+    good = DecodeEngine(p16, p16.clone(), 4)
+    block = DecodeEngine(p8, p8.clone(), 4, kv_block_scales=(s8, s8.clone()))
+    for engine, args in (
+            (DecodeEngine(p8, p8, 4, kv_scales=(1.0, 1.0)), (q, x, x, new, table, q.clone())),
+            (good, (q, x, x[:2], new, table, q.clone())), (good, (q, x, x, new, table, q[:2])),
+            (good, (q.bfloat16(), x.bfloat16(), x.bfloat16(), new, table, q.bfloat16())),
+            (block, (q, x[:, :1], x[:, :1], new, table, q.clone()))):
+        with pytest.raises(RuntimeError):
+            engine.prefill(*args, stack)
+    torch.cuda.synchronize()
+    assert stack.free_count.item() == 4 and table.tolist() == [[-1]]
+    good.prefill(q, x, x, new, table, q.clone(), stack)
+    no_error()
+    assert stack.free_count.item() == 3 and table.tolist() == [[0]]
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_prompt_beyond_4gb():
+    """Strided operands and packed rows whose bytes lie past 2^32."""
+    gap, n = 1 << 22, 600                     # elements between tokens: 8 MB
+    big = torch.empty(gap * n, dtype=torch.bfloat16, device="cuda")
+    q, k, v, cq, ck = packed([n], [n], 2, 1, "bf16", seed=12)
+    views, at = [], 0
+    for t in (q, k, v):
+        view = big.as_strided((n, t.shape[1], 128), (gap, 128, 1), at)
+        view.copy_(t)
+        views.append(view)
+        at += t.shape[1] * 128
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    ls = torch.full(q.shape[:2], 7.0, device="cuda")
+    ops.prompt_attention(*views, i32(cq), None, out, lse=ls)
+    no_error()
+    check_prompt(q, k, v, cq, ck, "bf16", out, ls)
+    del big, views
+    # the last rows of a long packed batch; nobody's rows before them
+    rows = (1 << 32) // (8 * 256) + 70
+    dq = torch.zeros(rows, 8, 128, dtype=torch.float16, device="cuda")
+    out = torch.zeros_like(dq)
+    q, k, v, cq, ck = packed([60], [60], 8, 2, "f16", seed=13)
+    dq[-60:] = q.cuda()
+    ops.prompt_attention(dq, k.cuda(), v.cuda(), i32([rows - 60, rows]), i32([0, 60]), out)
+    no_error()
+    small, _ = run_prompt(q, k, v, cq, ck)
+    assert torch.equal(out[-60:], small) and not out[:-60].any()
+
+
+@pytest.mark.parametrize("cache", ["f16", "block"])
+def test_pools_beyond_4gb(cache):
+    """Writes to and decode from the last pages of pools past 2^32 bytes."""
+    hq, hkv, page = 8, 4, 16
+    elem = 2 if cache == "f16" else 1
+    pool = (1 << 32) // (hkv * page * 128 * elem) + 9
+    n = 100
+    pages = np.arange(pool - 1, pool - 8, -1)
+    slots = np.concatenate([p * page + np.arange(page) for p in pages])[:n].astype(np.int32)
+    gen = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(n, hkv, 128, generator=gen).half() for _ in range(2))
+    q = torch.randn(1, hq, 128, generator=gen).half()
+    table, lens = pages[None], [n]
+    near = np.arange(7)[None]               # the same rows in a pool of 7 pages
+    local = np.arange(n, dtype=np.int32)
+    if cache == "f16":
+        outs = []
+        for size, s, t in ((pool, slots, table), (7, local, near)):
+            kp = torch.zeros(size, hkv, page, 128, dtype=torch.float16, device="cuda")
+            vp = torch.zeros_like(kp)
+            ops.kv_write(k.cuda(), v.cuda(), kp, vp, i32(s))
+            engine = DecodeEngine(kp, vp, hq)
+            out = torch.zeros(1, hq, 128, dtype=torch.float16, device="cuda")
+            engine.run(engine.upload(engine.plan_step(lens, t.astype(np.int32))), q.cuda(), out)
+            no_error()
+            outs.append((kp[torch.as_tensor(t[0]).cuda()], vp[torch.as_tensor(t[0]).cuda()], out))
+            del kp, vp, engine
+    else:
+        outs = []
+        for size, s, t in ((pool, slots, table), (7, local, near)):
+            kp = torch.zeros(size, hkv, page, 128, dtype=torch.uint8, device="cuda")
+            kp = kp.view(torch.float8_e4m3fn)
+            vp = torch.zeros_like(kp.view(torch.uint8)).view(torch.float8_e4m3fn)
+            ks = torch.zeros(size, hkv, 1, device="cuda")
+            vs = torch.zeros_like(ks)
+            ops.kv_write_fp8_block(k.cuda(), v.cuda(), kp, vp, ks, vs, i32(s))
+            out = run_decode(q, kp, ks, vp, vs, t, lens)
+            no_error()
+            at = torch.as_tensor(t[0]).cuda()
+            outs.append((kp.view(torch.uint8)[at], vp.view(torch.uint8)[at], ks[at], vs[at], out))
+            del kp, vp, ks, vs
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert outs[0][-1].any()
