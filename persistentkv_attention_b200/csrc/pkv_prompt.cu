@@ -174,7 +174,7 @@ pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, int sms, cudaS
         st = pp.Tk > 0 ? token_map(&mv, pp.v, pp.Tk, pp.Hkv, pp.v_tok, pp.v_head, dtype)
                        : token_map(&mv, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
     if (st != PKV_OK) return st;
-    const int G = pp.Hq / pp.Hkv;
+    const int G = pp.G;
     const int rows = G == 1 ? 2 * kPmTile : kPmTile;
     // every sequence has at most one tile that is not full
     const long long tiles = std::min<long long>((long long)pp.Tq / rows + pp.B, pp.Tq);
@@ -399,6 +399,7 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
     pp.Tk = k_tokens;
     pp.Hq = Hq;
     pp.Hkv = Hkv;
+    pp.G = G;
     pp.scale_log2 = (1.0f / sqrtf((float)kHeadDim)) * kLog2e;
     const Range o = operand_range(output, q_tokens, Hq, (long long)Hq * kRowBytes, kRowBytes);
     if (overlap(o, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||

@@ -16,7 +16,7 @@ struct PromptParams {
     float* lse;           // [Tq][Hq] or null
     unsigned* error;
     long long q_tok, q_head, k_tok, k_head, v_tok, v_head;
-    int B, Tq, Tk, Hq, Hkv;
+    int B, Tq, Tk, Hq, Hkv, G;
     float scale_log2;
 };
 

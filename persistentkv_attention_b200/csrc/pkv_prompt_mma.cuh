@@ -17,7 +17,7 @@ constexpr int kPmSoftmaxWarps = 8;
 constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10, kPmCheckWarp = 11;
 constexpr int kPmThreads = 384;
 constexpr int kPmParts = 4;  // parts of a block's weights, 32 keys each, handed over one by one
-constexpr int kPmStageOut = 32 * 64;  // a softmax warp's 32 rows x 32 output dims
+constexpr int kPmStageOut = 32 * 128;  // a softmax warp's 32 rows x 64 output dims
 constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes +
                                 kPmSoftmaxWarps * kPmStageOut + 512;
 // TMEM columns: scores of tile t at 128 t (its weights, 16 bit, in the first
@@ -34,13 +34,21 @@ template <typename T>
 constexpr float kPmLazy = std::is_same<T, __half>::value ? 14.0f : 32.0f;
 
 // One item of work: two query tiles that read the same keys.
-struct PmWork {
-    int q0, k0, lq, lk;  // the sequence's first query row and key, and lengths
-    int row0;            // first query row of the item in its sequence; -1: no more items
-    int group;           // head or pair of heads
-    int pad[2];
+struct alignas(16) PmWork {
+    int q0, k0, lq, lk;     // the sequence's first query row and key, and lengths
+    int row0;               // first query row of the item in its sequence; -1: no more items
+    int head0, kvh, n_tiles;
+    int first, n_blocks;    // this CTA's key blocks
+    int tail;               // keys of the last of them
+    int pad;
+    // keys that row i of the sequence sees
+    __device__ __forceinline__ int visible(int i) const {
+        return max(0, min(lk, i + 1 + lk - lq));
+    }
 };
-constexpr int kPmWorks = 2;  // current item and the next
+// The present item and those to come: with two, an item's schedule waited for the
+// end of the output of the last but one.
+constexpr int kPmWorks = 4;
 
 struct PmShared {
     uint4 launch;  // answer of the launch control
@@ -53,43 +61,26 @@ struct PmShared {
 };
 static_assert(sizeof(PmShared) <= 512, "prompt CTA's shared state");
 
-// What follows from an item for every role.
-struct PmItem {
-    int q0, k0, lq, lk, row0, head0, kvh, n_tiles, G;
-    int first, n_blocks;  // this CTA's key blocks
-    int tail;             // keys of the last of them
-    // keys that row i of the sequence sees
-    __device__ __forceinline__ int visible(int i) const {
-        return max(0, min(lk, i + 1 + lk - lq));
-    }
-};
-
 __device__ __forceinline__ int pm_rows_per_item(int G) { return G == 1 ? 2 * kPmTile : kPmTile; }
 
-// kSplit: the CTAs of a cluster share the item, its key blocks in equal parts.
+// What follows for every role from the sequence, the rows and the head or pair of
+// heads.  kSplit: the CTAs of a cluster share the item, its key blocks in equal
+// parts.
 template <bool kSplit>
-__device__ __forceinline__ PmItem pm_item(const PromptParams& p, const PmWork& w) {
-    PmItem it;
-    it.G = p.Hq / p.Hkv;
-    it.q0 = w.q0;
-    it.k0 = w.k0;
-    it.lq = w.lq;
-    it.lk = w.lk;
-    it.row0 = w.row0;
-    it.head0 = it.G == 1 ? w.group : 2 * w.group;
-    it.kvh = it.head0 / it.G;
-    it.n_tiles = (it.G == 1 && it.row0 + kPmTile >= it.lq) ? 1 : 2;
-    const int n_keys = it.visible(min(it.row0 + pm_rows_per_item(it.G), it.lq) - 1);
-    it.first = 0;
-    it.n_blocks = (n_keys + kPmTile - 1) / kPmTile;
-    it.tail = n_keys - (it.n_blocks - 1) * kPmTile;
+__device__ __forceinline__ void pm_item(const PromptParams& p, PmWork& w, int group) {
+    w.head0 = p.G == 1 ? group : 2 * group;
+    w.kvh = w.head0 / p.G;
+    w.n_tiles = (p.G == 1 && w.row0 + kPmTile >= w.lq) ? 1 : 2;
+    const int n_keys = w.visible(min(w.row0 + pm_rows_per_item(p.G), w.lq) - 1);
+    w.first = 0;
+    w.n_blocks = (n_keys + kPmTile - 1) / kPmTile;
+    w.tail = n_keys - (w.n_blocks - 1) * kPmTile;
     if (kSplit) {
-        const int all = it.n_blocks, rank = (int)cluster_rank(), n = (int)cluster_size();
-        it.first = all * rank / n;
-        it.n_blocks = all * (rank + 1) / n - it.first;
-        if (it.first + it.n_blocks < all) it.tail = kPmTile;
+        const int all = w.n_blocks, rank = (int)cluster_rank(), n = (int)cluster_size();
+        w.first = all * rank / n;
+        w.n_blocks = all * (rank + 1) / n - w.first;
+        if (w.first + w.n_blocks < all) w.tail = kPmTile;
     }
-    return it;
 }
 
 // Whole warp: the query tile number `rank`, counted from the end over all
@@ -170,11 +161,10 @@ __device__ __forceinline__ void pm_release_work(PmShared* sh, uint32_t n) {
 }
 
 // Both, with the item copied.
-template <bool kSplit>
 __device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uint32_t n,
-                                        PmItem& it) {
+                                        PmWork& it) {
     if (!pm_wait_work(p, sh, n)) return false;
-    it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
+    it = sh->work[n % kPmWorks];
     pm_release_work(sh, n);
     return true;
 }
@@ -186,17 +176,16 @@ template <typename T>
 __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uint8_t* s_kv,
                                         float2* s_state) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const PmWork w = sh->work[0];
     if (*(const volatile int*)&sh->work[0].row0 < 0 || *(const volatile int*)&sh->abort != 0) return;
-    const PmItem it = pm_item<false>(p, w);
+    const PmWork it = sh->work[0];
     const int n = (int)cluster_size();
     const uint32_t o_u32 = smem_u32(s_kv), st_u32 = smem_u32(s_state);
     for (int i = warp + kPmSoftmaxWarps * (int)cluster_rank(); i < it.n_tiles * kPmTile;
          i += kPmSoftmaxWarps * n) {
         const int t = i / kPmTile;
-        const int row = it.row0 + (it.G == 1 ? i : i - t * kPmTile);  // of the sequence
+        const int row = it.row0 + (p.G == 1 ? i : i - t * kPmTile);  // of the sequence
         if (row >= it.lq) continue;
-        const int head = it.G == 1 ? it.head0 : it.head0 + t;
+        const int head = p.G == 1 ? it.head0 : it.head0 + t;
         float2 st[8];
         float top = -INFINITY;
 #pragma unroll
@@ -311,17 +300,16 @@ __global__ void __launch_bounds__(kPmThreads, 1)
 
     if (warp == kPmPlanWarp) {
         // ------------------------------------------------------------ schedule
-        const int G = p.Hq / p.Hkv;
-        const int groups = G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
+        const int groups = p.G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
         int item = kSplit ? blockIdx.x / cluster_size() : blockIdx.x;
         int seen = 0, before = 0;
         uint32_t n = 0;  // items published
         bool ok = true;
         for (uint32_t round = 0; ok; ++round) {
             PmWork w;
-            const int found = pm_find(p, item / groups, pm_rows_per_item(G), w, seen, before);
-            w.group = item % groups;
+            const int found = pm_find(p, item / groups, pm_rows_per_item(p.G), w, seen, before);
             if (found > 0) {  // (a bad sequence is reported by the checking warp)
+                pm_item<kSplit>(p, w, item % groups);
                 if (n >= (uint32_t)kPmWorks)
                     ok = pm_wait_warp(p, sh, &sh->work_empty[n % kPmWorks],
                                       (n / kPmWorks - 1) & 1u);
@@ -381,11 +369,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             tma_load_3d(dst, &map, 0, head, token, bar);
             tma_load_3d(dst + kPmHalfBytes, &map, 64, head, token, bar);
         };
-        PmItem it;
+        PmWork it;
         uint32_t i = 0;      // K/V tiles issued: K0 V0 K1 V1 ... of each item
         uint32_t loads = 0;  // items with keys
         bool ok = true;
-        for (uint32_t n = 0; ok && pm_next<kSplit>(p, sh, n, it); ++n) {
+        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
             if (it.n_blocks == 0) {
                 if (lane == 0) mbar_arrive(&sh->issued);
                 continue;
@@ -396,8 +384,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             if (lane == 0) {
                 mbar_arrive_expect_tx(&sh->q_full, it.n_tiles * kPmTileBytes);
                 for (int t = 0; t < it.n_tiles; ++t)
-                    load(s_q + t * kPmTileBytes, map_q, it.G == 1 ? it.head0 : it.head0 + t,
-                         it.q0 + it.row0 + (it.G == 1 ? t * kPmTile : 0), &sh->q_full);
+                    load(s_q + t * kPmTileBytes, map_q, p.G == 1 ? it.head0 : it.head0 + t,
+                         it.q0 + it.row0 + (p.G == 1 ? t * kPmTile : 0), &sh->q_full);
                 for (int c = 0; ok && c < 2 * it.n_blocks; ++c, ++i) {
                     const int st = i % kPmStages;
                     if (i >= (uint32_t)kPmStages)
@@ -428,9 +416,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         // uniform values; one elected lane issues the products and commits.
         constexpr uint32_t kDescQk = mma_desc_f16(kPmTile, kPmTile, kBf16, false);
         constexpr uint32_t kDescPv = mma_desc_f16(kPmTile, kHeadDim, kBf16, true);
-        const uint64_t q_desc = smem_desc_sw128(smem_u32(s_q), 16, 1024);
-        const uint64_t k_desc = smem_desc_sw128(smem_u32(s_kv), 16, 1024);
-        const uint64_t v_desc = smem_desc_sw128(smem_u32(s_kv), kPmHalfBytes, 1024);
+        const uint32_t q_desc = smem_desc_sw128(smem_u32(s_q), 16);
+        const uint32_t k_desc = smem_desc_sw128(smem_u32(s_kv), 16);
+        const uint32_t v_desc = smem_desc_sw128(smem_u32(s_kv), kPmHalfBytes);
         constexpr uint32_t kTileStep = kPmTileBytes >> 4;  // in descriptor units
         // S of tile t from the K tile in stage st
         auto scores = [&](int t, int st) {
@@ -450,7 +438,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                            kDescPv, accumulate || ks > 0);
             }
         };
-        PmItem it{};
+        PmWork it{};
         uint32_t gb = 0;               // blocks of the items before
         uint32_t items = 0;            // items with keys
         uint32_t blocks[2] = {0u, 0u}, outs[2] = {0u, 0u};  // each tile's blocks and items
@@ -532,7 +520,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         const std::integral_constant<bool, false> kEven{};
         const std::integral_constant<bool, true> kOdd{};
         bool ok = true;
-        for (uint32_t n = 0; ok && pm_next<kSplit>(p, sh, n, it); ++n) {
+        for (uint32_t n = 0; ok && pm_next(p, sh, n, it); ++n) {
             if (it.n_blocks == 0) continue;
             const bool odd = (gb & 1u) != 0u;
             ok = pm_wait_warp(p, sh, &sh->q_full, items & 1u) &&
@@ -565,9 +553,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             int n_blocks, keys, clear;
             bool mine;
             {
-                const PmItem it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
+                const PmWork it = sh->work[n % kPmWorks];
                 mine = t < it.n_tiles;
-                const int tile0 = it.row0 + (it.G == 1 ? t * kPmTile : 0);
+                const int tile0 = it.row0 + (p.G == 1 ? t * kPmTile : 0);
                 keys = it.visible(tile0 + r) - it.first * kPmTile;
                 // blocks below need no mask for any row of the tile
                 clear = it.visible(tile0) / kPmTile - it.first;
@@ -662,9 +650,9 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             }
             if (!ok) break;
             // ---- output rows
-            const PmItem it = pm_item<kSplit>(p, sh->work[n % kPmWorks]);
-            const int qrow = it.row0 + (it.G == 1 ? t * kPmTile : 0) + r;  // of the sequence
-            const int head = it.G == 1 ? it.head0 : it.head0 + t;
+            const PmWork it = sh->work[n % kPmWorks];
+            const int qrow = it.row0 + (p.G == 1 ? t * kPmTile : 0) + r;  // of the sequence
+            const int head = p.G == 1 ? it.head0 : it.head0 + t;
             const bool real = qrow < it.lq;
             if (it.n_blocks > 0) {
                 ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
@@ -695,58 +683,68 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 continue;  // (the item's place is not needed again)
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            float worst = 0.f;  // NaN if any value is not finite
-            // Through shared memory, 32 dims at a time, so that a warp stores 64
-            // bytes of 8 rows at once: a thread writing its own row touches 32
+            const uint64_t inv2 = pack_f32x2(inv, inv);
+            uint64_t worst2[2] = {0ull, 0ull};  // NaN if any value is not finite
+            // Through shared memory, 64 dims at a time, so that a warp stores 128
+            // bytes of 4 rows at once: a thread writing its own row touches 32
             // lines an instruction, and the stores took longer than a block.
-            // 16-byte piece i of row r stands at i ^ (r / 2): no bank conflicts.
+            // 16-byte piece i of row r stands at i ^ (r % 8): no bank conflicts.
             uint8_t* stage = s_out + warp * kPmStageOut;
-            const int srow = lane >> 2, spiece = lane & 3;  // row of 8 and piece it stores
+            const int srow = lane >> 3, spiece = lane & 7;  // row of 4 and piece it stores
+            const int rows = it.lq - (qrow - lane);         // of the sequence, from the warp's first
+            uint4* dst = reinterpret_cast<uint4*>(
+                             reinterpret_cast<T*>(p.out) +
+                             ((size_t)(it.q0 + qrow - lane + srow) * p.Hq + head) * kHeadDim) + spiece;
+            const size_t step = (size_t)4 * p.Hq * (kRowBytes / 16);
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
+            for (int c = 0; c < 2; ++c) {
+                uint32_t o[64];
                 if (it.n_blocks > 0) {
-                    tmem_ld32(t_o + 32 * c, o);
+                    tmem_ld32(t_o + 64 * c, o);
+                    tmem_ld32(t_o + 64 * c + 32, o + 32);
                     tmem_wait_ld32(o);
+                    tmem_wait_ld32(o + 32);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    for (int i = 0; i < 64; ++i) o[i] = 0u;
                 }
-                if (c == 3 && it.n_blocks > 0) {
+                if (c == 1 && it.n_blocks > 0) {
                     // TMEM has been read: the next item's output may start
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh->o_empty[t]);
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) worst = fmaf(__uint_as_float(o[i]), 0.f, worst);
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t u[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 u;
-                    u.x = ElemOps<T>::pack(__uint_as_float(o[8 * i]) * inv,
-                                           __uint_as_float(o[8 * i + 1]) * inv);
-                    u.y = ElemOps<T>::pack(__uint_as_float(o[8 * i + 2]) * inv,
-                                           __uint_as_float(o[8 * i + 3]) * inv);
-                    u.z = ElemOps<T>::pack(__uint_as_float(o[8 * i + 4]) * inv,
-                                           __uint_as_float(o[8 * i + 5]) * inv);
-                    u.w = ElemOps<T>::pack(__uint_as_float(o[8 * i + 6]) * inv,
-                                           __uint_as_float(o[8 * i + 7]) * inv);
-                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = u;
+                    for (int x = 0; x < 4; ++x) {
+                        const uint64_t o2 = pack_f32x2(__uint_as_float(o[8 * i + 2 * x]),
+                                                       __uint_as_float(o[8 * i + 2 * x + 1]));
+                        float a, d;
+                        worst2[x & 1] = fma_f32x2(o2, 0ull, worst2[x & 1]);
+                        unpack_f32x2(mul_f32x2(o2, inv2), a, d);
+                        u[x] = ElemOps<T>::pack(a, d);
+                    }
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                        make_uint4(u[0], u[1], u[2], u[3]);
                 }
                 __syncwarp();
+                uint4 u[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 8 * k + srow;  // of the warp
-                    const uint4 u = *reinterpret_cast<const uint4*>(
-                        stage + row * 64 + ((spiece ^ ((row >> 1) & 3)) << 4));
-                    const int seq_row = qrow - lane + row;
-                    if (seq_row < it.lq)
-                        reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
-                                                 ((size_t)(it.q0 + seq_row) * p.Hq + head) *
-                                                     kHeadDim)[4 * c + spiece] = u;
+                for (int k = 0; k < 8; ++k) {  // (all loads first: the stores may alias)
+                    const int row = 4 * k + srow;  // of the warp
+                    u[k] = *reinterpret_cast<const uint4*>(
+                        stage + row * 128 + ((spiece ^ (row & 7)) << 4));
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (4 * k + srow < rows) dst[k * step + 8 * c] = u[k];
                 __syncwarp();
             }
+            float bad[2];
+            unpack_f32x2(add_f32x2(worst2[0], worst2[1]), bad[0], bad[1]);
+            const float worst = bad[0] + bad[1];
             if (real && p.lse != nullptr)
                 p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
                     l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
