@@ -585,9 +585,14 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                         tmem_ld32(t_s + 96, s + 96);
                     }
                     if (j >= clear) {
+                        // (32 keys that every row of the warp sees need no mask)
 #pragma unroll
-                        for (int c = 64 * h; c < 64 * h + 64; ++c)
-                            if (c >= lim) s[c] = 0xff800000u;
+                        for (int c0 = 64 * h; c0 < 64 * h + 64; c0 += 32) {
+                            if (__all_sync(0xffffffffu, lim >= c0 + 32)) continue;
+#pragma unroll
+                            for (int c = c0; c < c0 + 32; ++c)
+                                if (c >= lim) s[c] = 0xff800000u;
+                        }
                     }
 #pragma unroll
                     for (int c = 64 * h; c < 64 * h + 64; c += 2)
@@ -654,6 +659,11 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             const int qrow = it.row0 + (p.G == 1 ? t * kPmTile : 0) + r;  // of the sequence
             const int head = p.G == 1 ? it.head0 : it.head0 + t;
             const bool real = qrow < it.lq;
+            // (while the last product runs)
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (!kSplit && real && p.lse != nullptr)
+                p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
+                    l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
             if (it.n_blocks > 0) {
                 ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
                 if (!ok) break;
@@ -682,7 +692,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 s_state[t * kPmTile + r] = make_float2(m, l);
                 continue;  // (the item's place is not needed again)
             }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
             const uint64_t inv2 = pack_f32x2(inv, inv);
             uint64_t worst2[2] = {0ull, 0ull};  // NaN if any value is not finite
             // Through shared memory, 64 dims at a time, so that a warp stores 128
@@ -745,9 +754,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             float bad[2];
             unpack_f32x2(add_f32x2(worst2[0], worst2[1]), bad[0], bad[1]);
             const float worst = bad[0] + bad[1];
-            if (real && p.lse != nullptr)
-                p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
-                    l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
             // A value that is not finite may come from a key the row does not see
             // (weight 0 times an infinite or NaN V): such a row is computed again
             // from its own keys alone.
