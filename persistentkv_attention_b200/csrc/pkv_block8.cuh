@@ -328,8 +328,10 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
                         const int head = pid * p.Hkv + it.kvh;
                         const int off = tok % p.page_size;
                         y = head * p.page_size + off;
-                        sc = head * nblk + off / bp.block;
-                        sc_step = BOX > kB8Scale && bp.block == kB8Scale ? 1 : 0;
+                        const int blk = off / bp.block;
+                        sc = head * nblk + blk;
+                        // (a box lies within a page, so its second part's block does too)
+                        if (BOX > kB8Scale) sc_step = (off + kB8Scale) / bp.block - blk;
                     }
                 }
                 if (!round_free()) {
