@@ -548,6 +548,9 @@ def kv_append(k_new, v_new, k_pages, v_pages, block_table, positions, free_pages
             raise RuntimeError("a free-page list needs free_count and counters")
         _check_tensor(free_count, "free_count", torch.int32, 1)
         _check_tensor(counters, "counters", torch.int32, 1)
+        if free_pages.numel() == 0:
+            # no address, which would mean that there is no stack: one of no pages
+            free_pages = free_count = torch.zeros_like(free_count)
         fp, fc, ctr = free_pages.data_ptr(), free_count.data_ptr(), counters.data_ptr()
     _native.check(_native.load().pkv_kv_append(
         k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
@@ -727,7 +730,8 @@ def prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens
     for rows not served and behind the last token), ``cu_seqlens`` [B + 1],
     ``seq_lens`` [B] (the lengths after the call) and ``free_left`` [1] (may be
     ``free_count``).  ``counters``: one zeroed int32, left zero.  With
-    ``free_pages`` None every page is in ``block_table`` already.  See
+    ``free_pages`` None every page is in ``block_table`` already (an empty
+    ``free_pages`` is a stack without pages).  See
     ``pkv_prompt_slots`` for the rows that are not served.  No counterpart in
     the reference."""
     i32, dev, table, n = torch.int32, cached_lens.get_device(), block_table.shape, slots.shape
@@ -757,7 +761,9 @@ def prompt_slots(cached_lens, new_lens, block_table, slots, cu_seqlens, seq_lens
     fp = fc = fl = ctr = None
     capacity = 0
     if free_pages is not None:
-        fp, fc = free_pages.data_ptr(), free_count.data_ptr()
+        # (an empty tensor has no address, and none would mean that there is no stack)
+        fc = free_count.data_ptr()
+        fp = free_pages.data_ptr() or fc
         fl, ctr = free_left.data_ptr(), counters.data_ptr()
         capacity = free_pages.numel()
     _native.check(_native.load().pkv_prompt_slots(

@@ -2,12 +2,14 @@
 widest: block and page sizes, values that are not finite, scales far apart,
 nothing to do."""
 
+import numpy as np
 import pytest
 import torch
 
-from persistentkv_attention_b200 import _native
+from persistentkv_attention_b200 import _native, ops
+from persistentkv_attention_b200.serving import PageStack
 from tests.test_prompt_gpu import (DT, check_block_write, check_decode, decode_case, empty_cache,
-                                   run_decode, slots_of)
+                                   i32, run_decode, run_slots, slots_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +56,44 @@ def test_block_write_of_blocks_of_odd_multiples(page, block, dtype):
         x = x.to(DT[dtype]).cuda()
         check_block_write(x[:, :hkv], x[:, hkv:], all_slots[:, at:at + n].reshape(-1), kp, vp, ks, vs)
         at += n
+
+
+# ------------------------------------------------------------------ nothing there
+@pytest.mark.parametrize("in_place", [False, True])
+def test_slots_of_an_empty_stack(in_place):
+    """A free list of no pages serves no row that needs one, whatever the table
+    holds; rows that need none go on."""
+    cached, new = [0, 5, 16, 0], [3, 11, 1, 0]
+    table = np.arange(4)[:, None] * np.ones((1, 3), np.int64)
+    d, left, code = run_slots(cached, new, table, 16, 16, [], 0, in_place)
+    assert code == 0x80 and left == 0
+    assert d["s"].tolist() == [-1] * 3 + list(range(16 + 5, 32)) + [-1] * 2
+    assert d["seq"].tolist() == [0, 16, 16, 0] and np.array_equal(d["t"].cpu().numpy(), table)
+    # one that claims pages it cannot hold
+    d, left, code = run_slots(cached, new, table, 16, 16, [], 7, in_place)
+    assert code == 0x80 | 0x10 and left == 0 and (d["s"][:3] == -1).all()
+
+
+def test_slots_of_a_full_stack_of_no_pages():
+    stack = PageStack.full(0, "cuda")
+    s, cu, seq, table = i32([5, 5]), i32([0, 0]), i32([9]), i32([[0]])
+    ops.prompt_slots(i32([0]), i32([2]), table, s, cu, seq, stack.free_pages, stack.free_count,
+                     stack.free_count, stack.counters, 16)
+    torch.cuda.synchronize()
+    assert _native.device_error(clear=True) == 0x80
+    assert s.tolist() == [-1, -1] and seq.tolist() == [0] and stack.free_count.item() == 0
+
+
+def test_append_to_an_empty_stack():
+    """A token that opens a page finds none; one inside a page is written."""
+    kp = torch.zeros(2, 1, 16, 128, dtype=torch.float16, device="cuda")
+    vp, table = torch.zeros_like(kp), i32([[0, 0], [1, 0]])
+    x = torch.ones(2, 1, 128, dtype=torch.float16, device="cuda")
+    stack = PageStack.full(0, "cuda")
+    ops.kv_append(x, x, kp, vp, table, i32([16, 3]), stack.free_pages, stack.free_count,
+                  stack.counters)
+    torch.cuda.synchronize()
+    assert _native.device_error(clear=True) == 0x80
+    assert not kp[0].any() and kp[1, 0, 3].all() and kp.sum() == 128 and torch.equal(kp, vp)
+    assert stack.free_count.item() == 0 and stack.counters.item() == 0
+    assert table.tolist() == [[0, 0], [1, 0]]
