@@ -1110,7 +1110,9 @@ pkv_status pkv_paged_attention_auto_fp8_block(
     size_t workspace_bytes, int32_t* merge_counters, int B, int q_rows, int out_rows, int Hq,
     int Hkv, int head_dim, int physical_pages, int page_size, int max_pages, int block_tokens,
     pkv_dtype dtype, void* stream) {
-    if (output == nullptr) return fail(PKV_ERR_INVALID_ARGUMENT, "output must be a CUDA tensor");
+    // (tensors of no rows have no address)
+    if (B != 0 && output == nullptr)
+        return fail(PKV_ERR_INVALID_ARGUMENT, "output must be a CUDA tensor");
     if (k_scales == nullptr || v_scales == nullptr)
         return fail(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must be CUDA tensors");
     if (page_size <= 0) return fail(PKV_ERR_INVALID_ARGUMENT, "page_size must be positive");
@@ -1121,6 +1123,14 @@ pkv_status pkv_paged_attention_auto_fp8_block(
                     block_tokens, page_size);
     Common c{q_source, k_pages, v_pages, block_table, B, Hq, Hkv, head_dim,
              physical_pages, page_size, max_pages, dtype};
+    if (B == 0) {
+        if (k_pages == nullptr)
+            return fail(PKV_ERR_INVALID_ARGUMENT, "k_pages must be a CUDA tensor");
+        c.q = k_pages;
+        c.block_table = static_cast<const int32_t*>(k_pages);
+        const pkv_status st = check_common(c);
+        return st != PKV_OK ? st : ok_status();
+    }
     const BlockScales scales{k_scales, v_scales, block_tokens};
     return auto_common(c, seq_lens, q_indices, out_indices, output, nullptr, workspace,
                        workspace_bytes, merge_counters, q_rows, out_rows, stream, nullptr, false,

@@ -50,11 +50,13 @@ pkv_status write_params(WriteParams& wp, const void* k, const void* v, void* k_p
                         long long k_stride, long long k_head_stride, long long v_stride,
                         long long v_head_stride, int physical_pages, int page_size,
                         pkv_dtype dtype) {
-    if (k == nullptr || v == nullptr)
+    // (tensors of no tokens have no address)
+    if (T > 0 && (k == nullptr || v == nullptr))
         return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k and v must be CUDA tensors");
     if (k_pages == nullptr || v_pages == nullptr)
         return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_pages and v_pages must be CUDA tensors");
-    if (slots == nullptr) return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "slots must be a CUDA tensor");
+    if (T > 0 && slots == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "slots must be a CUDA tensor");
     if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
         return fail_fmt(PKV_ERR_UNSUPPORTED, "k has wrong dtype");
     if (head_dim != kHeadDim)

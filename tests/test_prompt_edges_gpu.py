@@ -7,9 +7,9 @@ import pytest
 import torch
 
 from persistentkv_attention_b200 import _native, ops
-from persistentkv_attention_b200.serving import PageStack
+from persistentkv_attention_b200.serving import DecodeEngine, PageStack
 from tests.test_prompt_gpu import (DT, check_block_write, check_decode, decode_case, empty_cache,
-                                   i32, run_decode, run_slots, slots_of)
+                                   i32, no_error, run_decode, run_slots, slots_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,28 @@ def test_append_to_an_empty_stack():
     assert not kp[0].any() and kp[1, 0, 3].all() and kp.sum() == 128 and torch.equal(kp, vp)
     assert stack.free_count.item() == 0 and stack.counters.item() == 0
     assert table.tolist() == [[0, 0], [1, 0]]
+
+
+@pytest.mark.parametrize("cache", ["f16", "block"])
+def test_no_tokens_and_no_rows(cache):
+    """Writes of no tokens, a decode of no rows and a prefill of empty prompts do
+    nothing."""
+    f16 = torch.float16
+    k, q = (torch.empty(0, h, 128, dtype=f16, device="cuda") for h in (2, 4))
+    kp, ks = empty_cache(4, 2, 16, 16)
+    vp, vs = empty_cache(4, 2, 16, 16)
+    stack, table = PageStack.full(4, "cuda"), i32([[-1, -1]])
+    if cache == "block":
+        ops.kv_write_fp8_block(k, k, kp, vp, ks, vs, i32([]))
+        ops.paged_attention_auto_fp8_block(q, kp, vp, ks, vs, i32(np.zeros((0, 2))), i32([]), q,
+                                           torch.empty(0, device="cuda"))
+        engine = DecodeEngine(kp, vp, 4, kv_block_scales=(ks, vs))
+    else:
+        kp, vp = (torch.full((4, 2, 16, 128), 7.0, dtype=f16, device="cuda") for _ in range(2))
+        ops.kv_write(k, k, kp, vp, i32([]))
+        engine = DecodeEngine(kp, vp, 4)
+    seq = engine.prefill(q, k, k, i32([0]), table, q, stack)
+    no_error()
+    assert seq.tolist() == [0] and stack.free_count.item() == 4 and table.tolist() == [[-1, -1]]
+    for t in (kp, vp):
+        assert (t == 7).all() if cache == "f16" else (t.view(torch.uint8) == 255).all()
