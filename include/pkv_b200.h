@@ -344,8 +344,9 @@ pkv_status pkv_paged_attention_auto_fp8_block(
  * other pointer with free_capacity 0, and is not read.  A page id that is
  * negative or too large for 32-bit slots gives slot -1 (PKV_DEVERR_PAGE_ID).
  * counters: one zeroed int32, left zero (used where free_left is free_count).
- * No buffer written may overlap cached_lens or new_lens.  Two calls that
- * overlap on the GPU must not share a stack or counters. */
+ * No buffer written may overlap another buffer of the call (but free_left may
+ * be free_count).  Two calls that overlap on the GPU must not share a stack or
+ * counters. */
 pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
                             int32_t* block_table, int32_t* slots, int32_t* cu_seqlens,
                             int32_t* seq_lens, const int32_t* free_pages,

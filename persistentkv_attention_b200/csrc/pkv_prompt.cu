@@ -252,6 +252,29 @@ pkv_status pkv_prompt_slots(const int32_t* cached_lens, const int32_t* new_lens,
     // (a length rounded up to pages fits into 32 bits too)
     if (((long long)max_pages + 1) * page_size > (1ll << 31))
         return fail_fmt(PKV_ERR_UNSUPPORTED, "max_pages * page_size exceeds 32-bit positions");
+    auto words = [](const int32_t* p, long long n) -> Range {
+        return {reinterpret_cast<const char*>(p), p != nullptr ? 4 * n : 0};
+    };
+    const bool stack = free_pages != nullptr;
+    const bool in_place = stack && free_left == free_count;
+    // what is written, the first stack ? 6 : 3 of them, then what is only read
+    const Range used[] = {words(slots, num_slots),
+                          words(cu_seqlens, B + 1ll),
+                          words(seq_lens, B),
+                          words(block_table, (long long)B * max_pages),
+                          words(free_left, stack ? 1 : 0),
+                          words(counters, stack ? 1 : 0),
+                          words(cached_lens, B),
+                          words(new_lens, B),
+                          words(free_pages, free_capacity),
+                          words(free_count, stack && !in_place ? 1 : 0)};
+    constexpr int kUsed = sizeof(used) / sizeof(used[0]);
+    for (int i = 0; i < (stack ? 6 : 3); ++i)
+        for (int j = i + 1; j < kUsed; ++j)
+            if (overlap(used[i], used[j]))
+                return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                                "the buffers that a slot map writes must not overlap each other or "
+                                "those it reads");
     int sms = 0;
     unsigned* error = nullptr;
     pkv_status st = device_state(&sms, &error);

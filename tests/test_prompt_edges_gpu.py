@@ -122,3 +122,21 @@ def test_no_tokens_and_no_rows(cache):
     assert seq.tolist() == [0] and stack.free_count.item() == 4 and table.tolist() == [[-1, -1]]
     for t in (kp, vp):
         assert (t == 7).all() if cache == "f16" else (t.view(torch.uint8) == 255).all()
+
+
+# ------------------------------------------------------------------ overlaps
+def test_slots_from_parts_of_one_buffer():
+    """Buffers that only touch, lengths that share their memory, and a stack
+    lowered in place are fine."""
+    buf = torch.zeros(200, dtype=torch.int32, device="cuda")
+    lens, cu, seq, slots = buf[0:2], buf[2:5], buf[5:7], buf[7:27]
+    table, free, count, ctr = buf[27:35].view(2, 4), buf[35:43], buf[43:44], buf[44:45]
+    lens.copy_(i32([7, 3])), free.copy_(i32(range(8))), count.fill_(8), buf[45:].fill_(9)
+    ops.prompt_slots(lens, lens, table, slots, cu, seq, free, count, count, ctr, 8)
+    no_error()
+    assert lens.tolist() == [7, 3] and cu.tolist() == [0, 7, 10] and seq.tolist() == [14, 6]
+    assert slots.tolist() == [7] + [56 + i for i in range(6)] + [3, 4, 5] + [-1] * 10
+    assert table.tolist() == [[0, 7, 0, 0], [0, 0, 0, 0]] and count.item() == 7
+    assert free.tolist() == list(range(8)) and ctr.item() == 0 and (buf[45:] == 9).all()
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        ops.prompt_slots(lens, lens, table, buf[8:28], cu, seq, free, count, count, ctr, 8)
