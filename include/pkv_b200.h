@@ -403,6 +403,18 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
                                 long long k_head_stride, long long v_stride,
                                 long long v_head_stride, pkv_dtype dtype, void* stream);
 
+/* What the write (pkv_kv_write_fp8_block where scales are given, else
+ * pkv_kv_write, block_tokens unused) and pkv_prompt_attention of T packed
+ * tokens would refuse, and an output or lse inside the cache; launches nothing.
+ * A caller that takes pages first (pkv_prompt_slots) asks before it does. */
+pkv_status pkv_prefill_check(const void* q, const void* k, const void* v, const void* output,
+                             const float* lse, const void* k_pages, const void* v_pages,
+                             const float* k_scales, const float* v_scales, int B, int T, int Hq,
+                             int Hkv, int head_dim, long long q_stride, long long q_head_stride,
+                             long long k_stride, long long k_head_stride, long long v_stride,
+                             long long v_head_stride, int physical_pages, int page_size,
+                             int block_tokens, pkv_dtype dtype);
+
 /* ---- KV append (the write side of a decode step) ----
  * Writes one new token per row into the paged pools: row b's k_new[b] /
  * v_new[b] ([B][Hkv][128], same 16-bit dtype as the pools) land at token

@@ -162,6 +162,10 @@ SIGNATURES = {
     "pkv_prompt_attention": (
         c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
                 c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, _P]),
+    "pkv_prefill_check": (
+        c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_longlong,
+                c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, c_int, c_int,
+                c_int]),
     "pkv_kv_append": (
         c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                 c_int, _P]),

@@ -106,6 +106,7 @@ bool overlap(const Range& a, const Range& b) {
 
 // K and V go to pools of their own, apart from the tokens that are read.
 pkv_status check_apart(const WriteParams& wp, int physical_pages, int elem_bytes) {
+    if (wp.T == 0) return PKV_OK;
     const long long pool = (long long)physical_pages * wp.Hkv * wp.page_size * kHeadDim * elem_bytes;
     const Range kp{reinterpret_cast<const char*>(wp.k_pages), pool};
     const Range vp{reinterpret_cast<const char*>(wp.v_pages), pool};
@@ -121,6 +122,53 @@ pkv_status grid_of(long long threads, int per_cta, unsigned* grid) {
     const long long n = (threads + per_cta - 1) / per_cta;
     if (n > INT_MAX) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many tokens for one launch");
     *grid = (unsigned)n;
+    return PKV_OK;
+}
+
+// The checks that only the 16-bit write makes; gives the grid.
+pkv_status copy_params(const WriteParams& wp, int physical_pages, unsigned* grid) {
+    const pkv_status st = check_apart(wp, physical_pages, 2);
+    if (st != PKV_OK) return st;
+    return grid_of((long long)wp.T * wp.Hkv * (kRowBytes / 16), kWriteThreads, grid);
+}
+
+// Rows of the e4m3 write's grid: its warps are (head, K or V, share of a window).
+long long block_rows(int Hkv, int split_log2) {
+    return (((2ll * Hkv) << split_log2) + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
+}
+
+// The checks that only the e4m3 write makes; fills the scales.
+pkv_status block_params(WriteParams& wp, float* k_scales, float* v_scales, int physical_pages,
+                        int block_tokens) {
+    if (k_scales == nullptr || v_scales == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must be CUDA tensors");
+    if (block_tokens <= 0 || block_tokens % 16 != 0 || wp.page_size % block_tokens != 0)
+        return fail_fmt(PKV_ERR_UNSUPPORTED,
+                        "a scale block must be a multiple of 16 tokens that divides the page; "
+                        "got %d tokens in pages of %d",
+                        block_tokens, wp.page_size);
+    // (a window is shared only while the whole grid is a few thousand warps)
+    if (block_rows(wp.Hkv, 0) > 65535)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "too many heads for one launch");
+    wp.k_scales = k_scales;
+    wp.v_scales = v_scales;
+    wp.block = block_tokens;
+    if (wp.T == 0) return PKV_OK;
+    const pkv_status st = check_apart(wp, physical_pages, 1);
+    if (st != PKV_OK) return st;
+    const long long pool = (long long)physical_pages * wp.Hkv * wp.page_size * kHeadDim;
+    const Range scales[2] = {
+        {reinterpret_cast<const char*>(k_scales), pool / kHeadDim / block_tokens * 4},
+        {reinterpret_cast<const char*>(v_scales), pool / kHeadDim / block_tokens * 4}};
+    if (overlap(scales[0], scales[1]))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must not overlap");
+    for (const Range& sc : scales)
+        if (overlap(sc, {reinterpret_cast<const char*>(wp.k_pages), pool}) ||
+            overlap(sc, {reinterpret_cast<const char*>(wp.v_pages), pool}) ||
+            overlap(sc, operand_range(wp.k, wp.T, wp.Hkv, wp.k_tok, wp.k_head)) ||
+            overlap(sc, operand_range(wp.v, wp.T, wp.Hkv, wp.v_tok, wp.v_head)))
+            return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
+                            "the scales must not overlap the pools or the tokens written");
     return PKV_OK;
 }
 
@@ -142,6 +190,85 @@ pkv_status token_map(CUtensorMap* map, const void* base, int T, int H, long long
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail_fmt(PKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return PKV_OK;
+}
+
+// Items of the launch: one per pair of query tiles and KV head's pair of heads.
+long long prompt_items(const PromptParams& pp) {
+    const int rows = pp.G == 1 ? 2 * kPmTile : kPmTile;
+    // every sequence has at most one tile that is not full
+    const long long tiles = std::min<long long>((long long)pp.Tq / rows + pp.B, pp.Tq);
+    return tiles * (pp.G == 1 ? pp.Hq : pp.Hq / 2);
+}
+
+// Shared checks of prompt attention; fills everything but the error word.  A
+// call without rows or sequences (nothing to launch) may lack any operand.
+pkv_status prompt_params(PromptParams& pp, const void* q, const void* k, const void* v,
+                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* output,
+                         float* lse, int B, int q_tokens, int k_tokens, int Hq, int Hkv,
+                         int head_dim, long long q_stride, long long q_head_stride,
+                         long long k_stride, long long k_head_stride, long long v_stride,
+                         long long v_head_stride, pkv_dtype dtype) {
+    if (q_tokens > 0 && (q == nullptr || output == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "q and output must be CUDA tensors");
+    if (k_tokens > 0 && (k == nullptr || v == nullptr))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k and v must be CUDA tensors");
+    if (cu_seqlens_q == nullptr)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "cu_seqlens_q must be a CUDA tensor");
+    if (cu_seqlens_k == nullptr) cu_seqlens_k = cu_seqlens_q;
+    if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "q has wrong dtype");
+    if (head_dim != kHeadDim)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "PersistentKV extension currently requires d=128");
+    if (Hkv <= 0) return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hkv must be positive");
+    if (Hq <= 0 || Hq % Hkv != 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hq must be divisible by Hkv");
+    const int G = Hq / Hkv;
+    if (!(G == 1 || G == 2 || G == 4 || G == 8))
+        return fail_fmt(PKV_ERR_UNSUPPORTED,
+                        "PersistentKV supports G=Hq/Hkv in {1,2,4,8}; got G=%d from Hq=%d Hkv=%d",
+                        G, Hq, Hkv);
+    if (B < 0 || q_tokens < 0 || k_tokens < 0)
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid prompt shape");
+    pkv_status st = check_strides("q", q_tokens, Hq, &q_stride, &q_head_stride);
+    if (st == PKV_OK) st = check_strides("k", k_tokens, Hkv, &k_stride, &k_head_stride);
+    if (st == PKV_OK) st = check_strides("v", k_tokens, Hkv, &v_stride, &v_head_stride);
+    if (st != PKV_OK) return st;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(output))
+        return fail_fmt(PKV_ERR_MISALIGNED, "q, k, v and output must be 16-byte aligned");
+    if (B == 0 || q_tokens == 0) return PKV_OK;
+    pp.q = static_cast<const uint8_t*>(q);
+    pp.k = static_cast<const uint8_t*>(k);
+    pp.v = static_cast<const uint8_t*>(v);
+    pp.cu_q = cu_seqlens_q;
+    pp.cu_k = cu_seqlens_k;
+    pp.out = output;
+    pp.lse = lse;
+    pp.q_tok = 2 * q_stride;
+    pp.q_head = 2 * q_head_stride;
+    pp.k_tok = 2 * k_stride;
+    pp.k_head = 2 * k_head_stride;
+    pp.v_tok = 2 * v_stride;
+    pp.v_head = 2 * v_head_stride;
+    pp.B = B;
+    pp.Tq = q_tokens;
+    pp.Tk = k_tokens;
+    pp.Hq = Hq;
+    pp.Hkv = Hkv;
+    pp.G = G;
+    pp.scale_log2 = (1.0f / sqrtf((float)kHeadDim)) * kLog2e;
+    const Range o = operand_range(output, q_tokens, Hq, (long long)Hq * kRowBytes, kRowBytes);
+    if (overlap(o, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
+        overlap(o, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
+        overlap(o, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "output must not overlap q, k or v");
+    const Range l{reinterpret_cast<const char*>(lse), lse ? (long long)q_tokens * Hq * 4 : 0};
+    if (overlap(l, o) || overlap(l, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
+        overlap(l, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
+        overlap(l, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
+        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "lse must not overlap output, q, k or v");
+    if (prompt_items(pp) > INT_MAX)
+        return fail_fmt(PKV_ERR_UNSUPPORTED, "too many tokens for one launch");
     return PKV_OK;
 }
 
@@ -176,20 +303,14 @@ pkv_status launch_prompt(const PromptParams& pp, pkv_dtype dtype, int sms, cudaS
         st = pp.Tk > 0 ? token_map(&mv, pp.v, pp.Tk, pp.Hkv, pp.v_tok, pp.v_head, dtype)
                        : token_map(&mv, pp.q, pp.Tq, pp.Hq, pp.q_tok, pp.q_head, dtype);
     if (st != PKV_OK) return st;
-    const int G = pp.G;
-    const int rows = G == 1 ? 2 * kPmTile : kPmTile;
-    // every sequence has at most one tile that is not full
-    const long long tiles = std::min<long long>((long long)pp.Tq / rows + pp.B, pp.Tq);
-    const long long items = tiles * (G == 1 ? pp.Hq : pp.Hq / 2);
+    const long long items = prompt_items(pp);
     // A cluster per item where that still leaves SMs free and each CTA gets
     // at least kPmSplitBlocks key blocks of an average sequence.
     int split = 1;
     while (split < 8 && items * split * 2 <= sms &&
            (long long)pp.Tk / pp.B >= (long long)kPmTile * kPmSplitBlocks * split * 2)
         split *= 2;
-    unsigned grid = 0;
-    st = grid_of(items * split, 1, &grid);
-    if (st != PKV_OK) return st;
+    const unsigned grid = (unsigned)(items * split);
     if (split == 1) {
         static std::atomic<unsigned long long> done{0ull};
         auto kern = pkv_prompt_mma_kernel<T, false>;
@@ -299,14 +420,12 @@ pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pag
                                  k_head_stride, v_stride, v_head_stride, physical_pages,
                                  page_size, dtype);
     if (st != PKV_OK) return st;
-    if (T == 0) return ok();
-    st = check_apart(wp, physical_pages, 2);
+    unsigned grid = 0;
+    st = copy_params(wp, physical_pages, &grid);
     if (st != PKV_OK) return st;
+    if (T == 0) return ok();
     int sms = 0;
     st = device_state(&sms, &wp.error);
-    if (st != PKV_OK) return st;
-    unsigned grid = 0;
-    st = grid_of((long long)T * Hkv * (kRowBytes / 16), kWriteThreads, &grid);
     if (st != PKV_OK) return st;
     pkv_kv_write_kernel<<<grid, kWriteThreads, 0, static_cast<cudaStream_t>(stream)>>>(wp);
     return launched("K/V write");
@@ -323,32 +442,9 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
                                  k_head_stride, v_stride, v_head_stride, physical_pages,
                                  page_size, dtype);
     if (st != PKV_OK) return st;
-    if (k_scales == nullptr || v_scales == nullptr)
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must be CUDA tensors");
-    if (block_tokens <= 0 || block_tokens % 16 != 0 || page_size % block_tokens != 0)
-        return fail_fmt(PKV_ERR_UNSUPPORTED,
-                        "a scale block must be a multiple of 16 tokens that divides the page; "
-                        "got %d tokens in pages of %d",
-                        block_tokens, page_size);
-    wp.k_scales = k_scales;
-    wp.v_scales = v_scales;
-    wp.block = block_tokens;
-    if (T == 0) return ok();
-    st = check_apart(wp, physical_pages, 1);
+    st = block_params(wp, k_scales, v_scales, physical_pages, block_tokens);
     if (st != PKV_OK) return st;
-    const long long pool = (long long)physical_pages * Hkv * page_size * kHeadDim;
-    const Range scales[2] = {
-        {reinterpret_cast<const char*>(k_scales), pool / kHeadDim / block_tokens * 4},
-        {reinterpret_cast<const char*>(v_scales), pool / kHeadDim / block_tokens * 4}};
-    if (overlap(scales[0], scales[1]))
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k_scales and v_scales must not overlap");
-    for (const Range& sc : scales)
-        if (overlap(sc, {static_cast<const char*>(k_pages), pool}) ||
-            overlap(sc, {static_cast<const char*>(v_pages), pool}) ||
-            overlap(sc, operand_range(k, T, Hkv, wp.k_tok, wp.k_head)) ||
-            overlap(sc, operand_range(v, T, Hkv, wp.v_tok, wp.v_head)))
-            return fail_fmt(PKV_ERR_INVALID_ARGUMENT,
-                            "the scales must not overlap the pools or the tokens written");
+    if (T == 0) return ok();
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
@@ -358,9 +454,7 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     while ((1 << wp.split_log2) < kRunRows &&
            (windows * 2 * Hkv << (wp.split_log2 + 1)) <= 32ll * sms)
         ++wp.split_log2;
-    const long long roles = (2ll * Hkv) << wp.split_log2;
-    const long long rows = (roles + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
-    if (rows > 65535) return fail_fmt(PKV_ERR_UNSUPPORTED, "too many heads for one launch");
+    const long long rows = block_rows(Hkv, wp.split_log2);
     const dim3 grid((unsigned)windows, (unsigned)rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PKV_DTYPE_F16)
@@ -377,71 +471,57 @@ pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,
                                 long long q_head_stride, long long k_stride,
                                 long long k_head_stride, long long v_stride,
                                 long long v_head_stride, pkv_dtype dtype, void* stream) {
-    if (q_tokens > 0 && (q == nullptr || output == nullptr))
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "q and output must be CUDA tensors");
-    if (k_tokens > 0 && (k == nullptr || v == nullptr))
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "k and v must be CUDA tensors");
-    if (cu_seqlens_q == nullptr)
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "cu_seqlens_q must be a CUDA tensor");
-    if (cu_seqlens_k == nullptr) cu_seqlens_k = cu_seqlens_q;
-    if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
-        return fail_fmt(PKV_ERR_UNSUPPORTED, "q has wrong dtype");
-    if (head_dim != kHeadDim)
-        return fail_fmt(PKV_ERR_UNSUPPORTED, "PersistentKV extension currently requires d=128");
-    if (Hkv <= 0) return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hkv must be positive");
-    if (Hq <= 0 || Hq % Hkv != 0)
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "Hq must be divisible by Hkv");
-    const int G = Hq / Hkv;
-    if (!(G == 1 || G == 2 || G == 4 || G == 8))
-        return fail_fmt(PKV_ERR_UNSUPPORTED,
-                        "PersistentKV supports G=Hq/Hkv in {1,2,4,8}; got G=%d from Hq=%d Hkv=%d",
-                        G, Hq, Hkv);
-    if (B < 0 || q_tokens < 0 || k_tokens < 0)
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "invalid prompt shape");
-    pkv_status st = check_strides("q", q_tokens, Hq, &q_stride, &q_head_stride);
-    if (st == PKV_OK) st = check_strides("k", k_tokens, Hkv, &k_stride, &k_head_stride);
-    if (st == PKV_OK) st = check_strides("v", k_tokens, Hkv, &v_stride, &v_head_stride);
-    if (st != PKV_OK) return st;
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(output))
-        return fail_fmt(PKV_ERR_MISALIGNED, "q, k, v and output must be 16-byte aligned");
-    if (B == 0 || q_tokens == 0) return ok();
     PromptParams pp;
-    pp.q = static_cast<const uint8_t*>(q);
-    pp.k = static_cast<const uint8_t*>(k);
-    pp.v = static_cast<const uint8_t*>(v);
-    pp.cu_q = cu_seqlens_q;
-    pp.cu_k = cu_seqlens_k;
-    pp.out = output;
-    pp.lse = lse;
-    pp.q_tok = 2 * q_stride;
-    pp.q_head = 2 * q_head_stride;
-    pp.k_tok = 2 * k_stride;
-    pp.k_head = 2 * k_head_stride;
-    pp.v_tok = 2 * v_stride;
-    pp.v_head = 2 * v_head_stride;
-    pp.B = B;
-    pp.Tq = q_tokens;
-    pp.Tk = k_tokens;
-    pp.Hq = Hq;
-    pp.Hkv = Hkv;
-    pp.G = G;
-    pp.scale_log2 = (1.0f / sqrtf((float)kHeadDim)) * kLog2e;
-    const Range o = operand_range(output, q_tokens, Hq, (long long)Hq * kRowBytes, kRowBytes);
-    if (overlap(o, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
-        overlap(o, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
-        overlap(o, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "output must not overlap q, k or v");
-    const Range l{reinterpret_cast<const char*>(lse), lse ? (long long)q_tokens * Hq * 4 : 0};
-    if (overlap(l, o) || overlap(l, operand_range(q, q_tokens, Hq, pp.q_tok, pp.q_head)) ||
-        overlap(l, operand_range(k, k_tokens, Hkv, pp.k_tok, pp.k_head)) ||
-        overlap(l, operand_range(v, k_tokens, Hkv, pp.v_tok, pp.v_head)))
-        return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "lse must not overlap output, q, k or v");
+    pkv_status st = prompt_params(pp, q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse, B, q_tokens,
+                                  k_tokens, Hq, Hkv, head_dim, q_stride, q_head_stride, k_stride,
+                                  k_head_stride, v_stride, v_head_stride, dtype);
+    if (st != PKV_OK) return st;
+    if (B == 0 || q_tokens == 0) return ok();
     int sms = 0;
     st = device_state(&sms, &pp.error);
     if (st != PKV_OK) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == PKV_DTYPE_F16 ? launch_prompt<__half>(pp, dtype, sms, s)
                                   : launch_prompt<__nv_bfloat16>(pp, dtype, sms, s);
+}
+
+pkv_status pkv_prefill_check(const void* q, const void* k, const void* v, const void* output,
+                             const float* lse, const void* k_pages, const void* v_pages,
+                             const float* k_scales, const float* v_scales, int B, int T, int Hq,
+                             int Hkv, int head_dim, long long q_stride, long long q_head_stride,
+                             long long k_stride, long long k_head_stride, long long v_stride,
+                             long long v_head_stride, int physical_pages, int page_size,
+                             int block_tokens, pkv_dtype dtype) {
+    // (slots and cu_seqlens are the caller's to come: any address stands in)
+    const int32_t* some = static_cast<const int32_t*>(k_pages);
+    const bool scaled = k_scales != nullptr || v_scales != nullptr;
+    WriteParams wp;
+    pkv_status st = write_params(wp, k, v, const_cast<void*>(k_pages), const_cast<void*>(v_pages),
+                                 some, T, Hkv, head_dim, k_stride, k_head_stride, v_stride,
+                                 v_head_stride, physical_pages, page_size, dtype);
+    unsigned grid = 0;
+    if (st == PKV_OK)
+        st = scaled ? block_params(wp, const_cast<float*>(k_scales), const_cast<float*>(v_scales),
+                                   physical_pages, block_tokens)
+                    : copy_params(wp, physical_pages, &grid);
+    PromptParams pp;
+    if (st == PKV_OK)
+        st = prompt_params(pp, q, k, v, some, some, const_cast<void*>(output),
+                           const_cast<float*>(lse), B, T, T, Hq, Hkv, head_dim, q_stride,
+                           q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, dtype);
+    if (st != PKV_OK) return st;
+    const long long pool = (long long)physical_pages * Hkv * page_size * kHeadDim;
+    const long long scale_bytes = scaled ? pool / kHeadDim / block_tokens * 4 : 0;
+    const Range cache[4] = {{static_cast<const char*>(k_pages), scaled ? pool : 2 * pool},
+                            {static_cast<const char*>(v_pages), scaled ? pool : 2 * pool},
+                            {reinterpret_cast<const char*>(k_scales), scale_bytes},
+                            {reinterpret_cast<const char*>(v_scales), scale_bytes}};
+    const long long rows = (long long)T * Hq;
+    for (const Range& c : cache)
+        if (overlap(c, {static_cast<const char*>(output), rows * kRowBytes}) ||
+            overlap(c, {reinterpret_cast<const char*>(lse), lse != nullptr ? rows * 4 : 0}))
+            return fail_fmt(PKV_ERR_INVALID_ARGUMENT, "output and lse must not overlap the cache");
+    return ok();
 }
 
 }  // extern "C"

@@ -901,6 +901,25 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, output, lse=None) -> N
         qst[0], qst[1], kst[0], kst[1], vst[0], vst[1], _DTYPES[dt], _stream_of(dev)))
 
 
+def _check_prefill(q, k, v, cu_seqlens, slots, output, lse, k_pages, v_pages, scales) -> None:
+    """Everything that the write (``kv_write_fp8_block`` with ``scales``, else
+    ``kv_write``) and ``prompt_attention`` of one batch of prompts would refuse."""
+    _check_prompt(q, k, v, cu_seqlens, None, output, lse)
+    _check_write(k, v, k_pages, v_pages, slots, k.dtype if scales is None else torch.float8_e4m3fn)
+    if q.size(0) != k.size(0):
+        raise RuntimeError("q, k and v must hold the same tokens")
+    ks, vs = (None, None) if scales is None else scales
+    block = 0 if scales is None else _check_block_scales(k_pages, ks, vs)
+    _check_current_device(k_pages, v_pages, slots, ks, vs)
+    _native.check(_native.load().pkv_prefill_check(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), output.data_ptr(),
+        None if lse is None else lse.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr(),
+        cu_seqlens.size(0) - 1, q.size(0), q.size(1), k.size(1), HEAD_DIM, q.stride(0), q.stride(1),
+        k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.size(0), k_pages.size(2), block,
+        _DTYPES[q.dtype]))
+
+
 def auto_workspace_bytes(batch: int, hq: int, hkv: int, sm_count: int = 0) -> int:
     """Workspace of ``paged_attention_auto`` (sm_count 0: the current device)."""
     return int(_native.load().pkv_auto_workspace_bytes(batch, hq, hkv, sm_count))

@@ -286,10 +286,9 @@ class DecodeEngine:
         i32 = dict(dtype=torch.int32, device=self.device)
         slots, cu = torch.empty(k.size(0), **i32), torch.empty(b + 1, **i32)
         seq_lens = torch.empty(b, **i32)
-        # wrong tensors are refused before pages are taken
-        ops._check_prompt(q, k, v, cu, None, out, lse)
-        ops._check_write(k, v, self.k_pages, self.v_pages, slots,
-                         self.k_pages.dtype if self.kv8 else k.dtype)
+        # what the calls after the slot map would refuse is refused before pages are taken
+        ops._check_prefill(q, k, v, cu, slots, out, lse, self.k_pages, self.v_pages,
+                           self.kv_block_scales)
         ops.prompt_slots(torch.zeros(b, **i32), new_lens, block_table, slots, cu, seq_lens,
                          *((None,) * 4 if stack is None else
                            (stack.free_pages, stack.free_count, stack.free_count, stack.counters)),

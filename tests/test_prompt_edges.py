@@ -41,3 +41,43 @@ APART = dict(cached=1 << 20, new=2 << 20, table=3 << 20, slots=4 << 20, cu=5 << 
 def test_slots_refuses_overlaps(lib, kw):
     assert slots(lib, **{**APART, **kw}) == 1
     assert b"must not overlap" in lib.pkv_last_error_message()
+
+
+# ------------------------------------------------------------------ prefill
+def prefill(lib, **kw):
+    """40 tokens of 32 / 8 heads, 64 pages of 16: each operand 256 MB from the next."""
+    a = dict(q=1 << 28, k=2 << 28, v=3 << 28, out=4 << 28, lse=5 << 28, kp=6 << 28, vp=7 << 28,
+             ks=None, vs=None, B=2, T=40, Hq=32, Hkv=8, d=128, qt=4096, qh=128, kt=1024, kh=128,
+             vt=1024, vh=128, P=64, page=16, block=0, dtype=0)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.pkv_prefill_check(*a.values())
+
+
+SCALED = dict(ks=8 << 28, vs=9 << 28, block=16)
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(), 0, ""), (dict(lse=None), 0, ""), (dict(T=0, q=None, k=None, v=None, out=None), 0, ""),
+    (dict(qt=4100), 3, "q strides"), (dict(kt=1028), 3, "k strides"), (dict(vh=-128), 3, "v strides"),
+    (dict(k=(2 << 28) + 2), 3, "16-byte"), (dict(q=(1 << 28) + 8), 3, "16-byte"),
+    (dict(out=(4 << 28) + 4), 3, "16-byte"), (dict(out=1 << 28), 1, "output must not overlap"),
+    (dict(lse=(4 << 28) + 4), 1, "lse must not overlap"), (dict(k=6 << 28), 1, "must not overlap"),
+    (dict(vp=6 << 28), 1, "must not overlap"), (dict(Hq=24), 2, "G=3"), (dict(d=64), 2, "d=128"),
+    (dict(P=1 << 28), 2, "32-bit slots"), (dict(dtype=4), 2, "dtype"), (dict(kp=None), 1, "k_pages"),
+    (dict(out=(6 << 28) + 4096), 1, "overlap the cache"), (dict(lse=7 << 28), 1, "overlap the cache"),
+    (dict(T=1 << 30, Hq=8, Hkv=1, qt=8, kt=8, vt=8), 1, "must not overlap")])
+def test_prefill_check(lib, scaled, kw, status, msg):
+    assert prefill(lib, **{**(SCALED if scaled else {}), **kw}) == status
+    assert msg in lib.pkv_last_error_message().decode()
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(vs=None), 1, "k_scales and v_scales"), (dict(block=8), 2, "multiple of 16"),
+    (dict(vs=8 << 28), 1, "must not overlap"), (dict(ks=(6 << 28) + 64), 1, "must not overlap"),
+    (dict(lse=8 << 28), 1, "overlap the cache"),
+    (dict(Hkv=1 << 18, Hq=1 << 18), 2, "too many heads")])
+def test_prefill_check_of_block_scales(lib, kw, status, msg):
+    assert prefill(lib, **{**SCALED, **kw}) == status
+    assert msg in lib.pkv_last_error_message().decode()

@@ -140,3 +140,51 @@ def test_slots_from_parts_of_one_buffer():
     assert free.tolist() == list(range(8)) and ctr.item() == 0 and (buf[45:] == 9).all()
     with pytest.raises(RuntimeError, match="must not overlap"):
         ops.prompt_slots(lens, lens, table, buf[8:28], cu, seq, free, count, count, ctr, 8)
+
+
+# ------------------------------------------------------------------ prefill
+@pytest.mark.parametrize("cache", ["f16", "block"])
+def test_prefill_takes_no_pages_for_what_it_refuses(cache):
+    """Strides, alignment, overlaps and scales that only the calls behind the slot
+    map would refuse."""
+    f16 = torch.float16
+    if cache == "block":
+        kp, ks = empty_cache(4, 2, 16, 16)
+        vp, vs = empty_cache(4, 2, 16, 16)
+        scales = dict(kv_block_scales=(ks, vs))
+    else:
+        kp, vp = (torch.zeros(4, 2, 16, 128, dtype=f16, device="cuda") for _ in range(2))
+        scales = {}
+    engine = DecodeEngine(kp, vp, 4, **scales)
+    q, k, v = (torch.randn(20, h, 128, device="cuda").to(f16) for h in (4, 2, 2))
+    out, lse = torch.zeros_like(q), torch.zeros(20, 4, device="cuda")
+    flat = torch.zeros(1 << 16, dtype=f16, device="cuda")
+    odd = flat.as_strided((20, 2, 128), (260, 128, 1))
+    off = flat.as_strided((20, 2, 128), (256, 128, 1), 4)
+    whole = kp.view(torch.uint8).view(-1).view(f16)      # the pool's memory
+    stack, table, new = PageStack.full(4, "cuda"), i32([[-1, -1]]), i32([20])
+    bad = [(engine, a) for a in (
+        (q, odd, v, out, None), (q, k, off, out, None), (q, k, v, q, None), (q[:19], k, v, out[:19], None),
+        (flat.as_strided((20, 4, 128), (516, 128, 1)), k, v, out, None),
+        (q, k, v, out, out.view(-1)[:160].view(torch.float32).view(20, 4)),
+        (q, whole[:5120].view(20, 2, 128), v, out, None),
+        (q, k, v, whole[:8192].view(16, 4, 128), None),
+        (q[:16], k[:16], v[:16], whole[:8192].view(16, 4, 128), None))]
+    if cache == "block":
+        for a, b in ((ks, ks), (ks, torch.zeros(4, 2, 2, device="cuda")), (ks.half(), vs.half()),
+                     (ks[:3], vs[:3])):
+            bad.append((DecodeEngine(kp, vp, 4, kv_block_scales=(a, b)), (q, k, v, out, None)))
+    else:
+        bad.append((DecodeEngine(kp, kp, 4), (q, k, v, out, None)))
+        bad.append((DecodeEngine(kp, vp[:3], 4), (q, k, v, out, None)))
+    kept = [t.view(torch.uint8).clone() for t in (kp, vp)]
+    for eng, (a, b, c, o, l) in bad:
+        with pytest.raises(RuntimeError):
+            eng.prefill(a, b, c, new, table, o, stack, l)
+        assert stack.free_count.item() == 4 and table.tolist() == [[-1, -1]]
+    no_error()
+    for t, was in zip((kp, vp), kept):
+        assert torch.equal(t.view(torch.uint8), was)
+    assert engine.prefill(q, k, v, new, table, out, stack, lse).tolist() == [20]
+    no_error()
+    assert stack.free_count.item() == 2 and table.tolist() == [[0, 1]]
