@@ -303,8 +303,8 @@ pkv_status pkv_paged_attention_auto_fp8(
  * K = k_scales[p][h][t / block_tokens] * value, V likewise; scales are
  * [P][Hkv][page_size / block_tokens], block_tokens a multiple of 16 that
  * divides page_size.  A scale is positive and finite, or zero for a block of
- * zeros; a V scale below 2^-60 counts as 2^-60.  q and output are fp16 or bf16
- * (dtype).  Pages and scales of tokens past a row's length are never used,
+ * zeros; those of one row may be any powers of two apart.  q and output are
+ * fp16 or bf16 (dtype).  Pages and scales of tokens past a row's length are never used,
  * whatever they hold.  No counterpart in the reference. */
 pkv_status pkv_paged_attention_auto_fp8_block(
     const void* q_source, const void* k_pages, const void* v_pages, const float* k_scales,

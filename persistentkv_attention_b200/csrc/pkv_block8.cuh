@@ -48,8 +48,12 @@ struct B8Lookups {
 // math falls behind HBM (64 rows up to 32768 tokens: 197 us, two threads 175 us).
 constexpr int kB8Threads = kThreads + 32;
 
-// V scales below this count as this.
-constexpr float kB8LeastScale = 0x1p-60f;
+// The sum is in 32 bits and may grow further before its reference moves.
+constexpr float kB8LazySum = 32.0f;
+// A state that leaves the CTA refers to the largest score or, where V scales are
+// beyond this many powers of two, to the largest contribution less it, so that
+// its accumulators stay far from fp32's largest.
+constexpr float kB8Headroom = 60.0f;
 
 template <int G, int NSLOTS>
 constexpr size_t block8_smem_bytes() {
@@ -90,13 +94,14 @@ __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, b
 // streams the row pieces of group g for one KV head, one producer warp and
 // four consumer warps, every 32-token stage to one warp.
 //
-// Mathematics.  With s_t the scaled score, b_t the V scale of token t's block
-// and p_t = exp(s_t + ln b_t - m):  O = sum p_t v_t / sum p_t / b_t, v_t the raw
-// e4m3 values.  So a V scale costs one add in a weight's exponent and one
-// factor in the sum, never touches the accumulators, and the running maximum
-// is that of a token's contribution s_t + ln b_t, so no block's scale can
-// push another's weights out of fp16's range.  A K scale is a factor of its
-// 16 tokens' scores.
+// Mathematics.  With s_t the scaled score, b_t the V scale of token t's block and
+// v_t the raw e4m3 values:  O = sum e^s_t b_t v_t / sum e^s_t.  A V scale costs
+// one add in a weight's exponent (p_t = exp(s_t + ln b_t - m)) and never touches
+// the accumulators, and their running maximum m is that of a token's contribution
+// s_t + ln b_t, so no block's scale can push another's weights out of fp16's
+// range.  The sum has a reference of its own, the largest score, since weights
+// that hold b_t say nothing about it once scales are 2^126 apart.  A K scale is a
+// factor of its 16 tokens' scores.
 //
 // Both products run as mma.sync m16n8k16 on fp16 (every e4m3 value is exact in
 // it), 16 tokens x 8 heads and 128 dims x 8 heads.  A lane's 16-byte loads are
@@ -495,7 +500,8 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
         }
         const int n_stages = aborted ? 0 : ceil_div_i(it.tok_end - it.tok_begin, kB8Tokens);
 
-        float m_run[2] = {-INFINITY, -INFINITY};
+        float m_run[2] = {-INFINITY, -INFINITY};  // what weights refer to, log2
+        float m_sum[2] = {-INFINITY, -INFINITY};  // what this lane's sum refers to
         float l_run[2] = {0.f, 0.f};
         float acc[8][4];
 #pragma unroll
@@ -562,7 +568,8 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
             if (lane == 0) mbar_arrive(&empty_bar[slot]);
 
             // ---- S^T: 2 x [16 tokens x 8 heads]
-            float sc[2][4];
+            float raw[2][4];  // scores, log2
+            float lg[2];      // log2 of the parts' V scales
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -581,34 +588,38 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
                 }
                 const float ks = i == 0 ? scales.x : scales.y;
                 const float vs = i == 0 ? scales.z : scales.w;
-                // a block of zeros (scale 0) still counts in the sum, as one of scale
-                // 2^-60: its weights stay 66 powers of two above fp32's least
-                const float lg = vs < kB8LeastScale ? -60.f : fast_log2(vs);
+                // -inf for a block of zeros; that of a part behind the row's end may be
+                // anything
+                lg[i] = 16 * i < valid ? fast_log2(vs) : 0.f;
                 const float f0 = qs[0] * ks, f1 = qs[1] * ks;
                 if (ks == 0.f) c[0] = c[1] = c[2] = c[3] = 0.f;  // K = 0, whatever the codes
                 const bool ok0 = 16 * i + g8 < valid, ok1 = 16 * i + g8 + 8 < valid;
-                sc[i][0] = ok0 ? fmaf(c[0], f0, lg) : -INFINITY;
-                sc[i][1] = ok0 ? fmaf(c[1], f1, lg) : -INFINITY;
-                sc[i][2] = ok1 ? fmaf(c[2], f0, lg) : -INFINITY;
-                sc[i][3] = ok1 ? fmaf(c[3], f1, lg) : -INFINITY;
+                raw[i][0] = ok0 ? c[0] * f0 : -INFINITY;
+                raw[i][1] = ok0 ? c[1] * f1 : -INFINITY;
+                raw[i][2] = ok1 ? c[2] * f0 : -INFINITY;
+                raw[i][3] = ok1 ? c[3] * f1 : -INFINITY;
             }
-            // ---- running maximum (log2 domain) of heads 2 t4 and 2 t4 + 1
-            float top[2];
+            // ---- running maxima (log2 domain) of heads 2 t4 and 2 t4 + 1: of the
+            // contributions over the warp, of the scores for this lane's sum
+            float top[2], largest[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float mx = fmaxf(fmaxf(sc[0][h], sc[0][2 + h]), fmaxf(sc[1][h], sc[1][2 + h]));
+                const float a = fmaxf(raw[0][h], raw[0][2 + h]);
+                const float b = fmaxf(raw[1][h], raw[1][2 + h]);
+                largest[h] = fmaxf(a, b);
+                float mx = fmaxf(a + lg[0], b + lg[1]);
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 top[h] = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             }
             const bool move0 = top[0] - m_run[0] > kB8Lazy, move1 = top[1] - m_run[1] > kB8Lazy;
-            if (__any_sync(0xffffffffu, move0 || move1)) {
+            const bool grow0 = largest[0] - m_sum[0] > kB8LazySum;
+            const bool grow1 = largest[1] - m_sum[1] > kB8LazySum;
+            if (__any_sync(0xffffffffu, move0 || move1 || grow0 || grow1)) {
                 const float c0 = move0 ? fast_exp2(m_run[0] - top[0]) : 1.f;
                 const float c1 = move1 ? fast_exp2(m_run[1] - top[1]) : 1.f;
                 if (move0) m_run[0] = top[0];
                 if (move1) m_run[1] = top[1];
-                l_run[0] *= c0;
-                l_run[1] *= c1;
 #pragma unroll
                 for (int mt = 0; mt < 8; ++mt) {
                     acc[mt][0] *= c0;
@@ -616,23 +627,30 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
                     acc[mt][2] *= c0;
                     acc[mt][3] *= c1;
                 }
+                if (grow0) {
+                    l_run[0] *= fast_exp2(m_sum[0] - largest[0]);
+                    m_sum[0] = largest[0];
+                }
+                if (grow1) {
+                    l_run[1] *= fast_exp2(m_sum[1] - largest[1]);
+                    m_sum[1] = largest[1];
+                }
             }
             // ---- weights, and O^T[128 x 8 heads] += V^T . P^T
             const float b0 = m_run[0] == -INFINITY ? 0.f : m_run[0];
             const float b1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+            const float r0 = m_sum[0] == -INFINITY ? 0.f : m_sum[0];
+            const float r1 = m_sum[1] == -INFINITY ? 0.f : m_sum[1];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float vs = i == 0 ? scales.z : scales.w;
-                // (a masked block's scale may be anything: fmaxf drops a NaN, and a
-                // weight of 0 must not meet an infinity)
-                const float inv = 1.f / fmaxf(vs, kB8LeastScale);
                 float pr[4];
-                pr[0] = fast_exp2(sc[i][0] - b0);
-                pr[1] = fast_exp2(sc[i][1] - b1);
-                pr[2] = fast_exp2(sc[i][2] - b0);
-                pr[3] = fast_exp2(sc[i][3] - b1);
-                l_run[0] = fmaf(pr[0] + pr[2], inv, l_run[0]);
-                l_run[1] = fmaf(pr[1] + pr[3], inv, l_run[1]);
+                const float u0 = lg[i] - b0, u1 = lg[i] - b1;
+                pr[0] = fast_exp2(raw[i][0] + u0);
+                pr[1] = fast_exp2(raw[i][1] + u1);
+                pr[2] = fast_exp2(raw[i][2] + u0);
+                pr[3] = fast_exp2(raw[i][3] + u1);
+                l_run[0] += fast_exp2(raw[i][0] - r0) + fast_exp2(raw[i][2] - r0);
+                l_run[1] += fast_exp2(raw[i][1] - r1) + fast_exp2(raw[i][3] - r1);
                 const uint32_t pb0 = movmatrix_trans(ElemOps<__half>::pack(pr[0], pr[1]));
                 const uint32_t pb1 = movmatrix_trans(ElemOps<__half>::pack(pr[2], pr[3]));
                 // chunk g8 holds the dims 16 g8 + 2 mt + (0, 1) of output tile mt's rows
@@ -662,11 +680,26 @@ __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
         float* mbuf = s_merge + buf * DecodeSmem<G>::kMergeFloats;
         float* mstat = s_mstat + buf * kConsumerWarps * 8;
         float* lstat = s_lstat + buf * kConsumerWarps * 8;
+        // one reference for the warp's sums and accumulators (a sum of NaN keeps
+        // the reference -inf and stays)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            float m = m_sum[h];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            m = fmaxf(m, m_run[h] - kB8Headroom);
+            if (m_sum[h] != -INFINITY) l_run[h] *= fast_exp2(m_sum[h] - m);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 4);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 8);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 16);
+            const float f = m == -INFINITY ? 1.f : fast_exp2(m_run[h] - m);
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                acc[mt][h] *= f;
+                acc[mt][2 + h] *= f;
+            }
+            m_run[h] = m;
         }
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {

@@ -58,6 +58,43 @@ def test_block_write_of_blocks_of_odd_multiples(page, block, dtype):
         at += n
 
 
+# ------------------------------------------------------------------ scales far apart
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("far", [(100, None), (None, 100), (120, -24), (-24, 120), (90, -130, 3),
+                                 (None, -140, None), (126, 0, None, -148, 60)])
+def test_decode_v_scales_any_powers_of_two_apart(far, fused):
+    """Blocks whose V scales are 2^a, 2^b, ... in turn (None: a block of zeros),
+    beyond fp32's exponents apart, every token about as likely as the others: each
+    counts in the sum.  Rows in one piece, in pieces of a few blocks, and blocks
+    in runs, so that pieces and warps hold scales of one kind."""
+    lens, page = [16 * 3 + 5, 16 * 40, 16 * 200 + 9, 7], 16
+    for run in (1, 2, 25):
+        q, kp, ks, vp, vs, table = decode_case(lens, 4, 1, page, 16, "bf16", seed=11, spread=0.0)
+        codes = vp.view(torch.uint8)
+        codes[(codes & 127) == 127] = 0      # (slots of no token)
+        vs.fill_(1.0)
+        for b, n in enumerate(lens):
+            for j in range(-(-n // page)):
+                power = far[(j // run) % len(far)]
+                vs[table[b, j], 0, 0] = 0.0 if power is None else 2.0 ** power
+        vs = vs.contiguous()
+        got = run_decode(q, kp, ks, vp, vs, table, lens, fused=fused)
+        check_decode(got, q, kp, ks, vp, vs, table, lens, "bf16")
+
+
+def test_decode_v_scales_all_small_or_large():
+    """A common power of two of all V scales is one of the output."""
+    lens = [16 * 30 + 3, 9]
+    q, kp, ks, vp, vs, table = decode_case(lens, 4, 2, 16, 16, "bf16", seed=12)
+    for power in (-140, -100, -60, 60, 110):
+        got = run_decode(q, kp, ks, vp, (vs.double() * 2.0 ** power).float(), table, lens)
+        if power == -140:      # (scales and outputs near fp32's least)
+            assert got.isfinite().all() and (got.double().abs() <= 2.0 ** -110).all()
+            continue
+        back = (got.double() * 2.0 ** -power).to(torch.bfloat16)
+        check_decode(back, q, kp, ks, vp, vs, table, lens, "bf16")
+
+
 # ------------------------------------------------------------------ nothing there
 @pytest.mark.parametrize("in_place", [False, True])
 def test_slots_of_an_empty_stack(in_place):
