@@ -389,10 +389,13 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
  * row that sees none gives zeros.  q [q_tokens][Hq][128], k / v
  * [k_tokens][Hkv][128] with the given strides (elements, multiples of 8),
  * output [q_tokens][Hq][128] contiguous, apart from the inputs; softmax scale
- * 1 / sqrt(128).  lse (or NULL, apart from all): [q_tokens][Hq] natural log of each row's sum of exponentials,
- * -inf for a row that sees no key.  Rows of no sequence are left as they
- * were, and a row's result depends on no key that it does not see, whatever
- * those hold.  A sequence whose ranges lie outside the tokens or run backwards
+ * 1 / sqrt(128).  lse (or NULL, apart from all): [q_tokens][Hq] natural log of
+ * each row's sum of exponentials, -inf for a row that sees no key.  Rows of no
+ * sequence are left as they were, and a row's result depends on no key that it
+ * does not see, whatever those hold.  An infinity or NaN among the V that a row
+ * sees makes that dimension of its output one.  Sums of weights (at most 1)
+ * times V are in 32 bits: bf16 values above 2^128 divided by the number of keys
+ * may overflow.  A sequence whose ranges lie outside the tokens or run backwards
  * is skipped and sets PKV_DEVERR_INDEX; the others' rows are computed only if
  * every range is in order. */
 pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,

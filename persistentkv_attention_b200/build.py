@@ -34,7 +34,7 @@ SOURCES = ["pkv_api.cu", "pkv_inst_f16_cpasync.cu", "pkv_inst_f16_tma.cu",
            "pkv_inst_bf16_cpasync.cu", "pkv_inst_bf16_tma.cu", "pkv_inst_e4m3.cu",
            "pkv_block8.cu", "pkv_prompt.cu", "pkv_sched.cpp", "pkv_engine.cpp"]
 HEADERS = ["pkv_device.cuh", "pkv_kernels.cuh", "pkv_aux_kernels.cuh", "pkv_launch.cuh",
-           "pkv_internal.h", "pkv_block8.cuh", "pkv_cache_kernels.cuh", "pkv_prompt_kernels.cuh",
+           "pkv_internal.h", "pkv_block8.cuh", "pkv_cache_kernels.cuh",
            "pkv_prompt_mma.cuh", "pkv_tcgen05.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden"]

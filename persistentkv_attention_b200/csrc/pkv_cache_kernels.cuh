@@ -278,27 +278,6 @@ __device__ __forceinline__ float block_scale(float amax) {
     return __uint_as_float((unsigned)(e + 127) << 23);
 }
 
-template <typename T>
-__device__ __forceinline__ float2 to_float2(uint32_t x);
-template <>
-__device__ __forceinline__ float2 to_float2<__half>(uint32_t x) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&x));
-}
-template <>
-__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t x) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
-}
-
-// The magnitude bits of 16-bit floats order as integers; the first that is not
-// finite:
-template <typename T>
-constexpr unsigned kInf16 = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-
-template <typename T>
-__device__ __forceinline__ float from_bits16(unsigned bits) {
-    return to_float2<T>(bits).x;
-}
-
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }

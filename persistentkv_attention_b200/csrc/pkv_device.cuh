@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace pkv {
 
 constexpr int kHeadDim = 128;        // reference: kernels/persistentkv_attention.cuh:26
@@ -267,12 +269,39 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// ---------------------------------------------------------------- 16-bit values
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t x);
+template <>
+__device__ __forceinline__ float2 to_float2<__half>(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+template <>
+__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t x) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+}
+
+// The magnitude bits of 16-bit floats order as integers; the first that is not
+// finite:
+template <typename T>
+constexpr unsigned kInf16 = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+
+template <typename T>
+__device__ __forceinline__ float from_bits16(unsigned bits) {
+    return to_float2<T>(bits).x;
+}
+
 template <typename T>
 struct ElemOps;
 
 template <>
 struct ElemOps<__half> {
     static constexpr bool kSplitP = false;
+    using Pair = __half2;
+    // 0 * (two values) + c
+    static __device__ __forceinline__ Pair zero_times(uint32_t x, Pair c) {
+        return __hfma2(*reinterpret_cast<const Pair*>(&x), __float2half2_rn(0.f), c);
+    }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1) {
         asm(
@@ -291,6 +320,10 @@ struct ElemOps<__half> {
 template <>
 struct ElemOps<__nv_bfloat16> {
     static constexpr bool kSplitP = true;
+    using Pair = __nv_bfloat162;
+    static __device__ __forceinline__ Pair zero_times(uint32_t x, Pair c) {
+        return __hfma2(*reinterpret_cast<const Pair*>(&x), __float2bfloat162_rn(0.f), c);
+    }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1) {
         asm(

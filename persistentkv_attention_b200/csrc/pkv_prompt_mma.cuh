@@ -2,36 +2,55 @@
 // tensor cores.  Included by pkv_prompt.cu only.
 #pragma once
 
-#include "pkv_prompt_kernels.cuh"
 #include "pkv_tcgen05.cuh"
 
 namespace pkv {
+
+struct PromptParams {
+    const uint8_t* q;  // [Tq][Hq][128], token / head strides in bytes
+    const uint8_t* k;  // [Tk][Hkv][128]
+    const uint8_t* v;
+    const int32_t* cu_q;  // [B + 1]
+    const int32_t* cu_k;  // [B + 1]
+    void* out;            // [Tq][Hq][128] contiguous
+    float* lse;           // [Tq][Hq] or null
+    unsigned* error;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    int B, Tq, Tk, Hq, Hkv, G;
+    float scale_log2;
+};
 
 constexpr int kPmTile = 128;                     // query rows of a tile, keys of a block
 constexpr int kPmTileBytes = kPmTile * kRowBytes;  // 32 KB: two 64-element halves of 16 KB
 constexpr int kPmHalfBytes = kPmTileBytes / 2;
 constexpr int kPmStages = 4;                     // K/V tiles in flight
 // 8 softmax warps (tile, 32 rows each), then one warp each for the products,
-// the copies and the schedule, and one that looks the ranges over.
+// the copies and the schedule (and the V tiles that hold keys which not every row
+// sees), and one that looks the ranges over.
 constexpr int kPmSoftmaxWarps = 8;
 constexpr int kPmMmaWarp = 8, kPmLoadWarp = 9, kPmPlanWarp = 10, kPmCheckWarp = 11;
 constexpr int kPmThreads = 384;
 constexpr int kPmParts = 4;  // parts of a block's weights, 32 keys each, handed over one by one
 constexpr int kPmStageOut = 32 * 128;  // a softmax warp's 32 rows x 64 output dims
 constexpr size_t kPmSmemBytes = 1024 + (size_t)(2 + kPmStages) * kPmTileBytes +
-                                kPmSoftmaxWarps * kPmStageOut + 512;
+                                kPmSoftmaxWarps * kPmStageOut + 640;
 // TMEM columns: scores of tile t at 128 t (its weights, 16 bit, in the first
 // 64 of them), output of tile t at 256 + 128 t.
 constexpr uint32_t kPmTmemColumns = 512;  // all there are
 // The running maximum that weights refer to is raised, and the output
 // rescaled, only when a row's maximum has grown by more than this many powers
-// of two; the division by the sum at the end takes the factor out again.  Weights
-// stay below 2^14 (fp16 reaches 2^16) or 2^32 (bf16 has fp32's range, and 2^32
-// leaves the sums all but 2^-95 of it), and a weight's relative rounding is the
-// same at any size.  With 2^8 every fourth block of a 16384-token prompt had
-// a row that moved, at about 1400 cycles each.
+// of two; the division by the sum at the end takes the factor out again.  fp16
+// weights stay below 2^14 (the type reaches 2^16); the largest is 1 at least, and
+// those below 2^-14 are rounded to 2^-25 of it.  bf16 has fp32's range: the
+// reference lies kPmLift above the running maximum, so that weights stay below 1 and
+// no sum of weights times V overflows that would not with weights of at most 1; a
+// weight's relative rounding is the same at any size.
+// With 2^8 every fourth block of a 16384-token prompt had a row that moved, at
+// about 1400 cycles each.
 template <typename T>
 constexpr float kPmLazy = std::is_same<T, __half>::value ? 14.0f : 32.0f;
+template <typename T>
+constexpr float kPmLift = std::is_same<T, __half>::value ? 0.0f : 32.0f;
 
 // One item of work: two query tiles that read the same keys.
 struct alignas(16) PmWork {
@@ -40,7 +59,7 @@ struct alignas(16) PmWork {
     int head0, kvh, n_tiles;
     int first, n_blocks;    // this CTA's key blocks
     int tail;               // keys of the last of them
-    int pad;
+    int clear;              // blocks before this one hold only keys that every row sees
     // keys that row i of the sequence sees
     __device__ __forceinline__ int visible(int i) const {
         return max(0, min(lk, i + 1 + lk - lq));
@@ -56,10 +75,12 @@ struct PmShared {
     uint64_t work_full[kPmWorks], work_empty[kPmWorks], launch_bar, issued;
     uint64_t q_full, q_empty, kv_full[kPmStages], kv_empty[kPmStages];
     uint64_t s_full[2], p_full[2][kPmParts], o_full[2], o_empty[2], drained;
+    uint64_t look[2], clean[2];  // of the two V stages
+    int dropped[kPmWorks];       // the item's V had values that were taken out
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(PmShared) <= 512, "prompt CTA's shared state");
+static_assert(sizeof(PmShared) <= 640, "prompt CTA's shared state");
 
 __device__ __forceinline__ int pm_rows_per_item(int G) { return G == 1 ? 2 * kPmTile : kPmTile; }
 
@@ -81,6 +102,7 @@ __device__ __forceinline__ void pm_item(const PromptParams& p, PmWork& w, int gr
         w.n_blocks = all * (rank + 1) / n - w.first;
         if (w.first + w.n_blocks < all) w.tail = kPmTile;
     }
+    w.clear = max(0, w.visible(w.row0) / kPmTile - w.first);
 }
 
 // Whole warp: the query tile number `rank`, counted from the end over all
@@ -169,6 +191,103 @@ __device__ __forceinline__ bool pm_next(const PromptParams& p, PmShared* sh, uin
     return true;
 }
 
+// A key's V that holds an infinity or NaN reaches a row that does not see the key
+// all the same, through a product with a weight of 0.  So such values are taken out
+// of the tiles whose keys not every row sees (`clear` and later), and come back
+// here, to the rows that do see them: output rows [row, row_end) of the sequence,
+// already written, get the sum of the values taken out among their keys from
+// `key` on.  Whole warp, lane l dims 4l .. 4l + 3.
+template <typename T>
+__device__ __forceinline__ void pm_restore(const PromptParams& p, const PmWork& it, int head,
+                                           int key, int row, int row_end) {
+    const int lane = threadIdx.x & 31;
+    const uint8_t* v = p.v + it.k0 * p.v_tok + it.kvh * p.v_head;
+    auto load = [&](int j) {
+        return __ldg(reinterpret_cast<const uint2*>(v + (size_t)j * p.v_tok) + lane);
+    };
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](uint2 u) {
+        const unsigned b[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((b[i] & 0x7fffu) >= kInf16<T>) sum[i] += from_bits16<T>(b[i]);
+    };
+    for (; row < row_end; ++row) {
+        const int n = it.visible(row);
+        for (; key + 8 <= n; key += 8) {
+            uint2 u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = load(key + i);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add(u[i]);
+        }
+        for (; key < n; ++key) add(load(key));
+        // (an infinity or NaN is no zero)
+        if (sum[0] != 0.f || sum[1] != 0.f || sum[2] != 0.f || sum[3] != 0.f) {
+            uint2* at = reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) +
+                                                 ((size_t)(it.q0 + row) * p.Hq + head) * kHeadDim) +
+                        lane;
+            const uint2 o = *at;
+            const float2 a = to_float2<T>(o.x), b = to_float2<T>(o.y);
+            *at = make_uint2(ElemOps<T>::pack(a.x + sum[0], a.y + sum[1]),
+                             ElemOps<T>::pack(b.x + sum[2], b.y + sum[3]));
+        }
+    }
+}
+
+// The same for the rows of a softmax warp.
+template <typename T>
+__device__ __forceinline__ void pm_restore_rows(const PromptParams& p, const PmWork* work) {
+    const PmWork it = *work;
+    const int warp = threadIdx.x >> 5, t = warp >> 2;
+    const int row = it.row0 + (p.G == 1 ? t * kPmTile : 0) + (warp & 3) * 32;
+    pm_restore<T>(p, it, p.G == 1 ? it.head0 : it.head0 + t, it.clear * kPmTile, row,
+                  min(row + 32, it.lq));
+}
+
+// Takes infinities and NaN out of the first `keys` rows of a V tile, and zeroes the
+// rows behind them; true if there was any to take out.  Whole warp.
+template <typename T>
+__device__ __forceinline__ bool pm_clean(uint8_t* tile, int keys) {
+    const int lane = threadIdx.x & 31;
+    // a lane's pieces of 16 bytes: of every fourth row, in both halves
+    constexpr int kPieces = kPmTile / 4;
+    uint4* const mine = reinterpret_cast<uint4*>(tile) + lane;
+    if (keys < kPmTile) {
+        for (int i = max(0, (keys - (lane >> 3) + 3) >> 2); i < kPieces; ++i)
+            mine[32 * i] = mine[32 * (kPieces + i)] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    // x * 0 is NaN for those and 0 for all others
+    typename ElemOps<T>::Pair none[4] = {};
+#pragma unroll 1
+    for (int i = 0; i < 2 * kPieces; i += 8) {
+        uint4 u[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) u[x] = mine[32 * (i + x)];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            none[0] = ElemOps<T>::zero_times(u[x].x, none[0]);
+            none[1] = ElemOps<T>::zero_times(u[x].y, none[1]);
+            none[2] = ElemOps<T>::zero_times(u[x].z, none[2]);
+            none[3] = ElemOps<T>::zero_times(u[x].w, none[3]);
+        }
+    }
+    const auto sum = __hadd2(__hadd2(none[0], none[1]), __hadd2(none[2], none[3]));
+    const bool found = __hisnan(sum.x) || __hisnan(sum.y);
+    if (!__any_sync(0xffffffffu, found)) return false;
+    if (found) {
+        auto finite = [](unsigned w) {
+            return ((w & 0x7fffu) >= kInf16<T> ? 0u : w & 0xffffu) |
+                   ((w >> 16 & 0x7fffu) >= kInf16<T> ? 0u : w & 0xffff0000u);
+        };
+        for (int i = 0; i < 2 * kPieces; ++i) {
+            const uint4 u = mine[32 * i];
+            mine[32 * i] = make_uint4(finite(u.x), finite(u.y), finite(u.z), finite(u.w));
+        }
+    }
+    return true;
+}
+
 // The cluster's parts of an item joined: softmax warp w of CTA `rank` takes every
 // n-th of its rows, lane l dims 4l .. 4l + 3, and reads the n CTAs' states through
 // their shared memory.
@@ -179,6 +298,9 @@ __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uin
     if (*(const volatile int*)&sh->work[0].row0 < 0 || *(const volatile int*)&sh->abort != 0) return;
     const PmWork it = sh->work[0];
     const int n = (int)cluster_size();
+    bool dropped = false;
+    for (int c = 0; c < n; ++c)
+        dropped = dropped || ld_cluster_u32(cluster_addr(smem_u32(&sh->dropped[0]), c)) != 0u;
     const uint32_t o_u32 = smem_u32(s_kv), st_u32 = smem_u32(s_state);
     for (int i = warp + kPmSoftmaxWarps * (int)cluster_rank(); i < it.n_tiles * kPmTile;
          i += kPmSoftmaxWarps * n) {
@@ -213,18 +335,16 @@ __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uin
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const size_t at = (size_t)(it.q0 + row) * p.Hq + head;
         T* out = reinterpret_cast<T*>(p.out) + at * kHeadDim;
-        const float worst = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, fmaf(o.w, 0.f, l * 0.f))));
-        if (__any_sync(0xffffffffu, worst != 0.f)) {
-            prompt_row<T>(p, p.q + (it.q0 + row) * p.q_tok + head * p.q_head,
-                          p.k + it.k0 * p.k_tok + it.kvh * p.k_head,
-                          p.v + it.k0 * p.v_tok + it.kvh * p.v_head, it.visible(row), out,
-                          p.lse != nullptr ? p.lse + at : nullptr, lane);
-            continue;
-        }
         reinterpret_cast<uint2*>(out)[lane] =
             make_uint2(ElemOps<T>::pack(o.x * inv, o.y * inv), ElemOps<T>::pack(o.z * inv, o.w * inv));
         if (lane == 0 && p.lse != nullptr)
-            p.lse[at] = l == 0.f ? -INFINITY : top * p.scale_log2 * kLn2 + logf(l);
+            p.lse[at] =
+                l == 0.f ? -INFINITY : (top * p.scale_log2 + kPmLift<T>) * kLn2 + logf(l);
+        if (dropped) {
+            __syncwarp();
+            pm_restore<T>(p, sh->work[0], head, it.visible(it.row0) / kPmTile * kPmTile, row,
+                          row + 1);
+        }
     }
 }
 
@@ -274,6 +394,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         for (int i = 0; i < kPmWorks; ++i) {
             mbar_init(&sh->work_full[i], 1);
             mbar_init(&sh->work_empty[i], kPmSoftmaxWarps + 2);  // one arrival per reading warp
+            sh->dropped[i] = 0;
         }
         mbar_init(&sh->launch_bar, 1);
         mbar_init(&sh->issued, 1);
@@ -288,6 +409,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             for (int i = 0; i < kPmParts; ++i) mbar_init(&sh->p_full[t][i], 4);  // the warps
             mbar_init(&sh->o_full[t], 1);
             mbar_init(&sh->o_empty[t], 4);
+            mbar_init(&sh->look[t], 1);
+            mbar_init(&sh->clean[t], 1);
         }
         mbar_init(&sh->drained, 1);
         sh->abort = 0;
@@ -304,11 +427,48 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         const int groups = p.G == 1 ? p.Hq : p.Hq / 2;  // fastest: they share keys in L2
         int item = kSplit ? blockIdx.x / cluster_size() : blockIdx.x;
         int seen = 0, before = 0;
-        uint32_t n = 0;  // items published
-        bool ok = true;
+        uint32_t n = 0;   // items published
+        uint32_t gb = 0;  // blocks of the items before
+        uint32_t looks[2] = {0u, 0u};  // V tiles looked over, per stage
+        bool ok = true, asked = false;
+        // V rows behind the last key belong to other sequences or to nobody and
+        // may hold anything, and so may the values of keys that a row does not
+        // see; their weights are 0, but 0 * NaN is not.  While the block's scores
+        // and weights are computed, this warp zeroes the rows behind the last
+        // key of block j's V tile and takes infinities and NaN out (pm_restore).
+        // 9 ragged prompts take 101 us with it and 99 with the rows behind the
+        // last key alone, 16384 tokens the same.
+        auto wait_copy = [&](int j) -> bool {  // started: the barrier is in its phase
+            const int x = (int)((gb + j) & 1u);  // V stage 1 or 3
+            return pm_wait_warp(p, sh, &sh->look[x], looks[x]++ & 1u);
+        };
+        auto clean = [&](const PmWork& w, int j) -> bool {
+            const int x = (int)((gb + j) & 1u);
+            if (!pm_wait_warp(p, sh, &sh->kv_full[2 * x + 1], ((gb + j) >> 1) & 1u)) return false;
+            if (pm_clean<T>(s_kv + (2 * x + 1) * kPmTileBytes,
+                            j + 1 == w.n_blocks ? w.tail : kPmTile) &&
+                lane == 0)
+                sh->dropped[(n - 1) % kPmWorks] = 1;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->clean[x]);
+            return true;
+        };
+        // The next item is asked for once the copies of this one's last blocks are
+        // under way: early enough that it is there when this one ends, late enough
+        // to be the fair one to take.
+        auto ask = [&]() {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sh->launch_bar, 16);
+                launch_cancel_async(&sh->launch, &sh->launch_bar);
+            }
+            __syncwarp();
+            asked = true;
+        };
         for (uint32_t round = 0; ok; ++round) {
             PmWork w;
             const int found = pm_find(p, item / groups, pm_rows_per_item(p.G), w, seen, before);
+            asked = false;
             if (found > 0) {  // (a bad sequence is reported by the checking warp)
                 pm_item<kSplit>(p, w, item % groups);
                 if (n >= (uint32_t)kPmWorks)
@@ -317,26 +477,31 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 if (!ok) break;
                 if (lane == 0) {
                     sh->work[n % kPmWorks] = w;
+                    sh->dropped[n % kPmWorks] = 0;
                     mbar_arrive(&sh->work_full[n % kPmWorks]);
                 }
                 __syncwarp();
                 ++n;
+                for (int j = w.clear; ok && j < w.n_blocks; ++j) {
+                    ok = wait_copy(j);
+                    if (!kSplit && ok && j + 1 == w.n_blocks) {
+                        ok = pm_wait_warp(p, sh, &sh->issued, (n - 1) & 1u);
+                        if (ok) ask();
+                    }
+                    ok = ok && clean(w, j);
+                }
+                gb += w.n_blocks;
                 if (kSplit) break;  // a cluster has one item
-                // The next item is asked for once the copies of this one's last
-                // blocks are under way: early enough that it is there when this
-                // one ends, late enough to be the fair one to take.
-                ok = pm_wait_warp(p, sh, &sh->issued, (n - 1) & 1u);
-                if (!ok) break;
+                if (ok && !asked) ok = pm_wait_warp(p, sh, &sh->issued, (n - 1) & 1u);
             }
             if (kSplit) break;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&sh->launch_bar, 16);
-                launch_cancel_async(&sh->launch, &sh->launch_bar);
-            }
-            __syncwarp();
+            if (ok && !asked) ask();
             // (the answer lands in this CTA: its wait heeds no abort)
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh->launch_bar, round & 1u, nullptr));
-            if (!ok && lane == 0 && atomicExch(&sh->abort, 1) == 0) raise_error(p.error, kErrTimeout);
+            if (asked &&
+                !__all_sync(0xffffffffu, mbar_wait_bounded(&sh->launch_bar, round & 1u, nullptr))) {
+                if (lane == 0 && atomicExch(&sh->abort, 1) == 0) raise_error(p.error, kErrTimeout);
+                ok = false;
+            }
             ok = ok && launch_cancelled(&sh->launch, item);
             fence_proxy_async_smem();  // read before the next answer is written
             __syncwarp();
@@ -399,6 +564,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     else
                         load(s_kv + st * kPmTileBytes, map_k, it.kvh, it.k0 + (it.first + (int)(c >> 1)) * kPmTile,
                              &sh->kv_full[st]);
+                    if ((c & 1) && (c >> 1) >= it.clear) mbar_arrive(&sh->look[st >> 1]);
                 }
                 mbar_arrive(&sh->issued);
             }
@@ -443,6 +609,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         uint32_t gb = 0;               // blocks of the items before
         uint32_t items = 0;            // items with keys
         uint32_t blocks[2] = {0u, 0u}, outs[2] = {0u, 0u};  // each tile's blocks and items
+        uint32_t cleaned[2] = {0u, 0u};  // V tiles looked over, per stage
         // Block j of the item; its K tile is in stage 0 or 2, V in the next: with
         // stages and tiles known at compile time every operand of a product is
         // a constant away from a loop invariant.
@@ -451,20 +618,13 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             constexpr int sk = decltype(odd)::value ? 0 : 2;
             const uint32_t g = gb + j;  // its V tile is number 2 g + 1 of the ring
             const bool more = j + 1 < it.n_blocks;
-            if (!pm_wait_warp(p, sh, &sh->kv_full[sv], (g >> 1) & 1u)) return false;
-            if (!more && it.tail < kPmTile) {
-                // Rows of V behind the last key belong to other sequences or to
-                // nobody and may hold anything; their weights are 0, and 0 * NaN
-                // is not: zero them (while the softmax is still at its weights).
-                uint8_t* tile = s_kv + sv * kPmTileBytes;
-                for (int x = it.tail * 8 + lane; x < kPmTile * 8; x += 32) {
-                    *reinterpret_cast<uint4*>(tile + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(tile + kPmHalfBytes + x * 16) =
-                        make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
+            // (a tile that is looked over has landed by then; one wait with either
+            // barrier: a second one cost 2 % of every block)
+            const bool looked = j >= it.clear;
+            if (!pm_wait_warp(p, sh, looked ? &sh->clean[sv >> 1] : &sh->kv_full[sv],
+                              (looked ? cleaned[sv >> 1] : g >> 1) & 1u))
+                return false;
+            cleaned[sv >> 1] += looked ? 1u : 0u;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (t >= it.n_tiles) break;
@@ -624,7 +784,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
+                const float base = m == -INFINITY ? 0.f : fmaf(m, p.scale_log2, kPmLift<T>);
                 const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
                 const uint64_t base2 = pack_f32x2(-base, -base);
                 uint64_t sum[2] = {0ull, 0ull};
@@ -664,7 +824,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (!kSplit && real && p.lse != nullptr)
                 p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
-                    l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l);
+                    l == 0.f ? -INFINITY : (m * p.scale_log2 + kPmLift<T>) * kLn2 + logf(l);
             if (it.n_blocks > 0) {
                 ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
                 if (!ok) break;
@@ -694,7 +854,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                 continue;  // (the item's place is not needed again)
             }
             const uint64_t inv2 = pack_f32x2(inv, inv);
-            uint64_t worst2[2] = {0ull, 0ull};  // NaN if any value is not finite
             // Through shared memory, 64 dims at a time, so that a warp stores 128
             // bytes of 4 rows at once: a thread writing its own row touches 32
             // lines an instruction, and the stores took longer than a block.
@@ -732,7 +891,6 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                         const uint64_t o2 = pack_f32x2(__uint_as_float(o[8 * i + 2 * x]),
                                                        __uint_as_float(o[8 * i + 2 * x + 1]));
                         float a, d;
-                        worst2[x & 1] = fma_f32x2(o2, 0ull, worst2[x & 1]);
                         unpack_f32x2(mul_f32x2(o2, inv2), a, d);
                         u[x] = ElemOps<T>::pack(a, d);
                     }
@@ -752,24 +910,10 @@ __global__ void __launch_bounds__(kPmThreads, 1)
                     if (4 * k + srow < rows) dst[k * step + 8 * c] = u[k];
                 __syncwarp();
             }
-            float bad[2];
-            unpack_f32x2(add_f32x2(worst2[0], worst2[1]), bad[0], bad[1]);
-            const float worst = bad[0] + bad[1];
-            // A value that is not finite may come from a key the row does not see
-            // (weight 0 times an infinite or NaN V): such a row is computed again
-            // from its own keys alone.
-            __syncwarp();
-            unsigned again = __ballot_sync(0xffffffffu, real && worst != 0.f);
-            while (again != 0u) {
-                const int i = __ffs(again) - 1;
-                again &= again - 1;
-                const int row = qrow - lane + i;  // of the sequence
-                const size_t to = (size_t)(it.q0 + row) * p.Hq + head;
-                prompt_row<T>(p, p.q + (it.q0 + row) * p.q_tok + head * p.q_head,
-                              p.k + it.k0 * p.k_tok + it.kvh * p.k_head,
-                              p.v + it.k0 * p.v_tok + it.kvh * p.v_head, it.visible(row),
-                              reinterpret_cast<T*>(p.out) + to * kHeadDim,
-                              p.lse != nullptr ? p.lse + to : nullptr, lane);
+            if (it.clear < it.n_blocks &&
+                *(const volatile int*)&sh->dropped[n % kPmWorks] != 0) {
+                __syncwarp();
+                pm_restore_rows<T>(p, &sh->work[n % kPmWorks]);
             }
             pm_release_work(sh, n);
         }

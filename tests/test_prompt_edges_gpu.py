@@ -6,10 +6,12 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import prompt_oracle as pr
 from persistentkv_attention_b200 import _native, ops
 from persistentkv_attention_b200.serving import DecodeEngine, PageStack
-from tests.test_prompt_gpu import (DT, check_block_write, check_decode, decode_case, empty_cache,
-                                   i32, no_error, run_decode, run_slots, slots_of)
+from tests.test_prompt_gpu import (DT, check_block_write, check_close, check_decode, check_lse,
+                                   check_prompt, decode_case, empty_cache, i32, no_error, packed,
+                                   run_decode, run_prompt, run_slots, slots_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -93,6 +95,117 @@ def test_decode_v_scales_all_small_or_large():
             continue
         back = (got.double() * 2.0 ** -power).to(torch.bfloat16)
         check_decode(back, q, kp, ks, vp, vs, table, lens, "bf16")
+
+
+# ------------------------------------------------------------------ values that are not finite
+def visible(row, cq, ck):
+    """(first key, end of keys) that a packed query row sees."""
+    b = int(np.searchsorted(cq, row, side="right")) - 1
+    return ck[b], max(ck[b], ck[b] + row - cq[b] + 1 + (ck[b + 1] - ck[b]) - (cq[b + 1] - cq[b]))
+
+
+def check_bad_values(lq, lk, hq, hkv, dtype, places, seed):
+    """V holds `places` (sequence, key, dim, value), by KV head alike: an output is
+    not finite where its row sees one, of the sign of those it sees, and every
+    other output is that of V without them."""
+    q, k, v, cq, ck = packed(lq, lk, hq, hkv, dtype, seed=seed, tail=3)
+    bad = v.clone()
+    v = v.clone()
+    bad[ck[-1]:] = float("nan")
+    for b, key, dim, value in places:
+        bad[ck[b] + key, :, dim] = value
+        v[ck[b] + key, :, dim] = 0.0
+    got, ls = run_prompt(q, k, bad, cq, ck)
+    want, lse, mag, size = pr.prompt_attention(q.double().numpy(), k.double().numpy(),
+                                               v.double().numpy(), cq, ck)
+    check_lse(ls, lse, size)
+    g = got.double().cpu().numpy()
+    for row in range(cq[-1]):
+        lo, hi = visible(row, np.asarray(cq), np.asarray(ck))
+        for dim in {d for _, _, d, _ in places}:
+            seen = {x for b, key, d, x in places if d == dim and lo <= ck[b] + key < hi}
+            if not seen:
+                continue
+            if len(seen) == 1 and seen <= {float("inf"), float("-inf")}:
+                # (a weight that the type rounds to zero makes a NaN of it)
+                ok = (g[row, :, dim] == seen.pop()) | np.isnan(g[row, :, dim])
+            else:
+                ok = np.isnan(g[row, :, dim])
+            assert ok.all()
+            want[row, :, dim] = np.nan
+    check_close(got, want, np.nan_to_num(mag), size, 1e3, dtype)
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (2, 2)])
+@pytest.mark.parametrize("lq,lk,places", [
+    ([300], [300], [(0, 0, 3, NAN)]),
+    ([300], [300], [(0, 0, 3, INF), (0, 130, 3, -INF), (0, 131, 9, INF), (0, 299, 0, NAN)]),
+    ([300, 200], [300, 200], [(0, 255, 1, INF), (0, 256, 2, -INF), (1, 127, 127, NAN),
+                              (1, 128, 64, INF), (1, 199, 65, -INF)]),
+    ([1], [77], [(0, 76, 5, INF), (0, 3, 6, NAN)]),
+    ([700, 9], [700, 140], [(0, 40 * i, 7 + i, INF) for i in range(17)] + [(1, 131, 0, NAN)]),
+    ([100], [300], [(0, 201, 3, INF), (0, 250, 3, INF), (0, 220, 4, NAN)]),
+    ([300], [40], [(0, 0, 1, INF), (0, 39, 2, NAN)]),
+    ([640], [640], [(0, 511, 11, INF), (0, 512, 12, -INF), (0, 639, 13, INF)])])
+def test_prompt_values_that_are_not_finite(lq, lk, places, hq, hkv, dtype):
+    check_bad_values(lq, lk, hq, hkv, dtype, places, seed=sum(lq))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (2, 2)])
+@pytest.mark.parametrize("lq,lk,places", [
+    ([6], [4500], [(0, 4495, 3, INF), (0, 4497, 3, -INF), (0, 4499, 4, NAN), (0, 100, 5, INF)]),
+    ([300], [4400], [(0, 4100, 3, INF), (0, 4101, 9, INF), (0, 4352, 3, -INF), (0, 4399, 4, NAN)]),
+    ([1], [4097], [(0, 4096, 0, INF), (0, 0, 1, -INF)]),
+    ([130, 2], [2100, 2051], [(0, 2047, 2, INF), (0, 2099, 3, NAN), (1, 2050, 4, INF)])])
+def test_prompt_split_values_that_are_not_finite(lq, lk, places, hq, hkv, dtype):
+    """The same where a cluster's CTAs share the keys."""
+    check_bad_values(lq, lk, hq, hkv, dtype, places, seed=sum(lk))
+
+
+@pytest.mark.parametrize("power", [-60, 60, 100, 112])
+def test_prompt_large_and_small_values(power):
+    """Values of bf16's range pass through 32-bit sums of weights of at most 1 (3000
+    values of 3 * 2^112: below 2^126): a common power of two of V is one of the
+    output."""
+    for lq, lk in (([300], [300]), ([5], [3000])):
+        q, k, v, cq, ck = packed(lq, lk, 4, 2, "bf16", seed=power, spread=3.0)
+        v = v.clamp(-3, 3)
+        got, ls = run_prompt(q, k, (v.double() * 2.0 ** power).to(torch.bfloat16), cq, ck)
+        back = (got.double() * 2.0 ** -power).to(torch.bfloat16)
+        check_prompt(q, k, v, cq, ck, "bf16", back, ls)
+
+
+def test_prompt_of_bad_values_takes_no_longer():
+    """One NaN at the first key, or nothing but NaN: the tensor cores still do the
+    work (a row computed on its own would take a hundred times as long)."""
+    n, hq, hkv = 4096, 8, 2
+    q, k, v, cq, _ = packed([n], [n], hq, hkv, "bf16", seed=1)
+    q, k, v, c = q.cuda(), k.cuda(), v.cuda(), i32(cq)
+    out = torch.empty_like(q)
+
+    def took(values):
+        times = []
+        for _ in range(4):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.prompt_attention(q, k, values, c, None, out)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    one, last, every = v.clone(), v.clone(), torch.full_like(v, NAN)
+    one[0, :, 5] = NAN
+    last[127::128] = INF
+    usual = took(v)
+    for values in (one, last, every):
+        assert took(values) < 10 * usual
+    no_error()
 
 
 # ------------------------------------------------------------------ nothing there
