@@ -410,6 +410,8 @@ class NativeEngine:
 
         from . import _native
 
+        if engine.kv8:
+            raise RuntimeError("the native host step serves 16-bit K/V caches")
         self._ct = ctypes
         self._lib = _native.load()
         self._check = _native.check

@@ -1,8 +1,11 @@
 """Host-side behaviour of the prompt entry points and the block-scaled decode at
 the edges of their contracts (no GPU, no kernel launch)."""
 
+from types import SimpleNamespace
+
 import pytest
 
+from persistentkv_attention_b200.serving import NativeEngine
 from tests.test_prompt_abi import decode, slots, write
 
 
@@ -81,3 +84,13 @@ def test_prefill_check(lib, scaled, kw, status, msg):
 def test_prefill_check_of_block_scales(lib, kw, status, msg):
     assert prefill(lib, **{**SCALED, **kw}) == status
     assert msg in lib.pkv_last_error_message().decode()
+
+
+# ------------------------------------------------------------------ native host step
+def test_native_step_refuses_e4m3_caches(monkeypatch):
+    """Its kernels would read an e4m3 pool as one of 16-bit values, past its end."""
+    from persistentkv_attention_b200 import _native
+
+    monkeypatch.setattr(_native, "load", lambda: pytest.fail("the library was reached"))
+    with pytest.raises(RuntimeError, match="16-bit K/V caches"):
+        NativeEngine(SimpleNamespace(kv8=True), 4, 8)
