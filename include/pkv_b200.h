@@ -371,7 +371,8 @@ pkv_status pkv_kv_write(const void* k, const void* v, void* k_pages, void* v_pag
  * pkv_prompt_slots places them.  A block's scale becomes the least power of two,
  * at least 2^-24, that brings the tokens' largest magnitude to 448 or below,
  * and at least the old scale if the first of them is not the block's first
- * token: the earlier tokens stay, moved to the new scale if it grew.  Values
+ * token: the earlier tokens stay, moved to the new scale if it grew (under an
+ * old scale of 0 they are zeros, whatever the codes).  Values
  * are rounded to nearest, ties to even.  Infinities and NaN do not set a
  * scale: the first are stored as +-448, the second as NaN.  Scales, pools and
  * tokens must not overlap. */

@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(kWriteThreads, 7)
                 const float ratio = old / scale;
                 for (int o = half; o < kept; o += 2) {
                     uint2* at = reinterpret_cast<uint2*>(block_base + (size_t)o * kHeadDim) + piece;
-                    uint2 c = *at;
+                    // (codes under a scale of 0 are zeros, whatever they hold)
+                    uint2 c = old == 0.f ? make_uint2(0u, 0u) : *at;
                     c.x = rescale_e4m3x2(c.x, ratio) | (rescale_e4m3x2(c.x >> 16, ratio) << 16);
                     c.y = rescale_e4m3x2(c.y, ratio) | (rescale_e4m3x2(c.y >> 16, ratio) << 16);
                     *at = c;

@@ -60,6 +60,25 @@ def test_block_write_of_blocks_of_odd_multiples(page, block, dtype):
         at += n
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_block_write_into_a_block_of_zeros(dtype):
+    """A block of scale 0 is zeros whatever its codes; a token that joins it leaves
+    the earlier ones zeros."""
+    kp, ks = empty_cache(2, 1, 32, 32)      # codes that are all NaN
+    vp, vs = empty_cache(2, 1, 32, 32)
+    ks.zero_(), vs.zero_()
+    x = torch.randn(3, 2, 128).to(DT[dtype]).cuda()
+    ops.kv_write_fp8_block(x[:, :1], x[:, 1:], kp, vp, ks, vs, i32([5, 6, 32 + 31]))
+    no_error()
+    for t, (p, s) in enumerate(((kp, ks), (vp, vs))):
+        got = pr.dequantised(p.view(torch.uint8).cpu().numpy(), s.cpu().numpy())[:, 0]
+        assert (got[0, :5] == 0).all() and (got[1, :31] == 0).all()
+        new = np.stack([got[0, 5], got[0, 6], got[1, 31]])
+        want = x[:, t].double().cpu().numpy()
+        # half a step of e4m3, or of its least value at a scale of at most 2^-6
+        assert (np.abs(new - want) <= 2.0 ** -4 * np.abs(want) + 2.0 ** -16).all()
+
+
 # ------------------------------------------------------------------ scales far apart
 @pytest.mark.parametrize("fused", [True, False])
 @pytest.mark.parametrize("far", [(100, None), (None, 100), (120, -24), (-24, 120), (90, -130, 3),
