@@ -111,9 +111,10 @@ __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, b
 // lines, bytes interleaved, eight output tiles.  No second pass over shared
 // memory and no transpose; that pass is what bounds the per-tensor route.
 // Bound: HBM, 256 bytes per token and KV head, for long batches (64 rows up to
-// 32768 tokens, 983 MB: 172 us, 5.7 TB/s; pages of 32 tokens 161 us, 6.1 TB/s);
-// for short ones the launch, the schedule, the first copies and the merge (one
-// row of 4096 tokens: 10.8 us, of which its bytes take 1.3).
+// 32768 tokens, 983 MB: 172 us, 5.7 TB/s; pages of 32 tokens 160 us, 6.1 TB/s; 168
+// and 157 without a reference of the sum's own); for short ones the launch, the
+// schedule, the first copies and the merge (one row of 4096 tokens: 11.1 us, of
+// which its bytes take 1.3).
 template <int G, typename T, int BOX, int NSLOTS>
 __global__ void __launch_bounds__(kB8Threads, PKV_MIN_CTAS_PER_SM)
     pkv_block8_kernel(const __grid_constant__ Block8Params bp,

@@ -306,11 +306,12 @@ constexpr int kRunRows = 16;  // tokens held in registers at a time
 // runs that start in it go to them in turn.  Long prompts start about one run
 // per window (one warp); the new tokens of a decode step are a run each, and
 // one warp would take them one after another (64 rows: 27.9 us; with a warp
-// each 4.5 us).  Lane l holds 16 bytes (8 elements) of tokens l / 16 + 2 i: 8 loads
-// in flight, 4 KB a warp, 28 warps an SM (72 registers; at 24 or 32 warps it took
-// 39 and 32 us where this takes 29.6).  Bound: issue slots and HBM for long
+// each 4.7 us).  Lane l holds 16 bytes (8 elements) of tokens l / 16 + 2 i: 8 loads
+// in flight, 4 KB a warp, 28 warps an SM (72 registers, 104 bytes of a thread spilled;
+// at 24 or 32 warps it took 39 and 32 us where this takes 30).  Bound: issue slots,
+// the spills and a shuffle per row for its slot among them, and HBM for long
 // prompts (2 bytes read, 1 written per element; 23k tokens of 8 heads, 143 MB:
-// 29.6 us, 4.8 TB/s), the chain slots -> tokens -> codes for short ones.
+// 30.0 us, 4.75 TB/s), the chain slots -> tokens -> codes for short ones.
 template <typename T>
 __global__ void __launch_bounds__(kWriteThreads, 7)
     pkv_kv_write_block_kernel(const __grid_constant__ WriteParams p) {

@@ -41,7 +41,7 @@ pkv_status check_strides(const char* name, int T, int H, long long* tok, long lo
 
 // Key blocks that a CTA of a split item gets at the least (prompt attention).  A
 // join costs about 8 us, a block 2: 16 queries over 8016 keys (32 heads) take
-// 114 us in one CTA per item and 47 in eight, 256 over 256 keys 12 and, in two, 21.
+// 114 us in one CTA per item and 51 in eight, 256 over 256 keys 11 and, in two, 21.
 constexpr int kPmSplitBlocks = 4;
 
 // Shared checks of the two writes; fills everything but the scales.
@@ -448,7 +448,8 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
     int sms = 0;
     st = device_state(&sms, &wp.error);
     if (st != PKV_OK) return st;
-    // up to a warp per token while the card has room for them (32 warps an SM)
+    // up to a warp per token while the grid has at most 32 warps an SM (28 of them
+    // are resident at a time)
     const long long windows = ((long long)T + kRunRows - 1) / kRunRows;
     wp.split_log2 = 0;
     while ((1 << wp.split_log2) < kRunRows &&

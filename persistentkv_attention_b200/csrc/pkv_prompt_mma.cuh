@@ -370,10 +370,10 @@ __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uin
 // without a workspace.
 //
 // Bound: the card's power cap, and a tile's chain scores -> softmax -> output.  One
-// prompt of 16384 tokens (32 heads, bf16) takes 2.03 ms, 1.08 PFLOP/s, 3750 cycles
+// prompt of 16384 tokens (32 heads, bf16) takes 2.05 ms, 1.07 PFLOP/s, 3750 cycles
 // per pair of tiles and block at 1.67 GHz under the cap; the products alone take
 // 2580, the exponentials 2050, and the tensor cores' nominal rate would be 2048.
-// An item's end costs 5500 cycles more: 9 prompts of 70 to 1487 tokens take 88 us.
+// An item's end costs 5500 cycles more: 9 prompts of 70 to 1487 tokens take 92 us.
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kPmThreads, 1)
     pkv_prompt_mma_kernel(const __grid_constant__ PromptParams p,
@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(kPmThreads, 1)
         // see; their weights are 0, but 0 * NaN is not.  While the block's scores
         // and weights are computed, this warp zeroes the rows behind the last
         // key of block j's V tile and takes infinities and NaN out (pm_restore).
-        // 9 ragged prompts take 101 us with it and 99 with the rows behind the
-        // last key alone, 16384 tokens the same.
+        // 9 ragged prompts take 92 us with it and 89 with the rows behind the last
+        // key alone, 16384 tokens the same.
         auto wait_copy = [&](int j) -> bool {  // started: the barrier is in its phase
             const int x = (int)((gb + j) & 1u);  // V stage 1 or 3
             return pm_wait_warp(p, sh, &sh->look[x], looks[x]++ & 1u);
