@@ -186,6 +186,49 @@ def test_prompt_split_values_that_are_not_finite(lq, lk, places, hq, hkv, dtype)
     check_bad_values(lq, lk, hq, hkv, dtype, places, seed=sum(lk))
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (3, 3)])
+def test_prompt_values_that_are_not_finite_among_many_items(hq, hkv):
+    """Several items a CTA, some of whose tiles hold such values: they stay with
+    their own rows."""
+    lens = [(37 * i) % 290 + 1 for i in range(330)]
+    places = [(b, (11 * b) % lens[b], b % 128, (INF, -INF, NAN)[b % 3])
+              for b in range(0, 330, 3) if b % 4]
+    check_bad_values(lens, lens, hq, hkv, "bf16", places, seed=3)
+
+
+def test_prompt_values_that_are_not_finite_in_a_graph():
+    """Replays over other values, and two calls at once, know nothing of one another."""
+    lens = [150, 129, 400]
+    q, k, v, cq, _ = packed(lens, lens, 4, 2, "f16", seed=8)
+    dq, dk, dv, c = q.cuda(), k.cuda(), v.cuda(), i32(cq)
+    want, _ = run_prompt(q, k, v, cq, None)
+    bad = dv.clone()
+    bad[cq[1] + 100, :, 7] = NAN
+    out = torch.zeros_like(dq)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.prompt_attention(dq, dk, dv, c, None, out)
+    clean = dv.clone()
+    for values in (bad, clean, bad):
+        dv.copy_(values)
+        graph.replay()
+        no_error()
+        is_nan = torch.zeros_like(out, dtype=torch.bool)
+        if values is bad:
+            is_nan[cq[1] + 100:cq[2], :, 7] = True
+        assert torch.equal(out.isnan(), is_nan) and torch.equal(out[~is_nan], want[~is_nan])
+    outs = [torch.zeros_like(out) for _ in range(12)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        with torch.cuda.stream(streams[i % 2]):
+            ops.prompt_attention(dq, dk, (bad, clean)[i % 2], c, None, o)
+    no_error()
+    for i, o in enumerate(outs):
+        keep = ~is_nan if i % 2 == 0 else torch.ones_like(is_nan)
+        assert torch.equal(o[keep], want[keep]) and (i % 2 or o.isnan().equal(is_nan))
+
+
 @pytest.mark.parametrize("power", [-60, 60, 100, 112])
 def test_prompt_large_and_small_values(power):
     """Values of bf16's range pass through 32-bit sums of weights of at most 1 (3000
