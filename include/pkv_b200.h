@@ -396,7 +396,7 @@ pkv_status pkv_kv_write_fp8_block(const void* k, const void* v, void* k_pages, v
  * does not see, whatever those hold.  An infinity or NaN among the V that a row
  * sees makes that dimension of its output one.  Sums of weights (at most 1)
  * times V are in 32 bits: bf16 values above 2^128 divided by the number of keys
- * may overflow.  A sequence whose ranges lie outside the tokens or run backwards
+ * may overflow, and ones below 2^-80 lose bits.  A sequence whose ranges lie outside the tokens or run backwards
  * is skipped and sets PKV_DEVERR_INDEX; the others' rows are computed only if
  * every range is in order. */
 pkv_status pkv_prompt_attention(const void* q, const void* k, const void* v,

@@ -51,6 +51,12 @@ template <typename T>
 constexpr float kPmLazy = std::is_same<T, __half>::value ? 14.0f : 32.0f;
 template <typename T>
 constexpr float kPmLift = std::is_same<T, __half>::value ? 0.0f : 32.0f;
+// 2^kPmLift: takes a sum of weights to the running maximum, exactly, so that its
+// logarithm is the small one.
+template <typename T>
+__device__ __forceinline__ float pm_unlift() {
+    return std::is_same<T, __half>::value ? 1.0f : 0x1p32f;
+}
 
 // One item of work: two query tiles that read the same keys.
 struct alignas(16) PmWork {
@@ -339,7 +345,7 @@ __device__ __forceinline__ void pm_join(const PromptParams& p, PmShared* sh, uin
             make_uint2(ElemOps<T>::pack(o.x * inv, o.y * inv), ElemOps<T>::pack(o.z * inv, o.w * inv));
         if (lane == 0 && p.lse != nullptr)
             p.lse[at] =
-                l == 0.f ? -INFINITY : (top * p.scale_log2 + kPmLift<T>) * kLn2 + logf(l);
+                l == 0.f ? -INFINITY : top * p.scale_log2 * kLn2 + logf(l * pm_unlift<T>());
         if (dropped) {
             __syncwarp();
             pm_restore<T>(p, sh->work[0], head, it.visible(it.row0) / kPmTile * kPmTile, row,
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(kPmThreads, 1)
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (!kSplit && real && p.lse != nullptr)
                 p.lse[(size_t)(it.q0 + qrow) * p.Hq + head] =
-                    l == 0.f ? -INFINITY : (m * p.scale_log2 + kPmLift<T>) * kLn2 + logf(l);
+                    l == 0.f ? -INFINITY : m * p.scale_log2 * kLn2 + logf(l * pm_unlift<T>());
             if (it.n_blocks > 0) {
                 ok = pm_wait_warp(p, sh, &sh->o_full[t], (blocks - 1) & 1u);
                 if (!ok) break;

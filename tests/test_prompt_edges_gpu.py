@@ -229,7 +229,7 @@ def test_prompt_values_that_are_not_finite_in_a_graph():
         assert torch.equal(o[keep], want[keep]) and (i % 2 or o.isnan().equal(is_nan))
 
 
-@pytest.mark.parametrize("power", [-60, 60, 100, 112])
+@pytest.mark.parametrize("power", [-78, -60, 60, 100, 112])
 def test_prompt_large_and_small_values(power):
     """Values of bf16's range pass through 32-bit sums of weights of at most 1 (3000
     values of 3 * 2^112: below 2^126): a common power of two of V is one of the
@@ -240,6 +240,17 @@ def test_prompt_large_and_small_values(power):
         got, ls = run_prompt(q, k, (v.double() * 2.0 ** power).to(torch.bfloat16), cq, ck)
         back = (got.double() * 2.0 ** -power).to(torch.bfloat16)
         check_prompt(q, k, v, cq, ck, "bf16", back, ls)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prompt_log_sums_are_exact_to_their_own_rounding(dtype):
+    """Scores of no size: the log-sum of n keys is ln n, up to the rounding of one
+    logarithm (2^-22 of it) and of sums of n ones."""
+    for lq, lk in ((300, 300), (3, 5000)):
+        q, k, v, cq, ck = packed([lq], [lk], 2, 1, dtype, seed=2)
+        _, ls = run_prompt(q, torch.zeros_like(k), v, cq, ck)
+        want = np.log(np.arange(lq) + 1.0 + lk - lq)[:, None]
+        assert (np.abs(ls.double().cpu().numpy() - want) <= 2.0 ** -22 * (want + 2)).all()
 
 
 def test_prompt_of_bad_values_takes_no_longer():
