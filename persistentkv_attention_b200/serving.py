@@ -279,7 +279,8 @@ class DecodeEngine:
         ``block_table`` [B, max_pages], or are in it already (None).  ``out`` gets
         the attention of each row over its own tokens, computed from the packed
         16-bit K/V.  A row that finds no pages (length 0 in the result) keeps
-        none of its K/V."""
+        none of its K/V.  Operands that the calls below would refuse are
+        refused before any page is taken."""
         if self.kv8 and self.kv_block_scales is None:
             raise RuntimeError("prefill writes 16-bit caches and e4m3 caches with block scales")
         b = block_table.size(0)
